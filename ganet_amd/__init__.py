@@ -9,6 +9,8 @@
                           the per-image formatting in tools/ganet/{tusimple,culane}/
                           test_dataset.py and tools/ganet/common.py)
   ganet_amd.lfa           the LFA tail: offsets -> DeformConv1D -> ReLU, fused
+  ganet_amd.norm          layer norm over channels (maps in both layouts, rows), with gradients
+  ganet_amd.optim         AdamW over many tensors (states in 32 or 8 bits), norm of all gradients
   ganet_amd.synth         seeded synthetic inputs of the hot path's shapes
 
 Everything computes in hand-written HIP kernels behind the C-ABI declared in
@@ -17,7 +19,7 @@ using an operator without the built library, or on CPU tensors, raises.
 """
 from . import _lib  # noqa: F401
 
-__all__ = ["dcn", "decode", "post_process", "formats", "lfa", "synth", "library_path"]
+__all__ = ["dcn", "decode", "post_process", "formats", "lfa", "norm", "optim", "synth", "library_path"]
 
 
 def library_path():

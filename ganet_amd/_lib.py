@@ -24,6 +24,8 @@ GANET_DCN_ALGO_KEEP_Y = 0x100
 GANET_DCN_BWD_OVERWRITE_X = 0x200
 DECODE_MAX_CENTERS = 2048
 DECODE_COUNT_STRIDE = 8
+GANET_LAYER_NORM_MAX_C = 16384
+GANET_STATE_BLOCK = 256
 
 EXPORTS = (
     "ganet_status_string", "ganet_abi_version", "ganet_dcn_out_size",
@@ -36,6 +38,9 @@ EXPORTS = (
     "ganet_decode_batch_noalloc", "ganet_decode_packed_workspace_bytes",
     "ganet_decode_batch_packed",
     "ganet_lanes_from_packed", "ganet_tusimple_from_lanes", "ganet_culane_text",
+    "ganet_layer_norm_forward", "ganet_layer_norm_backward",
+    "ganet_layer_norm_backward_workspace_bytes", "ganet_adamw_step",
+    "ganet_grad_norm", "ganet_grad_norm_workspace_bytes",
 )
 
 
@@ -68,6 +73,26 @@ class DecodeOut(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in (
         "counts", "centers_xy", "center_gid", "kpt_xy", "kpt_align", "kpt_root",
         "kpt_gid", "group_center", "group_count")]
+
+
+class LayerNormParams(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in (
+        "outer", "inner", "x_stride", "y_stride", "g_stride")] + [(n, ctypes.c_int32) for n in (
+            "C", "dtype", "weight_dtype")] + [("eps", ctypes.c_float)]
+
+
+class StepTensor(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "param", "grad", "exp_avg", "second", "exp_avg_scale", "second_scale", "master")] + [
+            ("n", ctypes.c_int64)]
+
+
+class AdamwParams(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "param_dtype", "grad_dtype", "state_bits", "skip_nonfinite")] + [
+            ("step", ctypes.c_int64), ("seed", ctypes.c_uint32), ("reserved", ctypes.c_uint32)] + [
+                (n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")] + [
+                    (n, ctypes.c_void_p) for n in ("grad_stats", "step_device", "lr_device")]
 
 
 class GanetError(RuntimeError):
@@ -165,6 +190,25 @@ def lib():
         L.ganet_culane_text.argtypes = [
             ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t,
             ctypes.c_void_p]
+        L.ganet_layer_norm_forward.restype = ctypes.c_int
+        L.ganet_layer_norm_forward.argtypes = [
+            ctypes.c_void_p] * 6 + [ctypes.POINTER(LayerNormParams), ctypes.c_void_p]
+        L.ganet_layer_norm_backward_workspace_bytes.restype = ctypes.c_size_t
+        L.ganet_layer_norm_backward_workspace_bytes.argtypes = [ctypes.POINTER(LayerNormParams)]
+        L.ganet_layer_norm_backward.restype = ctypes.c_int
+        L.ganet_layer_norm_backward.argtypes = [
+            ctypes.c_void_p] * 8 + [ctypes.POINTER(LayerNormParams), ctypes.c_void_p,
+                                    ctypes.c_size_t, ctypes.c_void_p]
+        # the tensor table: StepTensor rows, or the same words as an array of 64-bit integers
+        L.ganet_adamw_step.restype = ctypes.c_int
+        L.ganet_adamw_step.argtypes = [ctypes.c_void_p, ctypes.c_int,
+                                       ctypes.POINTER(AdamwParams), ctypes.c_void_p]
+        L.ganet_grad_norm_workspace_bytes.restype = ctypes.c_size_t
+        L.ganet_grad_norm_workspace_bytes.argtypes = [ctypes.c_void_p, ctypes.c_int]
+        L.ganet_grad_norm.restype = ctypes.c_int
+        L.ganet_grad_norm.argtypes = [
+            ctypes.c_void_p] * 3 + [ctypes.c_int, ctypes.c_double, ctypes.c_double] + [
+                ctypes.c_void_p] * 2 + [ctypes.c_size_t, ctypes.c_void_p]
         if L.ganet_abi_version() != 1:
             raise RuntimeError("ganet_amd: ABI version mismatch")
         _lib = L

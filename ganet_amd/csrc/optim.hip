@@ -1,0 +1,642 @@
+// AdamW over many tensors at once (states in 32 bits or in 8) and the norm of all gradients.
+//
+// Every operator here reads each value once, works a few tens of operations on it and writes it
+// back: HBM bounds them.  What is left to design is (a) that one launch serves many tensors of any
+// size, (b) that enough loads are in flight, (c) that nothing but the values moves.
+//
+// (a) The tensors' addresses travel in the kernel's arguments (no device table, no copy, nothing
+// that a captured graph would have to keep alive; argument blocks stay below 4 KiB, longer lists
+// take further launches).  A workgroup owns one chunk of one tensor; which one it finds by having
+// each lane compare one entry of the running chunk counts and counting the ballot.
+#include <math.h>
+
+#include "vec_device.h"
+
+namespace {
+
+using ganet_vec::bf16_t;
+using ganet_vec::f16_t;
+using ganet_vec::Vec;
+
+constexpr int kThreads = 256;
+
+// Which of the (at most 64) tensors of a launch a workgroup belongs to: `first` holds the number
+// of the first chunk of each, ascending.
+__device__ __forceinline__ int find_tensor(const int *first, int count, int chunk) {
+  const int lane = threadIdx.x & 63;
+  const unsigned long long below = __ballot(lane < count && first[lane < count ? lane : 0] <= chunk);
+  return __builtin_amdgcn_readfirstlane(__popcll(below) - 1);
+}
+
+// ---------------------------------------------------------------------------------------------
+// AdamW
+// ---------------------------------------------------------------------------------------------
+struct Hyper {
+  float b1, omb1, b2, omb2;     // betas and what is missing to 1 (formed in double)
+  float lr_c, rbc2, eps, decay; // lr / (1 - b1^t), 1 / sqrt(1 - b2^t), eps, 1 - lr * wd
+  float lr, wd, bc1, lnb1, lnb2;  // for the two pointers below
+  unsigned key;                 // of the random words: seed, and the step where the host has it
+  int skip;
+  const float *stats;           // [norm, coefficient, non-finite] or null
+  const long long *step;        // the step number on the device, or null
+  const float *lr_dev;
+};
+
+struct Coef {
+  float lr_c, rbc2, decay, gscale;
+  unsigned key;
+};
+
+// False: the step is to be left out.
+__device__ __forceinline__ bool coefficients(const Hyper &h, Coef &c) {
+  c.lr_c = h.lr_c;
+  c.rbc2 = h.rbc2;
+  c.decay = h.decay;
+  c.key = h.key;
+  c.gscale = 1.0f;
+  if (h.stats) {
+    if (h.skip && h.stats[2] != 0.0f) return false;
+    c.gscale = h.stats[1];
+  }
+  if (h.step || h.lr_dev) {
+    const float lr = h.lr_dev ? *h.lr_dev : h.lr;
+    float bc1 = h.bc1;
+    if (h.step) {
+      // 1 - b^t as -expm1(t ln b): ln b comes rounded from double, so the relative error of the
+      // whole stays at a few 2^-24 even where 1 - b^t is small
+      const long long t = *h.step;
+      bc1 = -expm1f((float)t * h.lnb1);
+      c.rbc2 = 1.0f / sqrtf(-expm1f((float)t * h.lnb2));
+      c.key = h.key + (unsigned)t * 0x9E3779B1u;
+    }
+    c.lr_c = lr / bc1;
+    c.decay = 1.0f - lr * h.wd;
+  }
+  return true;
+}
+
+constexpr int kTensors32 = 64;
+struct Args32 {
+  void *param[kTensors32];
+  const void *grad[kTensors32];
+  float *m[kTensors32];
+  float *v[kTensors32];
+  float *master[kTensors32];
+  long long n[kTensors32];
+  int first[kTensors32];
+  int count;
+  Hyper h;
+};
+static_assert(sizeof(Args32) <= 4096, "kernel arguments");
+
+constexpr int kVec32 = 4;       // values of a lane's vector
+constexpr int kUnroll32 = 4;    // vectors of a lane: 16 loads in flight
+constexpr int kChunk32 = kThreads * kVec32 * kUnroll32;
+
+template <typename TP, typename TG, bool MASTER>
+__global__ __launch_bounds__(kThreads) void adamw32_kernel(Args32 a) {
+  Coef c;
+  if (!coefficients(a.h, c)) return;
+  const int t = find_tensor(a.first, a.count, (int)blockIdx.x);
+  const long long at = (long long)((int)blockIdx.x - a.first[t]) * kChunk32;
+  const long long left = a.n[t] - at;
+  TP *p = (TP *)a.param[t] + at;
+  const TG *g = (const TG *)a.grad[t] + at;
+  float *m = a.m[t] + at, *v = a.v[t] + at;
+  float *w = MASTER ? a.master[t] + at : nullptr;
+
+  Vec<TP, kVec32> vp[kUnroll32];
+  Vec<TG, kVec32> vg[kUnroll32];
+  Vec<float, kVec32> vm[kUnroll32], vv[kUnroll32], vw[kUnroll32];
+#pragma unroll
+  for (int u = 0; u < kUnroll32; ++u) {
+    const int i = (u * kThreads + (int)threadIdx.x) * kVec32;
+    if (i < left) {
+      vg[u].load(g + i, left - i);
+      vm[u].load(m + i, left - i);
+      vv[u].load(v + i, left - i);
+      if constexpr (MASTER)
+        vw[u].load(w + i, left - i);
+      else
+        vp[u].load(p + i, left - i);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll32; ++u) {
+    const int i = (u * kThreads + (int)threadIdx.x) * kVec32;
+    if (i >= left) continue;
+#pragma unroll
+    for (int k = 0; k < kVec32; ++k) {
+      const float gr = vg[u].get(k) * c.gscale;
+      const float mm = a.h.b1 * vm[u].get(k) + a.h.omb1 * gr;
+      const float sq = a.h.b2 * vv[u].get(k) + a.h.omb2 * (gr * gr);
+      const float old = MASTER ? vw[u].get(k) : vp[u].get(k);
+      const float now = old * c.decay - c.lr_c * (mm / (sqrtf(sq) * c.rbc2 + a.h.eps));
+      vm[u].set(k, mm);
+      vv[u].set(k, sq);
+      if constexpr (MASTER) vw[u].set(k, now);
+      vp[u].set(k, now);   // 16-bit weights: rounded once, to nearest
+    }
+    vm[u].store(m + i, left - i);
+    vv[u].store(v + i, left - i);
+    if constexpr (MASTER) vw[u].store(w + i, left - i);
+    vp[u].store(p + i, left - i);
+  }
+}
+
+// ---- states in 8 bits -------------------------------------------------------------------------
+// m and r = sqrt(v) are held as e4m3 times one float32 scale for each 256 consecutive values of a
+// tensor (scale = the block's largest magnitude / 448).  r and not v: e4m3 spans 2^18, so v spans
+// 2^36, and the step divides by r.  Both are rounded up or down at random, with the probability
+// that keeps the mean: with beta2 = 0.999 an average moves by a thousandth a step, far less than
+// half of e4m3's spacing (2^-4), and rounding to nearest would stop it for good.  An r above zero
+// never becomes zero (m over a zero r would be a step of m / eps).
+constexpr int kBlock = GANET_STATE_BLOCK;
+constexpr int kTensors8 = 56;
+struct Args8 {
+  void *param[kTensors8];
+  const void *grad[kTensors8];
+  unsigned char *m[kTensors8];
+  unsigned char *r[kTensors8];
+  float *ms[kTensors8];
+  float *rs[kTensors8];
+  float *master[kTensors8];
+  long long n[kTensors8];
+  int first[kTensors8];
+  int count, tensor0;          // the first tensor's place in the whole list
+  Hyper h;
+};
+static_assert(sizeof(Args8) <= 4096, "kernel arguments");
+
+constexpr int kVec8 = 8;                            // values of a lane: 32 lanes hold a block
+constexpr int kUnroll8 = 2;
+constexpr int kChunk8 = kThreads * kVec8 * kUnroll8; // a whole number of blocks
+
+__device__ __forceinline__ unsigned mix32(unsigned x) {
+  x ^= x >> 16;
+  x *= 0xBB67AE85u;
+  x ^= x >> 15;
+  x *= 0x6A09E667u;
+  return x ^ (x >> 16);
+}
+
+// e4m3 bits of a (0 <= a <= 448), up or down by the 16 random bits.  float32's dropped 20 bits of
+// mantissa plus a random 20-bit number carry into the kept ones with the right probability; below
+// 2^-6, where e4m3 is evenly spaced by 2^-9, a + 2^-6 has that same spacing.
+__device__ __forceinline__ unsigned sr_e4m3(float a, unsigned r16) {
+  const bool small = a < 0x1p-6f;
+  const float y = small ? a + 0x1p-6f : a;
+  return ((__float_as_uint(y) + (r16 << 4) + 8u) >> 20) - (small ? 968u : 960u);
+}
+
+template <typename TP, typename TG, bool MASTER>
+__global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8 a) {
+  Coef c;
+  if (!coefficients(a.h, c)) return;
+  const int t = find_tensor(a.first, a.count, (int)blockIdx.x);
+  const long long at = (long long)((int)blockIdx.x - a.first[t]) * kChunk8;
+  const long long left = a.n[t] - at;
+  TP *p = (TP *)a.param[t] + at;
+  const TG *g = (const TG *)a.grad[t] + at;
+  unsigned char *m = a.m[t] + at, *r = a.r[t] + at;
+  const long long block0 = at / kBlock;
+  float *ms = a.ms[t] + block0, *rs = a.rs[t] + block0;
+  float *w = MASTER ? a.master[t] + at : nullptr;
+  const unsigned key = mix32(c.key + (unsigned)(a.tensor0 + t) * 0x85EBCA6Bu);
+  typedef unsigned char Byte8 __attribute__((ext_vector_type(8), aligned(1)));
+
+  Vec<TP, kVec8> vp[kUnroll8];
+  Vec<TG, kVec8> vg[kUnroll8];
+  Vec<float, kVec8> vw[kUnroll8];
+  unsigned vm[kUnroll8][2], vr[kUnroll8][2];
+  float sm[kUnroll8], sr[kUnroll8];
+#pragma unroll
+  for (int u = 0; u < kUnroll8; ++u) {
+    const int i = (u * kThreads + (int)threadIdx.x) * kVec8;
+    const long long k = left - i;
+    vm[u][0] = vm[u][1] = vr[u][0] = vr[u][1] = 0;
+    sm[u] = sr[u] = 0.0f;
+    vg[u].zero();
+    if (k <= 0) continue;
+    vg[u].load(g + i, k);
+    if constexpr (MASTER)
+      vw[u].load(w + i, k);
+    else
+      vp[u].load(p + i, k);
+    sm[u] = ((const GANET_GLOBAL float *)ms)[i / kBlock];
+    sr[u] = ((const GANET_GLOBAL float *)rs)[i / kBlock];
+    if (k >= kVec8) {
+      const Byte8 bm = *(const GANET_GLOBAL Byte8 *)(m + i);
+      const Byte8 br = *(const GANET_GLOBAL Byte8 *)(r + i);
+      const unsigned long long wm = __builtin_bit_cast(unsigned long long, bm);
+      const unsigned long long wr = __builtin_bit_cast(unsigned long long, br);
+      vm[u][0] = (unsigned)wm;
+      vm[u][1] = (unsigned)(wm >> 32);
+      vr[u][0] = (unsigned)wr;
+      vr[u][1] = (unsigned)(wr >> 32);
+    } else {
+      for (int j = 0; j < (int)k; ++j) {
+        vm[u][j >> 2] |= (unsigned)m[i + j] << (8 * (j & 3));
+        vr[u][j >> 2] |= (unsigned)r[i + j] << (8 * (j & 3));
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll8; ++u) {
+    const int i = (u * kThreads + (int)threadIdx.x) * kVec8;
+    const long long k = left - i;
+    float nm[kVec8], nr[kVec8];
+    float tm = 0.0f, tr = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kVec8; j += 2) {
+      const auto m2 = (j & 2) ? __builtin_amdgcn_cvt_pk_f32_fp8(vm[u][j >> 2], true)
+                              : __builtin_amdgcn_cvt_pk_f32_fp8(vm[u][j >> 2], false);
+      const auto r2 = (j & 2) ? __builtin_amdgcn_cvt_pk_f32_fp8(vr[u][j >> 2], true)
+                              : __builtin_amdgcn_cvt_pk_f32_fp8(vr[u][j >> 2], false);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float gr = vg[u].get(j + e) * c.gscale;
+        const float mm = a.h.b1 * (m2[e] * sm[u]) + a.h.omb1 * gr;
+        const float rr = r2[e] * sr[u];
+        const float root = sqrtf(a.h.b2 * (rr * rr) + a.h.omb2 * (gr * gr));
+        nm[j + e] = mm;
+        nr[j + e] = root;
+        tm = fmaxf(tm, fabsf(mm));
+        tr = fmaxf(tr, root);
+      }
+    }
+    tm = ganet_vec::group_max<32>(tm);
+    tr = ganet_vec::group_max<32>(tr);
+    // A gradient that is not finite reaches its own value only: it is left out of the scale (NaN
+    // already is) and becomes e4m3's NaN.
+    if (tm == INFINITY || tr == INFINITY) {
+      tm = tr = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kVec8; ++j) {
+        if (fabsf(nm[j]) < INFINITY) tm = fmaxf(tm, fabsf(nm[j]));
+        if (nr[j] < INFINITY) tr = fmaxf(tr, nr[j]);
+      }
+      tm = ganet_vec::group_max<32>(tm);
+      tr = ganet_vec::group_max<32>(tr);
+    }
+    if (tm < 0x1p-110f) tm = 0.0f;      // 448 / tm would overflow: such a block is held as zeros
+    const float im = tm > 0.0f ? 448.0f / tm : 0.0f;
+    const float ir = tr > 0.0f ? 448.0f / tr : 0.0f;
+    if (k <= 0) continue;               // uniform over a block's lanes but for the last block
+    const unsigned at_block = (unsigned)(block0 + i / kBlock);
+    const unsigned bkey = mix32(key + at_block * 0xC2B2AE35u);
+    unsigned om[2] = {0, 0}, orr[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < kVec8; ++j) {
+      unsigned h = bkey + (unsigned)((i + j) % kBlock) * 0x9E3779B1u;
+      h ^= h >> 16;
+      h *= 0xBB67AE85u;
+      h ^= h >> 15;
+      unsigned cm = sr_e4m3(fminf(fabsf(nm[j]) * im, 448.0f), h & 0xFFFFu);
+      unsigned cr = sr_e4m3(fminf(nr[j] * ir, 448.0f), h >> 16);
+      if (nr[j] > 0.0f && cr < 1u) cr = 1u;
+      if (!(fabsf(nm[j]) < INFINITY)) cm = 0x7Fu;
+      if (!(nr[j] < INFINITY)) cr = 0x7Fu;
+      cm |= (__float_as_uint(nm[j]) >> 24) & 0x80u;
+      om[j >> 2] |= cm << (8 * (j & 3));
+      orr[j >> 2] |= cr << (8 * (j & 3));
+      const float old = MASTER ? vw[u].get(j) : vp[u].get(j);
+      const float now = old * c.decay - c.lr_c * (nm[j] / (nr[j] * c.rbc2 + a.h.eps));
+      if constexpr (MASTER) vw[u].set(j, now);
+      vp[u].set(j, now);
+    }
+    if constexpr (MASTER) vw[u].store(w + i, k);
+    vp[u].store(p + i, k);
+    if (k >= kVec8) {
+      *(GANET_GLOBAL Byte8 *)(m + i) =
+          __builtin_bit_cast(Byte8, (unsigned long long)om[0] | (unsigned long long)om[1] << 32);
+      *(GANET_GLOBAL Byte8 *)(r + i) =
+          __builtin_bit_cast(Byte8, (unsigned long long)orr[0] | (unsigned long long)orr[1] << 32);
+    } else {
+      for (int j = 0; j < (int)k; ++j) {
+        m[i + j] = (unsigned char)(om[j >> 2] >> (8 * (j & 3)));
+        r[i + j] = (unsigned char)(orr[j >> 2] >> (8 * (j & 3)));
+      }
+    }
+    if (i % kBlock == 0) {
+      ((GANET_GLOBAL float *)ms)[i / kBlock] = tm / 448.0f;
+      ((GANET_GLOBAL float *)rs)[i / kBlock] = tr / 448.0f;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// The norm of all gradients
+// ---------------------------------------------------------------------------------------------
+// Squares are summed in float64: float32 would overflow at |g| = 1.8e19 and lose the small
+// gradients of a long sum, and the conversion and the addition hide behind the loads.  Each
+// workgroup leaves one partial sum, a second launch adds them in their order: the same inputs give
+// the same bits.
+constexpr int kTensorsN = 128;
+struct ArgsN {
+  const void *grad[kTensorsN];
+  long long n[kTensorsN];
+  int first[kTensorsN];
+  unsigned char dtype[kTensorsN];
+  int count;
+  long long chunk;
+  double *partial;
+};
+static_assert(sizeof(ArgsN) <= 4096, "kernel arguments");
+constexpr int kUnrollN = 4;
+
+template <typename T, int N>
+__device__ __forceinline__ double sum_squares(const T *g, long long n) {
+  double s[kUnrollN] = {0, 0, 0, 0};
+  long long i = (long long)threadIdx.x * N;
+  constexpr long long step = (long long)kThreads * N;
+  for (; i + (kUnrollN - 1) * step + N <= n; i += kUnrollN * step) {
+    Vec<T, N> v[kUnrollN];
+#pragma unroll
+    for (int u = 0; u < kUnrollN; ++u) v[u].load(g + i + u * step);
+#pragma unroll
+    for (int u = 0; u < kUnrollN; ++u)
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const double d = (double)v[u].get(k);
+        s[u] = fma(d, d, s[u]);
+      }
+  }
+  for (; i < n; i += step) {
+    Vec<T, N> v;
+    v.load(g + i, n - i);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const double d = (double)v.get(k);
+      s[0] = fma(d, d, s[0]);
+    }
+  }
+  return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+__global__ __launch_bounds__(kThreads) void grad_norm_kernel(ArgsN a) {
+  const int lane = threadIdx.x & 63;
+  int t = find_tensor(a.first, a.count < 64 ? a.count : 64, (int)blockIdx.x);
+  if (a.count > 64) {
+    const unsigned long long below =
+        __ballot(lane + 64 < a.count && a.first[lane + 64 < a.count ? lane + 64 : 0] <= (int)blockIdx.x);
+    t = __builtin_amdgcn_readfirstlane(t + __popcll(below));
+  }
+  const long long at = (long long)((int)blockIdx.x - a.first[t]) * a.chunk;
+  const long long n = a.n[t] - at < a.chunk ? a.n[t] - at : a.chunk;
+  double s;
+  if (a.dtype[t] == GANET_F32)
+    s = sum_squares<float, 4>((const float *)a.grad[t] + at, n);
+  else if (a.dtype[t] == GANET_BF16)
+    s = sum_squares<bf16_t, 8>((const bf16_t *)a.grad[t] + at, n);
+  else
+    s = sum_squares<f16_t, 8>((const f16_t *)a.grad[t] + at, n);
+  __shared__ double part[kThreads / 64];
+  s = wave_sum(s);
+  if (lane == 0) part[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double all = 0.0;
+    for (int w = 0; w < kThreads / 64; ++w) all += part[w];
+    a.partial[blockIdx.x] = all;
+  }
+}
+
+constexpr int kFinish = 1024;
+__global__ __launch_bounds__(kFinish) void grad_norm_finish_kernel(const double *partial, long long n,
+                                                                   double max_norm, double inv_scale,
+                                                                   float *stats) {
+  double s = 0.0;
+  for (long long i = threadIdx.x; i < n; i += kFinish) s += partial[i];
+  s = wave_sum(s);
+  __shared__ double part[kFinish / 64];
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double all = 0.0;
+    for (int w = 0; w < kFinish / 64; ++w) all += part[w];
+    const double norm = sqrt(all) * fabs(inv_scale);
+    const bool fine = (float)norm < INFINITY;       // false for NaN too
+    const double clip = max_norm / (norm + 1e-6);
+    stats[0] = (float)norm;
+    stats[1] = fine ? (float)(inv_scale * (clip < 1.0 ? clip : 1.0)) : 0.0f;
+    stats[2] = fine ? 0.0f : 1.0f;
+    stats[3] = 0.0f;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------
+constexpr long long kMostValues = 1ll << 40;      // of one tensor: no sum below overflows
+constexpr long long kMostBlocks = 1ll << 23;      // of one launch: its threads stay below 2^32
+
+bool dtype_ok(int d) { return d == GANET_F32 || d == GANET_BF16 || d == GANET_F16; }
+
+template <typename F>
+int with_types(int pd, int gd, bool master, F &&f) {
+  auto grad = [&](auto p, auto m) {
+    typedef decltype(p) TP;
+    if (gd == GANET_F32) return f(TP(), float(), m);
+    if (gd == GANET_BF16) return f(TP(), bf16_t(), m);
+    return f(TP(), f16_t(), m);
+  };
+  if (pd == GANET_F32) return grad(float(), std::false_type());
+  if (pd == GANET_BF16)
+    return master ? grad(bf16_t(), std::true_type()) : grad(bf16_t(), std::false_type());
+  return master ? grad(f16_t(), std::true_type()) : grad(f16_t(), std::false_type());
+}
+
+// Takes the list in launches of at most `most` tensors; chunk numbers into args.first.  A tensor
+// without values keeps its place and gets no chunk (its successor starts at the same number, and a
+// workgroup takes the last tensor that starts at or before its own).
+template <typename Args, typename Fill, typename Launch>
+int in_launches(const ganet_step_tensor *ts, int count, int most, long long chunk, Args &args, Fill &&fill,
+                Launch &&launch) {
+  int i = 0;
+  while (i < count) {
+    int k = 0;
+    long long blocks = 0;
+    for (; i < count && k < most; ++i, ++k) {
+      const long long need = (ts[i].n + chunk - 1) / chunk;
+      if (need > kMostBlocks) return GANET_ERR_UNSUPPORTED;
+      if (blocks + need > kMostBlocks) break;
+      args.first[k] = (int)blocks;
+      fill(k, ts[i], i);
+      blocks += need;
+    }
+    if (blocks == 0) continue;
+    args.count = k;
+    const int rc = launch((unsigned)blocks);
+    if (rc != GANET_OK) return rc;
+  }
+  return GANET_OK;
+}
+
+}  // namespace
+
+extern "C" int ganet_adamw_step(const ganet_step_tensor *tensors, int count, const ganet_adamw_params *p,
+                                ganet_stream_t stream) {
+  if (!p || (count > 0 && !tensors)) return GANET_ERR_NULL;
+  if (count < 0 || !dtype_ok(p->param_dtype) || !dtype_ok(p->grad_dtype) ||
+      (p->state_bits != 32 && p->state_bits != 8) || p->reserved != 0)
+    return GANET_ERR_BAD_SHAPE;
+  if (!(p->lr >= 0.0) || !(p->beta1 >= 0.0 && p->beta1 < 1.0) || !(p->beta2 >= 0.0 && p->beta2 < 1.0) ||
+      !(p->eps >= 0.0) || !(p->weight_decay >= 0.0) || isinf(p->lr) || isinf(p->eps) || isinf(p->weight_decay))
+    return GANET_ERR_BAD_SHAPE;
+  if (!p->step_device && p->step < 1) return GANET_ERR_BAD_SHAPE;
+  const bool small = p->state_bits == 8;
+  bool master = false, any = false;
+  for (int i = 0; i < count; ++i) {
+    const ganet_step_tensor &t = tensors[i];
+    if (t.n < 0 || t.n > kMostValues) return GANET_ERR_BAD_SHAPE;
+    if (t.n == 0) continue;            // has no addresses
+    if (!any) master = t.master != nullptr;
+    any = true;
+    if ((t.master != nullptr) != master) return GANET_ERR_BAD_SHAPE;
+    if (!t.param || !t.grad || !t.exp_avg || !t.second) return GANET_ERR_NULL;
+    if (small && (!t.exp_avg_scale || !t.second_scale)) return GANET_ERR_NULL;
+  }
+  if (master && p->param_dtype == GANET_F32) return GANET_ERR_BAD_SHAPE;
+
+  Hyper h;
+  h.b1 = (float)p->beta1;
+  h.omb1 = (float)(1.0 - p->beta1);
+  h.b2 = (float)p->beta2;
+  h.omb2 = (float)(1.0 - p->beta2);
+  const double t = p->step_device ? 1.0 : (double)p->step;
+  const double bc1 = p->beta1 > 0 ? -expm1(t * log(p->beta1)) : 1.0;
+  const double bc2 = p->beta2 > 0 ? -expm1(t * log(p->beta2)) : 1.0;
+  h.lr_c = (float)(p->lr / bc1);
+  h.rbc2 = (float)(1.0 / sqrt(bc2));
+  h.eps = (float)p->eps;
+  h.decay = (float)(1.0 - p->lr * p->weight_decay);
+  h.lr = (float)p->lr;
+  h.wd = (float)p->weight_decay;
+  h.bc1 = (float)bc1;
+  h.lnb1 = (float)log(p->beta1);      // -inf for 0: 1 - exp(-inf) = 1
+  h.lnb2 = (float)log(p->beta2);
+  h.key = p->seed + (p->step_device ? 0u : (unsigned)p->step * 0x9E3779B1u);
+  h.skip = p->skip_nonfinite != 0;
+  h.stats = p->grad_stats;
+  h.step = (const long long *)p->step_device;
+  h.lr_dev = p->lr_device;
+
+  hipStream_t s = (hipStream_t)stream;
+  if (!small) {
+    Args32 a;
+    a.h = h;
+    return in_launches(
+        tensors, count, kTensors32, kChunk32, a,
+        [&](int k, const ganet_step_tensor &x, int) {
+          a.param[k] = x.param;
+          a.grad[k] = x.grad;
+          a.m[k] = (float *)x.exp_avg;
+          a.v[k] = (float *)x.second;
+          a.master[k] = x.master;
+          a.n[k] = x.n;
+        },
+        [&](unsigned blocks) {
+          return with_types(p->param_dtype, p->grad_dtype, master, [&](auto tp, auto tg, auto tm) {
+            adamw32_kernel<decltype(tp), decltype(tg), decltype(tm)::value>
+                <<<dim3(blocks), dim3(kThreads), 0, s>>>(a);
+            return ganet_check_launch();
+          });
+        });
+  }
+  Args8 a;
+  a.h = h;
+  return in_launches(
+      tensors, count, kTensors8, kChunk8, a,
+      [&](int k, const ganet_step_tensor &x, int i) {
+        if (k == 0) a.tensor0 = i;
+        a.param[k] = x.param;
+        a.grad[k] = x.grad;
+        a.m[k] = (unsigned char *)x.exp_avg;
+        a.r[k] = (unsigned char *)x.second;
+        a.ms[k] = x.exp_avg_scale;
+        a.rs[k] = x.second_scale;
+        a.master[k] = x.master;
+        a.n[k] = x.n;
+      },
+      [&](unsigned blocks) {
+        return with_types(p->param_dtype, p->grad_dtype, master, [&](auto tp, auto tg, auto tm) {
+          adamw8_kernel<decltype(tp), decltype(tg), decltype(tm)::value>
+              <<<dim3(blocks), dim3(kThreads), 0, s>>>(a);
+          return ganet_check_launch();
+        });
+      });
+}
+
+// ---- norm ----
+namespace {
+// Values of a workgroup: one round of 2048 workgroups (8 on each of 256 CUs) for long lists, 8192
+// (8 float32 vectors a thread) at least.
+long long norm_chunk(const int64_t *numel, int count) {
+  long long total = 0;
+  for (int i = 0; i < count; ++i) total += numel[i];
+  const long long unit = 8192;
+  const long long even = (total + 2047) / 2048;
+  return even <= unit ? unit : (even + unit - 1) / unit * unit;
+}
+int norm_list_ok(const int64_t *numel, int count) {
+  if (count < 0 || count > (1 << 20)) return GANET_ERR_BAD_SHAPE;
+  if (count > 0 && !numel) return GANET_ERR_NULL;
+  for (int i = 0; i < count; ++i)
+    if (numel[i] < 0 || numel[i] > kMostValues) return GANET_ERR_BAD_SHAPE;
+  return GANET_OK;
+}
+}  // namespace
+
+extern "C" size_t ganet_grad_norm_workspace_bytes(const int64_t *numel, int count) {
+  if (norm_list_ok(numel, count) != GANET_OK) return 0;
+  const long long chunk = norm_chunk(numel, count);
+  long long blocks = 0;
+  for (int i = 0; i < count; ++i) blocks += (numel[i] + chunk - 1) / chunk;
+  return ganet_align_up((size_t)(blocks + 1) * sizeof(double), 256);
+}
+
+extern "C" int ganet_grad_norm(const void *const *grads, const int64_t *numel, const int32_t *dtypes, int count,
+                               double max_norm, double inv_scale, float *stats, void *workspace,
+                               size_t workspace_bytes, ganet_stream_t stream) {
+  const int bad = norm_list_ok(numel, count);
+  if (bad != GANET_OK) return bad;
+  if (!stats || !workspace || (count > 0 && (!grads || !dtypes))) return GANET_ERR_NULL;
+  if (!(max_norm >= 0.0) || !(fabs(inv_scale) < INFINITY)) return GANET_ERR_BAD_SHAPE;
+  for (int i = 0; i < count; ++i) {
+    if (!dtype_ok(dtypes[i])) return GANET_ERR_BAD_SHAPE;
+    if (numel[i] > 0 && !grads[i]) return GANET_ERR_NULL;
+  }
+  if (workspace_bytes < ganet_grad_norm_workspace_bytes(numel, count)) return GANET_ERR_WORKSPACE;
+  hipStream_t s = (hipStream_t)stream;
+  ArgsN a;
+  a.chunk = norm_chunk(numel, count);
+  long long done = 0;
+  for (int i = 0; i < count;) {
+    int k = 0;
+    long long blocks = 0;
+    for (; i < count && k < kTensorsN; ++i, ++k) {     // at most 2048 chunks beside one a tensor
+      a.grad[k] = grads[i];
+      a.n[k] = numel[i];
+      a.dtype[k] = (unsigned char)dtypes[i];
+      a.first[k] = (int)blocks;
+      blocks += (numel[i] + a.chunk - 1) / a.chunk;
+    }
+    if (blocks == 0) continue;
+    a.count = k;
+    a.partial = (double *)workspace + done;
+    grad_norm_kernel<<<dim3((unsigned)blocks), dim3(kThreads), 0, s>>>(a);
+    const int rc = ganet_check_launch();
+    if (rc != GANET_OK) return rc;
+    done += blocks;
+  }
+  grad_norm_finish_kernel<<<dim3(1), dim3(kFinish), 0, s>>>((const double *)workspace, done, max_norm, inv_scale,
+                                                          stats);
+  return ganet_check_launch();
+}

@@ -1,0 +1,116 @@
+// Device-side loads, stores and reductions shared by the training operators
+// (csrc/layer_norm.hip, csrc/optim.hip).  Internal, not part of the public ABI.
+#pragma once
+
+#include "dcn_device.h"
+
+namespace ganet_vec {
+
+using ganet_dcn::bf16_t;
+using ganet_dcn::f16_t;
+
+// What a value of T is to the vector types (bf16 travels as its 16 bits).
+template <typename T>
+struct Elem;
+template <>
+struct Elem<float> {
+  typedef float type;
+  __device__ static __forceinline__ float widen(float e) { return e; }
+  __device__ static __forceinline__ float narrow(float f) { return f; }
+};
+template <>
+struct Elem<f16_t> {
+  typedef _Float16 type;
+  __device__ static __forceinline__ float widen(_Float16 e) { return (float)e; }
+  __device__ static __forceinline__ _Float16 narrow(float f) { return (_Float16)f; }
+};
+template <>
+struct Elem<bf16_t> {
+  typedef unsigned short type;
+  __device__ static __forceinline__ float widen(unsigned short e) {
+    return __uint_as_float((unsigned)e << 16);
+  }
+  __device__ static __forceinline__ unsigned short narrow(float f) {
+    return ganet_dcn::from_f32<bf16_t>(f).v;
+  }
+};
+
+// N consecutive values, held as they lie in memory (16-bit values keep half the registers while
+// they wait) and widened where they are used.  The memory type is aligned like ONE value: a row
+// or a tensor may start anywhere (odd channel counts, views into a flat buffer), and global
+// memory takes 4- to 16-byte accesses at any address on gfx950, so one path serves every
+// alignment.
+template <typename T, int N>
+struct Vec {
+  typedef typename Elem<T>::type E;
+  typedef E Reg __attribute__((ext_vector_type(N)));
+  typedef E Mem __attribute__((ext_vector_type(N), aligned(sizeof(E))));
+  Reg v;
+
+  __device__ __forceinline__ float get(int i) const { return Elem<T>::widen(v[i]); }
+  __device__ __forceinline__ void set(int i, float f) { v[i] = Elem<T>::narrow(f); }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = (E)0;
+  }
+  __device__ __forceinline__ void load(const T *p) { v = *(const GANET_GLOBAL Mem *)(p); }
+  __device__ __forceinline__ void store(T *p) const { *(GANET_GLOBAL Mem *)(p) = v; }
+  // the first k values only; the rest reads as zero / is left alone
+  __device__ __forceinline__ void load(const T *p, long long k) {
+    if (k >= N) {
+      load(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = i < k ? ((const GANET_GLOBAL E *)p)[i] : (E)0;
+    }
+  }
+  __device__ __forceinline__ void store(T *p, long long k) const {
+    if (k >= N) {
+      store(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < k) ((GANET_GLOBAL E *)p)[i] = v[i];
+    }
+  }
+};
+
+// ---- lane exchanges without LDS: groups of 2, 4, 8 and 16 lanes by DPP, 32 by a swizzle, 64 by
+// the row broadcasts' counterpart (ds_bpermute) --------------------------------------------------
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+// the value of a partner lane; applied for 2, 4, ... W each lane has met all W of its group
+template <int W>
+__device__ __forceinline__ float partner(float v) {
+  if constexpr (W == 2) return dpp<0xB1>(v);         // quad_perm [1,0,3,2]
+  if constexpr (W == 4) return dpp<0x4E>(v);         // quad_perm [2,3,0,1]
+  if constexpr (W == 8) return dpp<0x141>(v);        // row_half_mirror
+  if constexpr (W == 16) return dpp<0x140>(v);       // row_mirror
+  if constexpr (W == 32)
+    return __uint_as_float(__builtin_amdgcn_ds_swizzle(__float_as_uint(v), 0x401F));  // lane ^ 16
+  return __shfl_xor(v, 32);
+}
+template <int W>
+__device__ __forceinline__ float group_sum(float v) {
+  if constexpr (W >= 2) v += partner<2>(v);
+  if constexpr (W >= 4) v += partner<4>(v);
+  if constexpr (W >= 8) v += partner<8>(v);
+  if constexpr (W >= 16) v += partner<16>(v);
+  if constexpr (W >= 32) v += partner<32>(v);
+  if constexpr (W >= 64) v += partner<64>(v);
+  return v;
+}
+template <int W>
+__device__ __forceinline__ float group_max(float v) {   // of values that are not NaN
+  if constexpr (W >= 2) v = fmaxf(v, partner<2>(v));
+  if constexpr (W >= 4) v = fmaxf(v, partner<4>(v));
+  if constexpr (W >= 8) v = fmaxf(v, partner<8>(v));
+  if constexpr (W >= 16) v = fmaxf(v, partner<16>(v));
+  if constexpr (W >= 32) v = fmaxf(v, partner<32>(v));
+  if constexpr (W >= 64) v = fmaxf(v, partner<64>(v));
+  return v;
+}
+
+}  // namespace ganet_vec

@@ -1,0 +1,381 @@
+"""The AdamW step over many tensors at once, and the norm of all gradients, on the gfx950 C-ABI
+(csrc/optim.hip).
+
+    m = b1 m + (1 - b1) g          v = b2 v + (1 - b2) g^2
+    p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
+
+No counterpart in the reference, whose training loop takes its optimizer from torch
+(mmdet/apis/train.py:83-168).
+
+  AdamW             torch.optim.Optimizer; states in 32 or 8 bits, float32 masters of 16-bit
+                    weights, clipping by the norm of all gradients without a pass or a wait of
+                    its own; register_with_mmcv() offers it to an `optimizer` config
+  adamw_step, adamw_step_8bit, grad_norm    the raw calls
+
+Parameters and gradients are float32, bfloat16 or float16, dense in any order (channels_last
+weights too).  CPU tensors raise NotImplementedError.
+"""
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from .dcn import _DTYPES
+
+BLOCK = _lib.GANET_STATE_BLOCK
+
+
+def _dense(t):
+    """Whether t's values fill their memory without gaps or overlaps, in any order."""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for step, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if step != expect:
+            return False
+        expect *= size
+    return True
+
+
+def _same_order(a, b):
+    """Whether two dense tensors of one shape lie alike in memory."""
+    if a.shape != b.shape:
+        return False
+    if a.is_contiguous() and b.is_contiguous():
+        return True
+    return all(x == y for x, y, n in zip(a.stride(), b.stride(), a.shape) if n != 1)
+
+
+def _one(tensors, what, device, dtype=None):
+    """Checks that a list's tensors share one device and dtype; returns the dtype."""
+    for t in tensors:
+        if not t.is_cuda:
+            raise NotImplementedError
+        if dtype is None:
+            dtype = t.dtype
+        if t.dtype != dtype:
+            raise TypeError("adamw: %s of dtypes %s and %s in one call" % (what, dtype, t.dtype))
+        if t.device != device:
+            raise ValueError("adamw: %s on %s and %s in one call" % (what, device, t.device))
+    return dtype
+
+
+def _in_order(params, others, what):
+    for p, t in zip(params, others):
+        if not _same_order(p, t):
+            raise ValueError("adamw: %s of shape %s and strides %s for a parameter of shape %s and "
+                             "strides %s" % (what, tuple(t.shape), t.stride(), tuple(p.shape),
+                                             p.stride()))
+
+
+def _step(params, grads, avgs, seconds, avg_scales, second_scales, bits, step, lr, betas, eps,
+          weight_decay, masters, grad_stats, skip_nonfinite, seed):
+    n = len(params)
+    for what, ts in (("gradients", grads), ("exp_avgs", avgs), ("second moments", seconds),
+                     ("masters", masters), ("scales", avg_scales), ("scales", second_scales)):
+        if ts is not None and len(ts) != n:
+            raise ValueError("adamw: %d %s for %d parameters" % (len(ts), what, n))
+    if n == 0:
+        return
+    device = params[0].device
+    pdtype = _one(params, "parameters", device)
+    gdtype = _one(grads, "gradients", device)
+    for t in (pdtype, gdtype):
+        if t not in _DTYPES:
+            raise TypeError("adamw: unsupported dtype %s" % t)
+    state = torch.float32 if bits == 32 else torch.float8_e4m3fn
+    _one(avgs, "states", device, state)
+    _one(seconds, "states", device, state)
+    if masters is not None:
+        if pdtype == torch.float32:
+            raise TypeError("adamw: masters of float32 parameters")
+        _one(masters, "masters", device, torch.float32)
+        _in_order(params, masters, "a master")
+    for p in params:
+        if not _dense(p):
+            raise ValueError("adamw: a parameter of shape %s and strides %s is not dense"
+                             % (tuple(p.shape), p.stride()))
+    _in_order(params, avgs, "a state")
+    _in_order(params, seconds, "a state")
+    if bits == 8:
+        for ts in (avg_scales, second_scales):
+            _one(ts, "scales", device, torch.float32)
+            for p, t in zip(params, ts):
+                if t.numel() != -(-p.numel() // BLOCK) or not t.is_contiguous():
+                    raise ValueError("adamw: a dense scale for each %d values of a parameter "
+                                     "is wanted" % BLOCK)
+    ordered = []                               # gradients in their parameters' order
+    for p, g in zip(params, grads):
+        if g.shape != p.shape:
+            raise ValueError("adamw: a gradient of shape %s for a parameter of shape %s"
+                             % (tuple(g.shape), tuple(p.shape)))
+        if not _same_order(p, g):
+            g = torch.empty_like(p, dtype=gdtype).copy_(g)
+        ordered.append(g)
+    written = [t.data_ptr() for ts in (params, avgs, seconds, masters) if ts is not None
+               for t in ts if t.numel()]
+    if len(set(written)) != len(written):
+        raise ValueError("adamw: a tensor is in the lists twice")
+
+    h = _lib.AdamwParams()
+    h.param_dtype, h.grad_dtype, h.state_bits = _DTYPES[pdtype], _DTYPES[gdtype], bits
+    h.skip_nonfinite = 1 if skip_nonfinite else 0
+    h.beta1, h.beta2, h.eps, h.weight_decay = betas[0], betas[1], eps, weight_decay
+    h.seed = int(seed) & 0xFFFFFFFF
+    held = []
+    if torch.is_tensor(step):
+        h.step_device = _scalar(step, torch.int64, device, "step", held)
+    else:
+        h.step = int(step)
+    if torch.is_tensor(lr):
+        h.lr_device = _scalar(lr, torch.float32, device, "lr", held)
+    else:
+        h.lr = lr
+    if grad_stats is not None:
+        if (grad_stats.dtype != torch.float32 or grad_stats.numel() != 4
+                or grad_stats.device != device or not grad_stats.is_contiguous()):
+            raise ValueError("adamw: grad_stats is the float32 [4] tensor of grad_norm")
+        h.grad_stats = grad_stats.data_ptr()
+    words = []
+    for i in range(n):
+        words += (params[i].data_ptr(), ordered[i].data_ptr(), avgs[i].data_ptr(),
+                  seconds[i].data_ptr(),
+                  avg_scales[i].data_ptr() if avg_scales is not None else 0,
+                  second_scales[i].data_ptr() if second_scales is not None else 0,
+                  masters[i].data_ptr() if masters is not None else 0, params[i].numel())
+    table = (ctypes.c_uint64 * len(words))(*words)
+    with torch.cuda.device(device):
+        rc = _lib.lib().ganet_adamw_step(ctypes.byref(table), n, ctypes.byref(h),
+                                         torch.cuda.current_stream(device).cuda_stream)
+    _lib.check(rc, "ganet_adamw_step")
+
+
+def _scalar(t, dtype, device, what, held):
+    if t.dtype != dtype or t.numel() != 1 or t.device != device:
+        raise ValueError("adamw: %s as a tensor is one %s on %s" % (what, dtype, device))
+    held.append(t)
+    return t.data_ptr()
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
+               weight_decay=1e-2, masters=None, grad_stats=None, skip_nonfinite=True):
+    """One step on all `params`, in place; exp_avgs and exp_avg_sqs are float32.
+
+    step: t, 1 at the first step (or a one-element int64 tensor on the device, as a captured graph
+    needs it; lr likewise as float32).  masters: float32 copies of 16-bit parameters: these are
+    stepped and the parameters get them rounded; without masters 16-bit parameters are stepped in
+    float32 and rounded to nearest, and updates below half a step of theirs are lost.
+    grad_stats: what grad_norm returned: gradients are multiplied by its coefficient on the way,
+    and with skip_nonfinite nothing changes where the norm is not finite.  Parameters in one call
+    share one dtype, gradients another; a gradient in another memory order is copied first."""
+    _step(params, grads, exp_avgs, exp_avg_sqs, None, None, 32, step, lr, betas, eps, weight_decay,
+          masters, grad_stats, skip_nonfinite, 0)
+
+
+def adamw_step_8bit(params, grads, exp_avgs, exp_rms, avg_scales, rms_scales, step, seed=0,
+                    lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, masters=None,
+                    grad_stats=None, skip_nonfinite=True):
+    """adamw_step with states in 8 bits: exp_avgs (m) and exp_rms (the root of the second moment)
+    are float8_e4m3fn of the parameter's shape, in units of avg_scales / rms_scales, one float32
+    for each 256 values in memory order (state_8bit makes them).  States are rounded up or down at
+    random, by a hash of (seed, step, the parameter's place in the list, the value's place in it):
+    the same inputs give the same bits.  Parameters move by the moments before that rounding."""
+    _step(params, grads, exp_avgs, exp_rms, avg_scales, rms_scales, 8, step, lr, betas, eps,
+          weight_decay, masters, grad_stats, skip_nonfinite, seed)
+
+
+def state_8bit(param):
+    """(exp_avg, exp_rms, avg_scale, rms_scale) of zeros for adamw_step_8bit."""
+    codes = [torch.zeros_like(param, dtype=torch.uint8).view(torch.float8_e4m3fn)
+             for _ in range(2)]
+    scales = [torch.zeros(-(-param.numel() // BLOCK), dtype=torch.float32, device=param.device)
+              for _ in range(2)]
+    return tuple(codes + scales)
+
+
+def grad_norm(grads, max_norm=None, inv_scale=1.0, out=None):
+    """The 2-norm of all gradients together, as a float32 [4] tensor on their device:
+    [norm, coefficient, 1 where the norm is not finite, 0].  norm is of inv_scale * gradients
+    (inv_scale: one over a loss scale); coefficient = inv_scale * min(1, max_norm / (norm + 1e-6)),
+    0 where the norm is not finite.  Nothing waits for the device; adamw_step and
+    adamw_step_8bit take the tensor as grad_stats.  Gradients of several dtypes may be mixed."""
+    grads = list(grads)
+    if out is None and not grads:
+        raise ValueError("grad_norm: no gradients")
+    device = grads[0].device if grads else out.device
+    dense = []
+    for g in grads:
+        if not g.is_cuda:
+            raise NotImplementedError
+        if g.dtype not in _DTYPES:
+            raise TypeError("grad_norm: unsupported dtype %s" % g.dtype)
+        if g.device != device:
+            raise ValueError("grad_norm: gradients on %s and %s" % (device, g.device))
+        dense.append(g if _dense(g) else g.contiguous())
+    max_norm = math.inf if max_norm is None else float(max_norm)
+    if not max_norm >= 0 or not math.isfinite(inv_scale):
+        raise ValueError("grad_norm: max_norm %r, inv_scale %r" % (max_norm, inv_scale))
+    L = _lib.lib()
+    n = len(dense)
+    ptrs = (ctypes.c_void_p * max(n, 1))(*[g.data_ptr() for g in dense])
+    numel = (ctypes.c_int64 * max(n, 1))(*[g.numel() for g in dense])
+    dtypes = (ctypes.c_int32 * max(n, 1))(*[_DTYPES[g.dtype] for g in dense])
+    with torch.cuda.device(device):
+        if out is None:
+            out = torch.empty(4, dtype=torch.float32, device=device)
+        elif (out.dtype != torch.float32 or out.numel() != 4 or out.device != device
+              or not out.is_contiguous()):
+            raise ValueError("grad_norm: out is a float32 [4] tensor on the gradients' device")
+        nbytes = L.ganet_grad_norm_workspace_bytes(numel, n)
+        ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
+        rc = L.ganet_grad_norm(ptrs, numel, dtypes, n, max_norm, inv_scale, out.data_ptr(),
+                               ws.data_ptr(), nbytes,
+                               torch.cuda.current_stream(device).cuda_stream)
+    _lib.check(rc, "ganet_grad_norm")
+    return out
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW over the parameters of a model, a few launches a step.
+
+    state_bits=8: moments in 8 bits (parameters of fewer than min_8bit_size values keep 32).
+    master_weights: 16-bit parameters get float32 masters, made from them at their first step.
+    max_grad_norm: the gradients of ALL parameters are clipped to this norm, on the way.
+    skip_nonfinite: with max_grad_norm (or grad_stats given to step) a step whose gradients' norm
+    is not finite changes no weight and no moment; the step number goes on.
+    capturable: step numbers live on the device, so that a step captured into a HIP graph counts
+    on when replayed; make one step before the capture.  lr may be a float32 tensor on the device.
+    `grad_stats` holds the last step's grad_norm tensor."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+                 state_bits=32, master_weights=False, max_grad_norm=None, skip_nonfinite=True,
+                 seed=0, min_8bit_size=4096, capturable=False):
+        if not torch.is_tensor(lr) and not (0 <= lr < math.inf):
+            raise ValueError("AdamW: lr %r" % (lr,))
+        if not all(0 <= b < 1 for b in betas):
+            raise ValueError("AdamW: betas %r" % (betas,))
+        if not 0 <= eps < math.inf or not 0 <= weight_decay < math.inf:
+            raise ValueError("AdamW: eps %r, weight_decay %r" % (eps, weight_decay))
+        if state_bits not in (32, 8):
+            raise ValueError("AdamW: states of %r bits" % (state_bits,))
+        if max_grad_norm is not None and not max_grad_norm >= 0:
+            raise ValueError("AdamW: max_grad_norm %r" % (max_grad_norm,))
+        super(AdamW, self).__init__(params, dict(lr=lr, betas=betas, eps=eps,
+                                                 weight_decay=weight_decay))
+        self.state_bits, self.master_weights = state_bits, master_weights
+        self.max_grad_norm, self.skip_nonfinite = max_grad_norm, skip_nonfinite
+        self.seed, self.min_8bit_size, self.capturable = seed, min_8bit_size, capturable
+        self.grad_stats = None
+
+    def _init_state(self, p, fresh):
+        """First step of a parameter.  `fresh`: the step counters made in this call, by device."""
+        if not p.is_cuda:
+            raise NotImplementedError
+        if p.dtype not in _DTYPES:
+            raise TypeError("AdamW: unsupported dtype %s" % p.dtype)
+        if not _dense(p):
+            raise ValueError("AdamW: a parameter of strides %s is not dense" % (p.stride(),))
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: make one step before the capture")
+        st = self.state[p]
+        if self.capturable:
+            if p.device not in fresh:
+                fresh[p.device] = torch.zeros((), dtype=torch.int64, device=p.device)
+            st["step"] = fresh[p.device]
+        else:
+            st["step"] = 0
+        if self.state_bits == 8 and p.numel() >= self.min_8bit_size:
+            st["exp_avg"], st["exp_rms"], st["avg_scale"], st["rms_scale"] = state_8bit(p.detach())
+        else:
+            st["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
+            st["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
+        if self.master_weights and p.dtype != torch.float32:
+            st["master"] = p.detach().float()
+
+    @torch.no_grad()
+    def step(self, closure=None, grad_stats=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        every = [(group, p) for group in self.param_groups for p in group["params"]
+                 if p.grad is not None]
+        if not every:
+            return loss
+        if any(p.grad.is_sparse for _, p in every):
+            raise RuntimeError("AdamW: sparse gradients")
+        if grad_stats is None and self.max_grad_norm is not None:
+            grad_stats = grad_norm([p.grad for _, p in every], self.max_grad_norm)
+        self.grad_stats = grad_stats
+        fresh, counters, lists = {}, {}, {}
+        for group, p in every:
+            if p not in self.state or "step" not in self.state[p]:
+                self._init_state(p, fresh)
+            st = self.state[p]
+            if self.capturable:
+                counters[id(st["step"])] = st["step"]
+                at = id(st["step"])
+            else:
+                st["step"] += 1
+                at = st["step"]
+            key = (id(group), p.device, p.dtype, p.grad.dtype, "avg_scale" in st, "master" in st,
+                   at)
+            lists.setdefault(key, (group, []))[1].append(p)
+        for t in counters.values():
+            t.add_(1)
+        for key, (group, ps) in lists.items():
+            st = [self.state[p] for p in ps]
+            common = dict(lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                          weight_decay=group["weight_decay"], grad_stats=grad_stats,
+                          masters=[s["master"] for s in st] if key[5] else None,
+                          skip_nonfinite=self.skip_nonfinite)
+            grads = [p.grad for p in ps]
+            if key[4]:
+                adamw_step_8bit(ps, grads, [s["exp_avg"] for s in st], [s["exp_rms"] for s in st],
+                                [s["avg_scale"] for s in st], [s["rms_scale"] for s in st],
+                                st[0]["step"], seed=self.seed, **common)
+            else:
+                adamw_step(ps, grads, [s["exp_avg"] for s in st], [s["exp_avg_sq"] for s in st],
+                           st[0]["step"], **common)
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """States keep the types they were saved in (torch would cast them to the parameter's)."""
+        super(AdamW, self).load_state_dict(state_dict)
+        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
+        ps = [p for group in self.param_groups for p in group["params"]]
+        counters = {}
+        for i, p in zip(ids, ps):
+            for name, value in state_dict["state"].get(i, {}).items():
+                if name == "step":
+                    value = int(value)
+                    if self.capturable:        # one counter for the parameters that share a number
+                        key = (p.device, value)
+                        if key not in counters:
+                            counters[key] = torch.full((), value, dtype=torch.int64,
+                                                       device=p.device)
+                        value = counters[key]
+                elif name in ("avg_scale", "rms_scale"):
+                    value = value.detach().to(p.device, copy=True)
+                elif torch.is_tensor(value):
+                    kept = torch.empty_like(p, dtype=value.dtype)
+                    value = kept.copy_(value.detach()) if value.dtype != torch.float8_e4m3fn else \
+                        _copy_codes(kept, value)
+                self.state[p][name] = value
+
+
+def _copy_codes(to, codes):
+    to.view(torch.uint8).copy_(codes.detach().view(torch.uint8))
+    return to
+
+
+def register_with_mmcv(force=False):
+    """Register AdamW as 'HipAdamW' in mmcv's OPTIMIZERS (optimizer=dict(type='HipAdamW', ...)).
+    An explicit call, as in ganet_amd.dcn; False when mmcv is absent."""
+    try:
+        from mmcv.runner import OPTIMIZERS
+    except Exception:
+        return False
+    OPTIMIZERS.register_module('HipAdamW', module=AdamW, force=force)
+    return True

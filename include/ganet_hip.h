@@ -14,7 +14,8 @@
  * A few measurement knobs are read from the environment ("Build, limits");
  * those that size a workspace are read once per process: set them before the first call.
  * Call them from one host thread per GPU with that GPU current.
- * Forward AND backward of the operators are here (ganet_deform_conv_backward), plus
+ * Forward AND backward of the operators are here (ganet_deform_conv_backward), the
+ * training operators next to them (3: layer norm, AdamW, the gradients' norm), plus
  * host-only routines that turn decoded records into the reference's result formats.
  *
  * Citations are file:line in the reference tree (Wolfwjs/GANet).
@@ -461,6 +462,103 @@ int ganet_tusimple_from_lanes(const int32_t *lanes, int B, const int32_t *h_samp
  * GANET_ERR_WORKSPACE when text_bytes < text_start[B] (text may be NULL to query). */
 int ganet_culane_text(const int32_t *lanes, int B, int threads, char *text, size_t text_bytes,
                       size_t *text_start);
+
+/* ------------------------------------------------------------------------
+ * (3) Training operators beside the layers of (1): layer norm over channels, the
+ * AdamW step over many tensors, the norm of all gradients.  No counterpart in the
+ * reference, which takes them from torch and mmcv (optimizer built by mmcv's Runner,
+ * mmdet/apis/train.py:83-168).
+ * ---------------------------------------------------------------------- */
+
+/* Layer norm over the C channels of each of outer * inner positions:
+ *   y = (x - mean) * rstd * weight + bias,  mean = sum x / C,
+ *   rstd = 1 / sqrt(sum (x - mean)^2 / C + eps).
+ * inner == 1: [outer][C] rows (tokens, or an NHWC map's pixels), `x_stride` etc. values
+ * apart (>= C); inner > 1: [outer][C][inner] (an NCHW map, inner = H * W), images
+ * `x_stride` values apart (>= C * inner), positions dense.
+ * Sums are float32; each output is rounded once, to nearest. */
+typedef struct {
+  int64_t outer;        /* rows, or images */
+  int64_t inner;        /* positions of an image whose channels are `inner` values apart; 1 for rows */
+  int64_t x_stride;     /* values from one row / image to the next: x */
+  int64_t y_stride;     /* ... of y (forward) or grad_x (backward) */
+  int64_t g_stride;     /* ... of grad_y (backward only) */
+  int32_t C;            /* 1 ... GANET_LAYER_NORM_MAX_C */
+  int32_t dtype;        /* ganet_dtype of x, y, grad_y, grad_x */
+  int32_t weight_dtype; /* ganet_dtype of weight, bias and their gradients */
+  float eps;            /* >= 0 */
+} ganet_layer_norm_params;
+
+#define GANET_LAYER_NORM_MAX_C 16384
+
+/* weight, bias [C], either may be NULL (1 and 0); mean, rstd [outer * inner] float32, both
+ * NULL where no backward follows.  y may be x. */
+int ganet_layer_norm_forward(const void *x, const void *weight, const void *bias, void *y,
+                             float *mean, float *rstd, const ganet_layer_norm_params *p,
+                             ganet_stream_t stream);
+
+/* grad_x, grad_weight, grad_bias may each be NULL (not all three) and are overwritten:
+ *   xh = (x - mean) * rstd, a = weight * grad_y,
+ *   grad_x = rstd * (a - mean_C(a) - xh * mean_C(a * xh)),
+ *   grad_weight = sum over positions of grad_y * xh, grad_bias = sum of grad_y.
+ * The sums over positions are formed in a fixed order: partial sums of each workgroup go
+ * to the workspace, a second launch adds them.  The same inputs give the same bits.
+ * grad_x may be grad_y or x. */
+size_t ganet_layer_norm_backward_workspace_bytes(const ganet_layer_norm_params *p);
+int ganet_layer_norm_backward(const void *x, const void *weight, const void *grad_y,
+                              const float *mean, const float *rstd, void *grad_x,
+                              void *grad_weight, void *grad_bias,
+                              const ganet_layer_norm_params *p, void *workspace,
+                              size_t workspace_bytes, ganet_stream_t stream);
+
+/* One tensor of an AdamW step: dense, `n` values, all device memory, all in the same order. */
+typedef struct {
+  void *param;             /* param_dtype */
+  const void *grad;        /* grad_dtype */
+  void *exp_avg;           /* state_bits 32: float32 [n]; 8: OCP e4m3 [n] */
+  void *second;            /* 32: float32 exp_avg_sq [n]; 8: e4m3 root of it [n] */
+  float *exp_avg_scale;    /* 8 only: [ceil(n / GANET_STATE_BLOCK)] */
+  float *second_scale;     /* 8 only */
+  float *master;           /* NULL, or the float32 weights of 16-bit `param`: then these are
+                              stepped and `param` is only written, their rounded copy.  In a
+                              list all have one or none has. */
+  int64_t n;
+} ganet_step_tensor;
+
+#define GANET_STATE_BLOCK 256   /* values that share a scale in the 8-bit states */
+
+/* g = grad * stats[1] (1 without stats);  m = beta1 m + (1 - beta1) g;
+ * v = beta2 v + (1 - beta2) g^2;
+ * param = param (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps).
+ * In 8 bits m and sqrt(v) are kept as e4m3 times a float32 scale for each 256 values
+ * (largest magnitude / 448), rounded up or down at random: the random word of a value is a
+ * hash of (seed, t, the tensor's place in the list, the value's place in it), so the same
+ * inputs give the same bits.  The parameter's step uses m and v before that rounding. */
+typedef struct {
+  int32_t param_dtype, grad_dtype; /* ganet_dtype */
+  int32_t state_bits;              /* 32 or 8 */
+  int32_t skip_nonfinite;          /* 1: with stats[2] != 0 nothing is changed */
+  int64_t step;                    /* t >= 1 */
+  uint32_t seed;                   /* state_bits 8 */
+  uint32_t reserved;               /* 0 */
+  double lr, beta1, beta2, eps, weight_decay;
+  const float *grad_stats;         /* NULL, or what ganet_grad_norm wrote (device) */
+  const int64_t *step_device;      /* NULL, or t on the device (a captured graph counts on) */
+  const float *lr_device;          /* NULL, or lr on the device */
+} ganet_adamw_params;
+
+int ganet_adamw_step(const ganet_step_tensor *tensors /* host array */, int count,
+                     const ganet_adamw_params *p, ganet_stream_t stream);
+
+/* stats[0] = norm = |inv_scale| * sqrt(sum of all squares), summed in float64;
+ * stats[1] = inv_scale * min(1, max_norm / (norm + 1e-6)): what the gradients are to be
+ * multiplied by (max_norm = INFINITY: no clipping); stats[2] = 1 where the norm is not a
+ * finite float32 (then stats[1] = 0), else 0; stats[3] = 0.  `grads`, `numel`, `dtypes` are host arrays;
+ * stats [4] float32 and the workspace device memory.  Nothing waits for the device. */
+size_t ganet_grad_norm_workspace_bytes(const int64_t *numel, int count);
+int ganet_grad_norm(const void *const *grads, const int64_t *numel, const int32_t *dtypes,
+                    int count, double max_norm, double inv_scale, float *stats,
+                    void *workspace, size_t workspace_bytes, ganet_stream_t stream);
 
 #ifdef __cplusplus
 }
