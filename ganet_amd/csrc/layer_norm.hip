@@ -15,6 +15,7 @@
 namespace {
 
 using ganet_vec::bf16_t;
+using ganet_vec::Elem;
 using ganet_vec::f16_t;
 using ganet_vec::group_sum;
 using ganet_vec::Vec;
@@ -40,98 +41,51 @@ __device__ __forceinline__ float load_weight(const void *w, int dtype, int c, fl
 
 template <typename T>
 __device__ __forceinline__ float load1(const T *p) {
-  Vec<T, 1> v;
-  v.load(p);
-  return v.get(0);
+  return Elem<T>::widen(*(const GANET_GLOBAL typename Elem<T>::type *)p);
 }
 template <typename T>
 __device__ __forceinline__ void store1(T *p, float f) {
-  Vec<T, 1> v;
-  v.set(0, f);
-  v.store(p);
+  *(GANET_GLOBAL typename Elem<T>::type *)p = Elem<T>::narrow(f);
 }
 
-// The sum over a workgroup of `WAVES` wavefronts, in every lane; `part` [WAVES] is free again
-// after the second barrier of the next call.
-template <int WAVES>
-__device__ __forceinline__ float block_sum(float v, float *part) {
-  v = group_sum<64>(v);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = 0.0f;
+template <typename T, int N>
+__device__ __forceinline__ void load_some(const T *p, int left, float (&out)[N]) {
+  if (left >= N) {
+    const typename Vec<T, N>::Reg v = *(const GANET_GLOBAL typename Vec<T, N>::Mem *)p;
 #pragma unroll
-  for (int i = 0; i < WAVES; ++i) v += part[i];
-  __syncthreads();
+    for (int k = 0; k < N; ++k) out[k] = Elem<T>::widen(v[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) out[k] = k < left ? load1(p + k) : 0.0f;
+  }
+}
+
+// N consecutive weights from column c on, `none` where there are none
+template <int N>
+__device__ __forceinline__ void load_weights(const void *w, int dtype, int c, int C, float none, float (&out)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) out[k] = none;
+  if (!w || c >= C) return;
+  if (dtype == GANET_F32)
+    load_some<float, N>((const float *)w + c, C - c, out);
+  else if (dtype == GANET_BF16)
+    load_some<bf16_t, N>((const bf16_t *)w + c, C - c, out);
+  else
+    load_some<f16_t, N>((const f16_t *)w + c, C - c, out);
+}
+
+// Adds a value over the lanes that are LANES apart (the row groups of a wavefront).
+template <int LANES>
+__device__ __forceinline__ float across_groups(float v) {
+#pragma unroll
+  for (int o = LANES; o < 64; o <<= 1) v += __shfl_xor(v, o);
   return v;
 }
 
 // ---------------------------------------------------------------------------------------------
-// Any C: a row (or 64 positions of a plane) per workgroup, the values read again for each pass
+// Planes of any C: 64 positions a workgroup, the values read again for each pass
 // ---------------------------------------------------------------------------------------------
 constexpr int kThreads = 256;
-
-template <typename T>
-__global__ __launch_bounds__(kThreads) void ln_rows_any_fwd(Args a) {
-  __shared__ float part[kThreads / 64];
-  for (long long row = blockIdx.x; row < a.outer; row += gridDim.x) {
-    const T *x = (const T *)a.x + row * a.xs;
-    T *y = (T *)a.y + row * a.ys;
-    float s = 0.0f;
-    for (int c = threadIdx.x; c < a.C; c += kThreads) s += load1(x + c);
-    const float mean = block_sum<kThreads / 64>(s, part) / a.c;   // exact for equal values
-    s = 0.0f;
-    for (int c = threadIdx.x; c < a.C; c += kThreads) {
-      const float d = load1(x + c) - mean;
-      s += d * d;
-    }
-    const float rstd = 1.0f / sqrtf(block_sum<kThreads / 64>(s, part) * a.inv_c + a.eps);
-    for (int c = threadIdx.x; c < a.C; c += kThreads)
-      store1(y + c, (load1(x + c) - mean) * rstd * load_weight(a.w, a.wdtype, c, 1.0f) +
-                        load_weight(a.b, a.wdtype, c, 0.0f));
-    if (threadIdx.x == 0 && a.mean) {
-      a.mean[row] = mean;
-      a.rstd[row] = rstd;
-    }
-  }
-}
-
-template <typename T>
-__global__ __launch_bounds__(kThreads) void ln_rows_any_bwd(Args a) {
-  __shared__ float part[kThreads / 64];
-  extern __shared__ float sums[];               // [2][C]: a thread's own columns
-  if (a.partial)
-    for (int c = threadIdx.x; c < 2 * a.C; c += kThreads) sums[c] = 0.0f;
-  __syncthreads();
-  for (long long row = blockIdx.x; row < a.outer; row += gridDim.x) {
-    const T *x = (const T *)a.x + row * a.xs;
-    const T *g = (const T *)a.g + row * a.gs;
-    T *dx = (T *)a.y + row * a.ys;
-    const float mean = a.mean[row], rstd = a.rstd[row];
-    float s1 = 0.0f, s2 = 0.0f;
-    for (int c = threadIdx.x; c < a.C; c += kThreads) {
-      const float xh = (load1(x + c) - mean) * rstd, dy = load1(g + c);
-      const float wa = dy * load_weight(a.w, a.wdtype, c, 1.0f);
-      s1 += wa;
-      s2 += wa * xh;
-      if (a.partial) {
-        sums[c] += dy * xh;
-        sums[a.C + c] += dy;
-      }
-    }
-    if (!a.y) continue;
-    const float m1 = block_sum<kThreads / 64>(s1, part) * a.inv_c;
-    const float m2 = block_sum<kThreads / 64>(s2, part) * a.inv_c;
-    for (int c = threadIdx.x; c < a.C; c += kThreads) {
-      const float xh = (load1(x + c) - mean) * rstd;
-      const float wa = load1(g + c) * load_weight(a.w, a.wdtype, c, 1.0f);
-      store1(dx + c, rstd * (wa - m1 - xh * m2));
-    }
-  }
-  __syncthreads();
-  if (a.partial)
-    for (int c = threadIdx.x; c < 2 * a.C; c += kThreads)
-      a.partial[(long long)blockIdx.x * 2 * a.C + c] = sums[c];
-}
 
 // Planes: lane l of every wavefront owns position 64 * tile + l, the wavefronts share the channels.
 constexpr int kTile = 64;
@@ -227,22 +181,481 @@ __global__ __launch_bounds__(kThreads) void ln_planes_any_bwd(Args a) {
       a.partial[(long long)blockIdx.x * 2 * a.C + c] = sums[c];
 }
 
-// Adds the workgroups' sums: 64 channels a workgroup, its four wavefronts take every fourth of
-// the `n` partial rows.  blockIdx.y: 0 the weight's gradient, 1 the bias's.
-__global__ __launch_bounds__(kThreads) void ln_finish(const float *partial, int n, int C, void *dw, void *db,
-                                                      int dtype) {
-  __shared__ float part[kThreads / 64][64];
+// ---------------------------------------------------------------------------------------------
+// Rows in registers: each value is read once
+// ---------------------------------------------------------------------------------------------
+// A row is spread over LANES lanes (a part of a wavefront, one, four or sixteen), NV vectors of 16
+// bytes each, and stays in registers from the load to the store: mean, variance and output take one
+// pass over memory.  Narrow rows share a wavefront (64 / LANES of them), so that every load moves
+// 1 KiB whatever C is.
+template <typename T>
+constexpr int kN = 16 / (int)sizeof(T);
+
+// The sum over a row's lanes, in each of them.
+template <int LANES>
+__device__ __forceinline__ float row_sum(float v, float *part, int slot) {
+  if constexpr (LANES <= 64) {
+    return group_sum<LANES>(v);
+  } else {
+    // `part` holds two sets of one float a wavefront; calls alternate, so one barrier a call does
+    constexpr int W = LANES / 64;
+    v = group_sum<64>(v);
+    if ((threadIdx.x & 63) == 0) part[slot * W + (threadIdx.x >> 6)] = v;
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) v += part[slot * W + i];
+    return v;
+  }
+}
+
+// Forward.  R rows of a lane are loaded before the first is worked on: 64 bytes a lane in flight
+// where rows are plenty.
+template <typename T, int LANES, int NV, int R>
+__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_rows_fwd(Args a) {
+  constexpr int N = kN<T>;
+  constexpr int THREADS = LANES > 256 ? LANES : 256;
+  constexpr int ROWS = THREADS / LANES;              // of a workgroup at once
+  __shared__ float part[2 * (LANES > 64 ? LANES / 64 : 1)];
+  const int l = (int)threadIdx.x % LANES;
+  const long long row0 = (long long)blockIdx.x * (ROWS * R) + (int)threadIdx.x / LANES;
+  Vec<T, N> x[R][NV];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const long long row = row0 + r * ROWS;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * LANES + l) * N;
+      if (row < a.outer && c < a.C)
+        x[r][v].load((const T *)a.x + row * a.xs + c, a.C - c);
+      else
+        x[r][v].zero();
+    }
+  }
+  float w[NV][N], b[NV][N];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int c = (v * LANES + l) * N;
+    load_weights<N>(a.w, a.wdtype, c, a.C, 1.0f, w[v]);
+    load_weights<N>(a.b, a.wdtype, c, a.C, 0.0f, b[v]);
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const long long row = row0 + r * ROWS;
+    float s = 0.0f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int k = 0; k < N; ++k) s += x[r][v].get(k);
+    const float mean = row_sum<LANES>(s, part, 0) / a.c;      // exact for equal values
+    s = 0.0f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      x[r][v].forget();
+      const int left = a.C - (v * LANES + l) * N;
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const float d = x[r][v].get(k) - mean;
+        s += k < left ? d * d : 0.0f;
+      }
+    }
+    const float rstd = 1.0f / sqrtf(row_sum<LANES>(s, part, 1) * a.inv_c + a.eps);
+    if (row >= a.outer) continue;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * LANES + l) * N;
+      if (c >= a.C) continue;
+      x[r][v].forget();
+      Vec<T, N> y;
+#pragma unroll
+      for (int k = 0; k < N; ++k) y.set(k, (x[r][v].get(k) - mean) * rstd * w[v][k] + b[v][k]);
+      y.store((T *)a.y + row * a.ys + c, a.C - c);
+    }
+    if (l == 0 && a.mean) {
+      a.mean[row] = mean;
+      a.rstd[row] = rstd;
+    }
+  }
+}
+
+// Backward.  Workgroups of sixteen wavefronts stay, one on each CU, and take rows in turn; a lane
+// keeps its columns' sums of grad_weight and grad_bias in registers and requests the next row
+// before it works on this one.  Few, large workgroups: each leaves [2][C] floats to be added.
+constexpr int kBwdThreads = 1024;
+
+template <typename T, int LANES, int NV, bool SUMS>
+__global__ __launch_bounds__(kBwdThreads) void ln_rows_bwd(Args a) {
+  constexpr int N = kN<T>;
+  constexpr int ROWS = kBwdThreads / LANES;
+  constexpr int W = LANES > 64 ? LANES / 64 : 1;
+  __shared__ float part[4 * (kBwdThreads / 64)];
+  extern __shared__ float sums[];                    // [2][C], for the end
+  const int l = (int)threadIdx.x % LANES;
+  const int group = (int)threadIdx.x / LANES;
+  float w[NV][N], dw[NV][N], db[NV][N];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    load_weights<N>(a.w, a.wdtype, (v * LANES + l) * N, a.C, 1.0f, w[v]);
+#pragma unroll
+    for (int k = 0; k < N; ++k) dw[v][k] = db[v][k] = 0.0f;
+  }
+  Vec<T, N> x[NV], g[NV];
+  float mean, rstd;
+  auto fetch = [&](long long row) {
+    const bool in = row < a.outer;
+    mean = in ? a.mean[row] : 0.0f;
+    rstd = in ? a.rstd[row] : 0.0f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * LANES + l) * N;
+      if (in && c < a.C) {
+        x[v].load((const T *)a.x + row * a.xs + c, a.C - c);
+        g[v].load((const T *)a.g + row * a.gs + c, a.C - c);
+      } else {
+        x[v].zero();
+        g[v].zero();
+      }
+    }
+  };
+  constexpr bool AHEAD = NV * N <= 8;                // more fill the 128 registers by themselves
+  const long long step = (long long)gridDim.x * ROWS;
+  const long long first = (long long)blockIdx.x * ROWS;
+  if (AHEAD) fetch(first + group);
+  int turn = 0;
+  for (long long base = first; base < a.outer; base += step) {      // uniform over the workgroup
+    const long long row = base + group;
+    Vec<T, N> xr[NV], gr[NV];
+    if (!AHEAD) fetch(row);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      xr[v] = x[v];
+      gr[v] = g[v];
+    }
+    const float mu = mean, rs = rstd;
+    if (AHEAD && base + step < a.outer) fetch(row + step);
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        // zero past the row's end: grad_y is zero there
+        const float xh = (xr[v].get(k) - mu) * rs, dy = gr[v].get(k);
+        const float wa = dy * w[v][k];
+        s1 += wa;
+        s2 += wa * xh;
+        if constexpr (SUMS) {
+          dw[v][k] += dy * xh;
+          db[v][k] += dy;
+        }
+      }
+    if (!a.y) continue;
+    float m1, m2;
+    if constexpr (LANES <= 64) {
+      m1 = group_sum<LANES>(s1) * a.inv_c;
+      m2 = group_sum<LANES>(s2) * a.inv_c;
+    } else {
+      s1 = group_sum<64>(s1);
+      s2 = group_sum<64>(s2);
+      float *p = part + turn * 2 * (kBwdThreads / 64);
+      turn ^= 1;                                     // two sets: one barrier a row
+      if ((threadIdx.x & 63) == 0) {
+        p[threadIdx.x >> 6] = s1;
+        p[kBwdThreads / 64 + (threadIdx.x >> 6)] = s2;
+      }
+      __syncthreads();
+      m1 = m2 = 0.0f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        m1 += p[group * W + i];
+        m2 += p[kBwdThreads / 64 + group * W + i];
+      }
+      m1 *= a.inv_c;
+      m2 *= a.inv_c;
+    }
+    if (row >= a.outer) continue;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      xr[v].forget();
+      gr[v].forget();
+    }
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * LANES + l) * N;
+      if (c >= a.C) continue;
+      Vec<T, N> d;
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const float xh = (xr[v].get(k) - mu) * rs;
+        d.set(k, rs * (gr[v].get(k) * w[v][k] - m1 - xh * m2));
+      }
+      d.store((T *)a.y + row * a.ys + c, a.C - c);
+    }
+  }
+  if constexpr (!SUMS) return;
+  // the rows' groups add into LDS one after another: a fixed order
+  if constexpr (LANES < 64) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        dw[v][k] = across_groups<LANES>(dw[v][k]);
+        db[v][k] = across_groups<LANES>(db[v][k]);
+      }
+  }
+  constexpr int TURNS = LANES < 64 ? kBwdThreads / 64 : ROWS;
+  const int mine = LANES < 64 ? (int)threadIdx.x / 64 : group;
+  for (int i = 0; i < TURNS; ++i) {
+    __syncthreads();
+    if (mine != i || (LANES < 64 && ((int)threadIdx.x & 63) >= LANES)) continue;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const int c = (v * LANES + l) * N + k;
+        if (c >= a.C) continue;
+        sums[c] = dw[v][k] + (i ? sums[c] : 0.0f);
+        sums[a.C + c] = db[v][k] + (i ? sums[a.C + c] : 0.0f);
+      }
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < 2 * a.C; c += kBwdThreads)
+    a.partial[(long long)blockIdx.x * 2 * a.C + c] = sums[c];
+}
+
+// ---------------------------------------------------------------------------------------------
+// Planes in registers
+// ---------------------------------------------------------------------------------------------
+// A workgroup owns 16 vectors of neighbouring positions (VB bytes each, 256 bytes of a channel's
+// plane at VB = 16) and all channels; a wavefront's four rows of 16 lanes and its WAVES wavefronts
+// are 4 WAVES slots, each with up to NC consecutive channels in registers.  Sums over channels: a
+// lane's own, then the four rows, then the wavefronts through LDS.
+template <typename T, int VB, int NC, int WAVES>
+struct Plane {
+  static constexpr int N = VB / (int)sizeof(T);
+  static constexpr int TILE = 16 * N;
+  static constexpr int SLOTS = 4 * WAVES;
+  static constexpr int THREADS = 64 * WAVES;
+};
+
+// s[N] of each lane, added over the workgroup's slots, in every lane.
+template <int N, int WAVES>
+__device__ __forceinline__ void slots_sum(float (&s)[N], float (*part)[16][N]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int k = 0; k < N; ++k) s[k] = ganet_vec::rows_sum(s[k]);
+  if (lane < 16) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) part[wave][lane][k] = s[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) s[k] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i)
+#pragma unroll
+    for (int k = 0; k < N; ++k) s[k] += part[i][lane & 15][k];
+}
+
+// Where a lane's N positions begin.  A vector that would pass the plane's end is moved back to end
+// there (the plane holds N positions at least): every lane then loads and stores whole vectors; the
+// positions it shares with another lane get the same values from both, and `own` says from which
+// element on they count in sums over positions (N: none).
+template <int N>
+__device__ __forceinline__ long long plane_position(long long pos, long long inner, int &own) {
+  const long long left = inner - pos;
+  own = left >= N ? 0 : (left > 0 ? N - (int)left : N);
+  return left >= N ? pos : inner - N;
+}
+
+template <typename T, int VB, int NC, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void ln_planes_fwd(Args a, int tiles, int nc) {
+  typedef Plane<T, VB, NC, WAVES> P;
+  constexpr int N = P::N;
+  __shared__ __align__(16) float part[2][WAVES][16][N];
+  __shared__ float weights[2][P::SLOTS * NC];
+  int own;
+  const long long img = blockIdx.x / tiles;
+  const long long pos = plane_position<N>(
+      (long long)(blockIdx.x % tiles) * P::TILE + (threadIdx.x & 15) * N, a.inner, own);
+  const int c0 = (int)(threadIdx.x >> 4) * nc;       // nc <= NC channels of a slot
+  const T *x = (const T *)a.x + img * a.xs + (long long)c0 * a.inner + pos;
+  Vec<T, N> v[NC];
+#pragma unroll
+  for (int k = 0; k < NC; ++k) {
+    v[k].zero();
+    if (k < nc && c0 + k < a.C) v[k].load(x + k * a.inner);
+  }
+  for (int c = threadIdx.x; c < a.C; c += P::THREADS) {
+    weights[0][c] = load_weight(a.w, a.wdtype, c, 1.0f);
+    weights[1][c] = load_weight(a.b, a.wdtype, c, 0.0f);
+  }
+  float mean[N], rstd[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) mean[j] = rstd[j] = 0.0f;
+#pragma unroll
+  for (int k = 0; k < NC; ++k)
+#pragma unroll
+    for (int j = 0; j < N; ++j) mean[j] += v[k].get(j);
+  slots_sum<N, WAVES>(mean, part[0]);                // its barrier also covers the weights
+#pragma unroll
+  for (int k = 0; k < NC; ++k) v[k].forget();
+#pragma unroll
+  for (int j = 0; j < N; ++j) mean[j] /= a.c;
+#pragma unroll
+  for (int k = 0; k < NC; ++k) {
+    const bool in = k < nc && c0 + k < a.C;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float d = in ? v[k].get(j) - mean[j] : 0.0f;
+      rstd[j] += d * d;
+    }
+  }
+  slots_sum<N, WAVES>(rstd, part[1]);
+#pragma unroll
+  for (int k = 0; k < NC; ++k) v[k].forget();
+#pragma unroll
+  for (int j = 0; j < N; ++j) rstd[j] = 1.0f / sqrtf(rstd[j] * a.inv_c + a.eps);
+  T *y = (T *)a.y + img * a.ys + (long long)c0 * a.inner + pos;
+#pragma unroll
+  for (int k = 0; k < NC; ++k) {
+    if (k < nc && c0 + k < a.C) {
+      const float w = weights[0][c0 + k], b = weights[1][c0 + k];
+      Vec<T, N> o;
+#pragma unroll
+      for (int j = 0; j < N; ++j) o.set(j, (v[k].get(j) - mean[j]) * rstd[j] * w + b);
+      o.store(y + k * a.inner);
+    }
+  }
+  if (threadIdx.x < 16 && a.mean) {
+    Vec<float, N> m, r;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      m.set(j, mean[j]);
+      r.set(j, rstd[j]);
+    }
+    m.store(a.mean + img * a.inner + pos);
+    r.store(a.rstd + img * a.inner + pos);
+  }
+}
+
+template <typename T, int VB, int NC, int WAVES, bool SUMS>
+__global__ __launch_bounds__(64 * WAVES) void ln_planes_bwd(Args a, int tiles, int nc) {
+  typedef Plane<T, VB, NC, WAVES> P;
+  constexpr int N = P::N;
+  __shared__ __align__(16) float part[2][2][WAVES][16][N];
+  __shared__ float weights[P::SLOTS * NC];
+  const int c0 = (int)(threadIdx.x >> 4) * nc;
+  for (int c = threadIdx.x; c < a.C; c += P::THREADS) weights[c] = load_weight(a.w, a.wdtype, c, 1.0f);
+  __syncthreads();
+  float dw[NC], db[NC];
+#pragma unroll
+  for (int k = 0; k < NC; ++k) dw[k] = db[k] = 0.0f;
+  int turn = 0;
+  for (long long i = blockIdx.x; i < a.outer * tiles; i += gridDim.x, turn ^= 1) {
+    int own;
+    const long long img = i / tiles;
+    const long long pos = plane_position<N>((i % tiles) * P::TILE + (threadIdx.x & 15) * N, a.inner, own);
+    const long long c_at = (long long)c0 * a.inner + pos;
+    const T *x = (const T *)a.x + img * a.xs + c_at, *g = (const T *)a.g + img * a.gs + c_at;
+    Vec<T, N> vx[NC], vg[NC];
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      vx[k].zero();
+      vg[k].zero();
+      if (k < nc && c0 + k < a.C) {
+        vx[k].load(x + k * a.inner);
+        vg[k].load(g + k * a.inner);
+      }
+    }
+    Vec<float, N> mean, rstd;
+    mean.load(a.mean + img * a.inner + pos);
+    rstd.load(a.rstd + img * a.inner + pos);
+    float m1[N], m2[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) m1[j] = m2[j] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      if (k < nc) {
+        const float w = c0 + k < a.C ? weights[c0 + k] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const float xh = (vx[k].get(j) - mean.v[j]) * rstd.v[j], dy = vg[k].get(j);
+          m1[j] += dy * w;
+          m2[j] += dy * w * xh;
+          if constexpr (SUMS) {
+            const float counted = j >= own ? dy : 0.0f;
+            dw[k] += counted * xh;
+            db[k] += counted;
+          }
+        }
+      }
+    }
+    if (!a.y) continue;
+    // two sets of part: the next tile's sums do not wait for this one's readers
+    slots_sum<N, WAVES>(m1, part[turn][0]);
+    slots_sum<N, WAVES>(m2, part[turn][1]);
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      vx[k].forget();
+      vg[k].forget();
+    }
+    T *dx = (T *)a.y + img * a.ys + c_at;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      if (k < nc && c0 + k < a.C) {
+        const float w = weights[c0 + k];
+        Vec<T, N> o;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const float xh = (vx[k].get(j) - mean.v[j]) * rstd.v[j];
+          o.set(j, rstd.v[j] * (vg[k].get(j) * w - m1[j] * a.inv_c - xh * (m2[j] * a.inv_c)));
+        }
+        o.store(dx + k * a.inner);
+      }
+    }
+  }
+  if constexpr (SUMS) {
+    float *out = a.partial + (long long)blockIdx.x * 2 * a.C;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const float sw = group_sum<16>(dw[k]), sb = group_sum<16>(db[k]);
+      if ((threadIdx.x & 15) == 0 && k < nc && c0 + k < a.C) {
+        out[c0 + k] = sw;
+        out[a.C + c0 + k] = sb;
+      }
+    }
+  }
+}
+
+// Adds the workgroups' sums: 64 channels a workgroup, its 16 wavefronts take every 16th of the `n`
+// partial rows, four loads at a time.  blockIdx.y: 0 the weight's gradient, 1 the bias's.
+constexpr int kFinish = 1024;
+__global__ __launch_bounds__(kFinish) void ln_finish(const float *partial, int n, int C, void *dw, void *db,
+                                                     int dtype) {
+  __shared__ float part[kFinish / 64][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c = blockIdx.x * 64 + lane;
   void *out = blockIdx.y ? db : dw;
   if (!out) return;
   float s = 0.0f;
-  if (c < C)
-    for (int i = wave; i < n; i += kThreads / 64) s += partial[((long long)i * 2 + blockIdx.y) * C + c];
+  if (c < C) {
+    const float *p = partial + (long long)blockIdx.y * C + c;
+    constexpr int W = kFinish / 64;
+    int i = wave;
+    for (; i + 3 * W < n; i += 4 * W) {
+      float f[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) f[u] = load1(p + (long long)(i + u * W) * 2 * C);
+      s += (f[0] + f[1]) + (f[2] + f[3]);
+    }
+    for (; i < n; i += W) s += load1(p + (long long)i * 2 * C);
+  }
   part[wave][lane] = s;
   __syncthreads();
   if (wave != 0 || c >= C) return;
-  s = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+  s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kFinish / 64; ++i) s += part[i][lane];
   if (dtype == GANET_F32)
     store1((float *)out + c, s);
   else if (dtype == GANET_BF16)
@@ -254,6 +667,8 @@ __global__ __launch_bounds__(kThreads) void ln_finish(const float *partial, int 
 // ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
+constexpr long long kMostBlocks = 1ll << 22;      // of one launch: its threads stay below 2^32
+
 bool dtype_ok(int d) { return d == GANET_F32 || d == GANET_BF16 || d == GANET_F16; }
 
 int params_ok(const ganet_layer_norm_params *p, bool backward) {
@@ -296,10 +711,141 @@ int with_type(int dtype, F &&f) {
   return f(f16_t());
 }
 
-// Workgroups of the backward, each with sums of its own: two on each of the 256 CUs.
+// ---- which kernel ----
+// Rows: the narrowest of these that holds C, i.e. LANES * NV vectors of 16 bytes.
+template <typename T, typename F>
+int with_row_shape(int C, F &&f) {
+  const int vecs = (C + kN<T> - 1) / kN<T>;
+#define GANET_ROW(LANES, NV) \
+  if (vecs <= (LANES) * (NV)) return f(std::integral_constant<int, LANES>(), std::integral_constant<int, NV>())
+  GANET_ROW(1, 1);
+  GANET_ROW(2, 1);
+  GANET_ROW(4, 1);
+  GANET_ROW(8, 1);
+  GANET_ROW(16, 1);
+  GANET_ROW(32, 1);
+  GANET_ROW(64, 1);
+  GANET_ROW(64, 2);
+  GANET_ROW(256, 1);
+  GANET_ROW(256, 2);
+  GANET_ROW(1024, 1);
+  GANET_ROW(1024, 2);
+  if constexpr (sizeof(T) == 4) GANET_ROW(1024, 4);
+#undef GANET_ROW
+  return GANET_ERR_UNSUPPORTED;           // past GANET_LAYER_NORM_MAX_C
+}
+
+long long tiles_of(const ganet_layer_norm_params *p, int tile) { return (p->inner + tile - 1) / tile; }
+
+// Planes: the fewest registers that hold C; a forward keeps one map, a backward two.
+enum { kAny = 0 };
+template <bool BACKWARD, typename T, typename F>
+int with_plane_shape(const ganet_layer_norm_params *p, F &&f) {
+#define GANET_PLANE(VB, NC, WAVES)                                                                      \
+  if (p->C <= 4 * (WAVES) * (NC) && p->inner >= (VB) / (int)sizeof(T))                                                                          \
+    return f(std::integral_constant<int, VB>(), std::integral_constant<int, NC>(),                      \
+             std::integral_constant<int, WAVES>())
+  GANET_PLANE(16, 4, 4);
+  GANET_PLANE(16, 8, 4);
+  if constexpr (!BACKWARD) {
+    GANET_PLANE(16, 16, 4);
+    GANET_PLANE(16, 32, 4);
+    GANET_PLANE(16, 32, 8);
+  } else if constexpr (sizeof(T) == 4) {
+    GANET_PLANE(16, 16, 4);
+    GANET_PLANE(16, 16, 8);
+    GANET_PLANE(8, 32, 8);
+  } else {
+    GANET_PLANE(16, 8, 8);
+    GANET_PLANE(8, 16, 8);
+    GANET_PLANE(8, 32, 8);
+  }
+#undef GANET_PLANE
+  return f(std::integral_constant<int, kAny>(), std::integral_constant<int, 1>(), std::integral_constant<int, 1>());
+}
+
+// Workgroups of the backward, each with sums of its own: what is on the chip at once.
 int backward_blocks(const ganet_layer_norm_params *p) {
-  const long long work = p->inner == 1 ? p->outer : p->outer * ((p->inner + kTile - 1) / kTile);
-  return (int)(work < 512 ? work : 512);
+  int blocks = 0;
+  with_type(p->dtype, [&](auto t) {
+    typedef decltype(t) T;
+    if (p->inner == 1)
+      return with_row_shape<T>(p->C, [&](auto lanes, auto) {
+        const long long need = (p->outer + kBwdThreads / lanes.value - 1) / (kBwdThreads / lanes.value);
+        blocks = (int)(need < 256 ? need : 256);
+        return GANET_OK;
+      });
+    return with_plane_shape<true, T>(p, [&](auto vb, auto nc, auto waves) {
+      if constexpr (vb.value == kAny) {
+        const long long need = p->outer * tiles_of(p, kTile);
+        blocks = (int)(need < 512 ? need : 512);
+      } else {
+        typedef Plane<T, vb.value, nc.value, waves.value> P;
+        const long long need = p->outer * tiles_of(p, P::TILE);
+        const int most = waves.value == 8 ? 256 : 512;        // two wavefronts a SIMD
+        blocks = (int)(need < most ? need : most);
+      }
+      return GANET_OK;
+    });
+  });
+  return blocks;
+}
+
+template <typename T>
+int launch_forward(const ganet_layer_norm_params *p, const Args &a, hipStream_t s) {
+  if (p->inner == 1)
+    return with_row_shape<T>(p->C, [&](auto lanes, auto nv) {
+      constexpr int L = lanes.value, NV = nv.value;
+      constexpr int threads = L > 256 ? L : 256, rows = threads / L;
+      // four vectors of a lane in flight once that still leaves 4 workgroups a CU
+      constexpr int R = NV == 1 ? 4 : (NV == 2 ? 2 : 1);
+      const long long many = (p->outer + rows * R - 1) / (rows * R);
+      const bool deep = R > 1 && L <= 64 && many >= 1024;
+      const long long blocks = deep ? many : (p->outer + rows - 1) / rows;
+      if (blocks > kMostBlocks) return (int)GANET_ERR_UNSUPPORTED;
+      if constexpr (R > 1 && L <= 64) {
+        if (deep) {
+          ln_rows_fwd<T, L, NV, R><<<dim3((unsigned)blocks), dim3(threads), 0, s>>>(a);
+          return ganet_check_launch();
+        }
+      }
+      ln_rows_fwd<T, L, NV, 1><<<dim3((unsigned)blocks), dim3(threads), 0, s>>>(a);
+      return ganet_check_launch();
+    });
+  return with_plane_shape<false, T>(p, [&](auto vb, auto nc, auto waves) {
+    if constexpr (vb.value == kAny) {
+      const long long work = p->outer * tiles_of(p, kTile);
+      ln_planes_any_fwd<T><<<dim3((unsigned)(work < 8192 ? work : 8192)), dim3(kThreads), 0, s>>>(a);
+    } else {
+      typedef Plane<T, vb.value, nc.value, waves.value> P;
+      const long long tiles = tiles_of(p, P::TILE);
+      if (p->outer * tiles > kMostBlocks) return (int)GANET_ERR_UNSUPPORTED;
+      ln_planes_fwd<T, vb.value, nc.value, waves.value>
+          <<<dim3((unsigned)(p->outer * tiles)), dim3(P::THREADS), 0, s>>>(a, (int)tiles,
+                                                                          (p->C + P::SLOTS - 1) / P::SLOTS);
+    }
+    return ganet_check_launch();
+  });
+}
+
+template <typename T, bool SUMS>
+int launch_backward(const ganet_layer_norm_params *p, const Args &a, int blocks, hipStream_t s) {
+  const size_t lds = SUMS ? (size_t)2 * p->C * sizeof(float) : 0;
+  if (p->inner == 1)
+    return with_row_shape<T>(p->C, [&](auto lanes, auto nv) {
+      ln_rows_bwd<T, lanes.value, nv.value, SUMS><<<dim3(blocks), dim3(kBwdThreads), lds, s>>>(a);
+      return ganet_check_launch();
+    });
+  return with_plane_shape<true, T>(p, [&](auto vb, auto nc, auto waves) {
+    if constexpr (vb.value == kAny) {
+      ln_planes_any_bwd<T><<<dim3(blocks), dim3(kThreads), lds, s>>>(a);
+    } else {
+      typedef Plane<T, vb.value, nc.value, waves.value> P;
+      ln_planes_bwd<T, vb.value, nc.value, waves.value, SUMS>
+          <<<dim3(blocks), dim3(P::THREADS), 0, s>>>(a, (int)tiles_of(p, P::TILE), (p->C + P::SLOTS - 1) / P::SLOTS);
+    }
+    return ganet_check_launch();
+  });
 }
 
 }  // namespace
@@ -317,17 +863,8 @@ extern "C" int ganet_layer_norm_forward(const void *x, const void *weight, const
   a.y = y;
   a.mean = mean;
   a.rstd = rstd;
-  hipStream_t s = (hipStream_t)stream;
-  const long long work = p->inner == 1 ? p->outer : p->outer * ((p->inner + kTile - 1) / kTile);
-  const unsigned blocks = (unsigned)(work < 8192 ? work : 8192);
-  return with_type(p->dtype, [&](auto t) {
-    typedef decltype(t) T;
-    if (p->inner == 1)
-      ln_rows_any_fwd<T><<<dim3(blocks), dim3(kThreads), 0, s>>>(a);
-    else
-      ln_planes_any_fwd<T><<<dim3(blocks), dim3(kThreads), 0, s>>>(a);
-    return ganet_check_launch();
-  });
+  return with_type(p->dtype,
+                   [&](auto t) { return launch_forward<decltype(t)>(p, a, (hipStream_t)stream); });
 }
 
 extern "C" size_t ganet_layer_norm_backward_workspace_bytes(const ganet_layer_norm_params *p) {
@@ -358,19 +895,14 @@ extern "C" int ganet_layer_norm_backward(const void *x, const void *weight, cons
     a.rstd = (float *)rstd;
     a.partial = sums ? (float *)workspace : nullptr;
     blocks = backward_blocks(p);
-    const size_t lds = sums ? (size_t)2 * p->C * sizeof(float) : 0;
     const int rc = with_type(p->dtype, [&](auto t) {
       typedef decltype(t) T;
-      if (p->inner == 1)
-        ln_rows_any_bwd<T><<<dim3(blocks), dim3(kThreads), lds, s>>>(a);
-      else
-        ln_planes_any_bwd<T><<<dim3(blocks), dim3(kThreads), lds, s>>>(a);
-      return ganet_check_launch();
+      return sums ? launch_backward<T, true>(p, a, blocks, s) : launch_backward<T, false>(p, a, blocks, s);
     });
     if (rc != GANET_OK) return rc;
   }
   if (!sums) return GANET_OK;
-  ln_finish<<<dim3((p->C + 63) / 64, 2), dim3(kThreads), 0, s>>>((const float *)workspace, blocks, p->C, grad_weight,
+  ln_finish<<<dim3((p->C + 63) / 64, 2), dim3(kFinish), 0, s>>>((const float *)workspace, blocks, p->C, grad_weight,
                                                                 grad_bias, p->weight_dtype);
   return ganet_check_launch();
 }

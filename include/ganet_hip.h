@@ -492,7 +492,7 @@ typedef struct {
 #define GANET_LAYER_NORM_MAX_C 16384
 
 /* weight, bias [C], either may be NULL (1 and 0); mean, rstd [outer * inner] float32, both
- * NULL where no backward follows.  y may be x. */
+ * NULL where no backward follows.  y must not overlap x. */
 int ganet_layer_norm_forward(const void *x, const void *weight, const void *bias, void *y,
                              float *mean, float *rstd, const ganet_layer_norm_params *p,
                              ganet_stream_t stream);
@@ -503,7 +503,7 @@ int ganet_layer_norm_forward(const void *x, const void *weight, const void *bias
  *   grad_weight = sum over positions of grad_y * xh, grad_bias = sum of grad_y.
  * The sums over positions are formed in a fixed order: partial sums of each workgroup go
  * to the workspace, a second launch adds them.  The same inputs give the same bits.
- * grad_x may be grad_y or x. */
+ * Outputs must not overlap inputs. */
 size_t ganet_layer_norm_backward_workspace_bytes(const ganet_layer_norm_params *p);
 int ganet_layer_norm_backward(const void *x, const void *weight, const void *grad_y,
                               const float *mean, const float *rstd, void *grad_x,
