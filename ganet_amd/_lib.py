@@ -215,6 +215,25 @@ def lib():
     return _lib
 
 
+def call(index, fn, *args):
+    """fn(*args, stream) with GPU `index` current, on torch's current stream there.  The device
+    guard and the stream object cost 3 us a call: both are left out where they change nothing."""
+    import torch
+    if torch.cuda.current_device() == index:
+        return fn(*args, _raw_stream(index))
+    with torch.cuda.device(index):
+        return fn(*args, _raw_stream(index))
+
+
+def _raw_stream(index):
+    import torch
+    global _raw_stream
+    # the address alone, without a Stream object around it
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+        lambda i: torch.cuda.current_stream(i).cuda_stream)
+    return _raw_stream(index)
+
+
 def status_string(status):
     return lib().ganet_status_string(int(status)).decode()
 

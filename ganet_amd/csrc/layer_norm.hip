@@ -289,7 +289,7 @@ __global__ __launch_bounds__(kBwdThreads) void ln_rows_bwd(Args a) {
   constexpr int ROWS = kBwdThreads / LANES;
   constexpr int W = LANES > 64 ? LANES / 64 : 1;
   __shared__ float part[4 * (kBwdThreads / 64)];
-  extern __shared__ float sums[];                    // [2][C], for the end
+  extern __shared__ __align__(16) float sums[];      // [groups][columns], for the end
   const int l = (int)threadIdx.x % LANES;
   const int group = (int)threadIdx.x / LANES;
   float w[NV][N], dw[NV][N], db[NV][N];
@@ -391,35 +391,41 @@ __global__ __launch_bounds__(kBwdThreads) void ln_rows_bwd(Args a) {
       d.store((T *)a.y + row * a.ys + c, a.C - c);
     }
   }
-  if constexpr (!SUMS) return;
-  // the rows' groups add into LDS one after another: a fixed order
-  if constexpr (LANES < 64) {
+  if constexpr (SUMS) {
+    // The row groups' sums meet in LDS, [groups][columns], the weight's and then the bias's (64 KiB
+    // at most), and are added in their order.
+    constexpr int COLS = LANES * NV * N;
+    constexpr int GROUPS = LANES < 64 ? kBwdThreads / 64 : ROWS;
+    const int mine = LANES < 64 ? (int)threadIdx.x / 64 : group;
+    float *out = a.partial + (long long)blockIdx.x * 2 * a.C;
+    if constexpr (LANES < 64) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
+      for (int v = 0; v < NV; ++v)
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        dw[v][k] = across_groups<LANES>(dw[v][k]);
-        db[v][k] = across_groups<LANES>(db[v][k]);
+        for (int k = 0; k < N; ++k) {
+          dw[v][k] = across_groups<LANES>(dw[v][k]);
+          db[v][k] = across_groups<LANES>(db[v][k]);
+        }
+    }
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      __syncthreads();
+      if (LANES >= 64 || ((int)threadIdx.x & 63) < LANES) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+          for (int k = 0; k < N; ++k)
+            sums[mine * COLS + (v * LANES + l) * N + k] = which ? db[v][k] : dw[v][k];
       }
-  }
-  constexpr int TURNS = LANES < 64 ? kBwdThreads / 64 : ROWS;
-  const int mine = LANES < 64 ? (int)threadIdx.x / 64 : group;
-  for (int i = 0; i < TURNS; ++i) {
-    __syncthreads();
-    if (mine != i || (LANES < 64 && ((int)threadIdx.x & 63) >= LANES)) continue;
+      __syncthreads();
+      for (int c = threadIdx.x; c < a.C; c += kBwdThreads) {
+        float s = 0.0f;
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const int c = (v * LANES + l) * N + k;
-        if (c >= a.C) continue;
-        sums[c] = dw[v][k] + (i ? sums[c] : 0.0f);
-        sums[a.C + c] = db[v][k] + (i ? sums[a.C + c] : 0.0f);
+        for (int i = 0; i < GROUPS; ++i) s += sums[i * COLS + c];
+        out[which * a.C + c] = s;
       }
+    }
   }
-  __syncthreads();
-  for (int c = threadIdx.x; c < 2 * a.C; c += kBwdThreads)
-    a.partial[(long long)blockIdx.x * 2 * a.C + c] = sums[c];
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -627,35 +633,34 @@ __global__ __launch_bounds__(64 * WAVES) void ln_planes_bwd(Args a, int tiles, i
   }
 }
 
-// Adds the workgroups' sums: 64 channels a workgroup, its 16 wavefronts take every 16th of the `n`
-// partial rows, four loads at a time.  blockIdx.y: 0 the weight's gradient, 1 the bias's.
+// Adds the workgroups' sums: 32 channels a workgroup (whole 128-byte lines), its 32 half wavefronts
+// take every 32nd of the `n` <= 512 partial rows, eight loads at a time: latency is all there is.
+// blockIdx.y: 0 the weight's gradient, 1 the bias's.
 constexpr int kFinish = 1024;
+constexpr int kFinishCols = 32;
 __global__ __launch_bounds__(kFinish) void ln_finish(const float *partial, int n, int C, void *dw, void *db,
                                                      int dtype) {
-  __shared__ float part[kFinish / 64][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = blockIdx.x * 64 + lane;
+  constexpr int SLOTS = kFinish / kFinishCols;
+  __shared__ float part[SLOTS][kFinishCols];
+  const int col = threadIdx.x % kFinishCols, slot = threadIdx.x / kFinishCols;
+  const int c = blockIdx.x * kFinishCols + col;
   void *out = blockIdx.y ? db : dw;
   if (!out) return;
   float s = 0.0f;
-  if (c < C) {
-    const float *p = partial + (long long)blockIdx.y * C + c;
-    constexpr int W = kFinish / 64;
-    int i = wave;
-    for (; i + 3 * W < n; i += 4 * W) {
-      float f[4];
+  const float *p = partial + (long long)blockIdx.y * C + (c < C ? c : 0);
+  for (int i = slot; i < n; i += 8 * SLOTS) {
+    float f[8];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) f[u] = load1(p + (long long)(i + u * W) * 2 * C);
-      s += (f[0] + f[1]) + (f[2] + f[3]);
-    }
-    for (; i < n; i += W) s += load1(p + (long long)i * 2 * C);
+    for (int u = 0; u < 8; ++u) f[u] = i + u * SLOTS < n ? load1(p + (long long)(i + u * SLOTS) * 2 * C) : 0.0f;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s += f[u];
   }
-  part[wave][lane] = s;
+  part[slot][col] = s;
   __syncthreads();
-  if (wave != 0 || c >= C) return;
+  if (slot != 0 || c >= C) return;
   s = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kFinish / 64; ++i) s += part[i][lane];
+  for (int i = 0; i < SLOTS; ++i) s += part[i][col];
   if (dtype == GANET_F32)
     store1((float *)out + c, s);
   else if (dtype == GANET_BF16)
@@ -830,15 +835,18 @@ int launch_forward(const ganet_layer_norm_params *p, const Args &a, hipStream_t 
 
 template <typename T, bool SUMS>
 int launch_backward(const ganet_layer_norm_params *p, const Args &a, int blocks, hipStream_t s) {
-  const size_t lds = SUMS ? (size_t)2 * p->C * sizeof(float) : 0;
   if (p->inner == 1)
     return with_row_shape<T>(p->C, [&](auto lanes, auto nv) {
-      ln_rows_bwd<T, lanes.value, nv.value, SUMS><<<dim3(blocks), dim3(kBwdThreads), lds, s>>>(a);
+      constexpr int L = lanes.value, NV = nv.value;
+      constexpr int groups = L < 64 ? kBwdThreads / 64 : kBwdThreads / L;
+      constexpr size_t room = SUMS ? (size_t)groups * L * NV * kN<T> * sizeof(float) : 0;
+      ln_rows_bwd<T, L, NV, SUMS><<<dim3(blocks), dim3(kBwdThreads), room, s>>>(a);
       return ganet_check_launch();
     });
   return with_plane_shape<true, T>(p, [&](auto vb, auto nc, auto waves) {
     if constexpr (vb.value == kAny) {
-      ln_planes_any_bwd<T><<<dim3(blocks), dim3(kThreads), lds, s>>>(a);
+      ln_planes_any_bwd<T>
+          <<<dim3(blocks), dim3(kThreads), SUMS ? (size_t)2 * p->C * sizeof(float) : 0, s>>>(a);
     } else {
       typedef Plane<T, vb.value, nc.value, waves.value> P;
       ln_planes_bwd<T, vb.value, nc.value, waves.value, SUMS>
@@ -902,7 +910,7 @@ extern "C" int ganet_layer_norm_backward(const void *x, const void *weight, cons
     if (rc != GANET_OK) return rc;
   }
   if (!sums) return GANET_OK;
-  ln_finish<<<dim3((p->C + 63) / 64, 2), dim3(kFinish), 0, s>>>((const float *)workspace, blocks, p->C, grad_weight,
+  ln_finish<<<dim3((p->C + kFinishCols - 1) / kFinishCols, 2), dim3(kFinish), 0, s>>>((const float *)workspace, blocks, p->C, grad_weight,
                                                                 grad_bias, p->weight_dtype);
   return ganet_check_launch();
 }

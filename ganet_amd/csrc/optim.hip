@@ -180,14 +180,31 @@ __device__ __forceinline__ unsigned mix32(unsigned x) {
   return x ^ (x >> 16);
 }
 
-// e4m3 bits of a (0 <= a <= 448), up or down by the 16 random bits.  float32's dropped 20 bits of
-// mantissa plus a random 20-bit number carry into the kept ones with the right probability; below
-// 2^-6, where e4m3 is evenly spaced by 2^-9, a + 2^-6 has that same spacing.
-__device__ __forceinline__ unsigned sr_e4m3(float a, unsigned r16) {
-  const bool small = a < 0x1p-6f;
-  const float y = small ? a + 0x1p-6f : a;
-  return ((__float_as_uint(y) + (r16 << 4) + 8u) >> 20) - (small ? 968u : 960u);
+// A value as e4m3 in byte SEL of `to`, up or down by 16 random bits (the upper ones of `random`).
+// The instruction adds the upper 20 bits of its second operand to the 20 bits of mantissa that
+// e4m3 drops and truncates; below 2^-6, where e4m3 is evenly spaced by 2^-9, to as many bits below
+// 2^-9 (both compared with that definition on a million values: no difference).  Bit 15 stands for
+// half of the sixteenth bit, so that the numbers are centred.
+template <int SEL>
+__device__ __forceinline__ unsigned to_e4m3(float v, unsigned random, unsigned to) {
+  return (unsigned)__builtin_amdgcn_cvt_sr_fp8_f32(v, (int)(random | 0x8000u), (int)to, SEL);
 }
+
+__device__ __forceinline__ unsigned max3(unsigned a, unsigned b, unsigned c) {
+  const unsigned m = b > c ? b : c;
+  return a > m ? a : m;
+}
+// The largest of 32 lanes' values
+__device__ __forceinline__ unsigned block_max(unsigned v) {
+  auto with = [&](unsigned o) { v = v > o ? v : o; };
+  with((unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true));
+  with((unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true));
+  with((unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true));
+  with((unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, true));
+  with((unsigned)__builtin_amdgcn_ds_swizzle((int)v, 0x401F));
+  return v;
+}
+constexpr unsigned kInf = 0x7F800000u;
 
 template <typename TP, typename TG, bool MASTER>
 __global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8 a) {
@@ -235,10 +252,12 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8 a) {
       vr[u][0] = (unsigned)wr;
       vr[u][1] = (unsigned)(wr >> 32);
     } else {
-      for (int j = 0; j < (int)k; ++j) {
-        vm[u][j >> 2] |= (unsigned)m[i + j] << (8 * (j & 3));
-        vr[u][j >> 2] |= (unsigned)r[i + j] << (8 * (j & 3));
-      }
+#pragma unroll
+      for (int j = 0; j < kVec8; ++j)
+        if (j < k) {
+          vm[u][j >> 2] |= (unsigned)m[i + j] << (8 * (j & 3));
+          vr[u][j >> 2] |= (unsigned)r[i + j] << (8 * (j & 3));
+        }
     }
   }
 #pragma unroll
@@ -246,7 +265,10 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8 a) {
     const int i = (u * kThreads + (int)threadIdx.x) * kVec8;
     const long long k = left - i;
     float nm[kVec8], nr[kVec8];
-    float tm = 0.0f, tr = 0.0f;
+    // Magnitudes are compared as integers: the order is the same, and what is not finite comes out
+    // on top.
+    unsigned um = 0, ur = 0;
+    const float b1s = a.h.b1 * sm[u];
 #pragma unroll
     for (int j = 0; j < kVec8; j += 2) {
       const auto m2 = (j & 2) ? __builtin_amdgcn_cvt_pk_f32_fp8(vm[u][j >> 2], true)
@@ -256,54 +278,71 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8 a) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float gr = vg[u].get(j + e) * c.gscale;
-        const float mm = a.h.b1 * (m2[e] * sm[u]) + a.h.omb1 * gr;
         const float rr = r2[e] * sr[u];
-        const float root = sqrtf(a.h.b2 * (rr * rr) + a.h.omb2 * (gr * gr));
-        nm[j + e] = mm;
-        nr[j + e] = root;
-        tm = fmaxf(tm, fabsf(mm));
-        tr = fmaxf(tr, root);
+        nm[j + e] = fmaf(m2[e], b1s, a.h.omb1 * gr);
+        // v_sqrt_f32 and v_rcp_f32 below: 1.5 * 2^-24 of the value each, a tenth of the exact
+        // forms' instructions; a second moment under 2^-126 counts as zero
+        nr[j + e] = __builtin_amdgcn_sqrtf(fmaf(a.h.b2 * rr, rr, a.h.omb2 * gr * gr));
       }
+      um = max3(um, __float_as_uint(nm[j]) & 0x7FFFFFFFu, __float_as_uint(nm[j + 1]) & 0x7FFFFFFFu);
+      ur = max3(ur, __float_as_uint(nr[j]), __float_as_uint(nr[j + 1]));
     }
-    tm = ganet_vec::group_max<32>(tm);
-    tr = ganet_vec::group_max<32>(tr);
-    // A gradient that is not finite reaches its own value only: it is left out of the scale (NaN
-    // already is) and becomes e4m3's NaN.
-    if (tm == INFINITY || tr == INFINITY) {
-      tm = tr = 0.0f;
+    um = block_max(um);
+    ur = block_max(ur);
+    // A gradient that is not finite reaches its own value only: it is left out of the scales and
+    // becomes e4m3's NaN.
+    unsigned bad = 0;
+    if (um >= kInf || ur >= kInf) {
+      um = ur = 0;
 #pragma unroll
       for (int j = 0; j < kVec8; ++j) {
-        if (fabsf(nm[j]) < INFINITY) tm = fmaxf(tm, fabsf(nm[j]));
-        if (nr[j] < INFINITY) tr = fmaxf(tr, nr[j]);
+        const unsigned mb = __float_as_uint(nm[j]) & 0x7FFFFFFFu, rb = __float_as_uint(nr[j]);
+        if (mb >= kInf || rb >= kInf) bad |= 1u << j;
+        if (mb < kInf && mb > um) um = mb;
+        if (rb < kInf && rb > ur) ur = rb;
       }
-      tm = ganet_vec::group_max<32>(tm);
-      tr = ganet_vec::group_max<32>(tr);
+      um = block_max(um);
+      ur = block_max(ur);
     }
+    float tm = __uint_as_float(um);
+    const float tr = __uint_as_float(ur);
     if (tm < 0x1p-110f) tm = 0.0f;      // 448 / tm would overflow: such a block is held as zeros
-    const float im = tm > 0.0f ? 448.0f / tm : 0.0f;
-    const float ir = tr > 0.0f ? 448.0f / tr : 0.0f;
-    if (k <= 0) continue;               // uniform over a block's lanes but for the last block
-    const unsigned at_block = (unsigned)(block0 + i / kBlock);
-    const unsigned bkey = mix32(key + at_block * 0xC2B2AE35u);
+    const float im = tm > 0.0f ? 448.0f * __builtin_amdgcn_rcpf(tm) : 0.0f;
+    const float ir = tr > 0.0f ? 448.0f * __builtin_amdgcn_rcpf(tr) : 0.0f;
+    if (k <= 0) continue;               // after the exchanges between a block's lanes
+    const unsigned bkey = mix32(key + (unsigned)(block0 + i / kBlock) * 0xC2B2AE35u);
     unsigned om[2] = {0, 0}, orr[2] = {0, 0};
-#pragma unroll
-    for (int j = 0; j < kVec8; ++j) {
+    auto value = [&](auto J) {
+      constexpr int j = J.value;
       unsigned h = bkey + (unsigned)((i + j) % kBlock) * 0x9E3779B1u;
       h ^= h >> 16;
       h *= 0xBB67AE85u;
       h ^= h >> 15;
-      unsigned cm = sr_e4m3(fminf(fabsf(nm[j]) * im, 448.0f), h & 0xFFFFu);
-      unsigned cr = sr_e4m3(fminf(nr[j] * ir, 448.0f), h >> 16);
-      if (nr[j] > 0.0f && cr < 1u) cr = 1u;
-      if (!(fabsf(nm[j]) < INFINITY)) cm = 0x7Fu;
-      if (!(nr[j] < INFINITY)) cr = 0x7Fu;
-      cm |= (__float_as_uint(nm[j]) >> 24) & 0x80u;
-      om[j >> 2] |= cm << (8 * (j & 3));
-      orr[j >> 2] |= cr << (8 * (j & 3));
+      om[j >> 2] = to_e4m3<(j & 3)>(__builtin_amdgcn_fmed3f(nm[j] * im, -448.0f, 448.0f), h << 16, om[j >> 2]);
+      // above zero and below e4m3's smallest: the smallest
+      orr[j >> 2] = to_e4m3<(j & 3)>(
+          __builtin_amdgcn_fmed3f(nr[j] * ir, nr[j] > 0.0f ? 0x1p-9f : 0.0f, 448.0f), h & 0xFFFF0000u, orr[j >> 2]);
       const float old = MASTER ? vw[u].get(j) : vp[u].get(j);
-      const float now = old * c.decay - c.lr_c * (nm[j] / (nr[j] * c.rbc2 + a.h.eps));
+      const float part = nm[j] * __builtin_amdgcn_rcpf(fmaf(nr[j], c.rbc2, a.h.eps));
+      const float now = fmaf(-c.lr_c, part, old * c.decay);
       if constexpr (MASTER) vw[u].set(j, now);
       vp[u].set(j, now);
+    };
+    value(std::integral_constant<int, 0>());
+    value(std::integral_constant<int, 1>());
+    value(std::integral_constant<int, 2>());
+    value(std::integral_constant<int, 3>());
+    value(std::integral_constant<int, 4>());
+    value(std::integral_constant<int, 5>());
+    value(std::integral_constant<int, 6>());
+    value(std::integral_constant<int, 7>());
+    if (bad) {
+#pragma unroll
+      for (int j = 0; j < kVec8; ++j)
+        if (bad >> j & 1) {
+          om[j >> 2] |= 0x7Fu << (8 * (j & 3));
+          orr[j >> 2] |= 0x7Fu << (8 * (j & 3));
+        }
     }
     if constexpr (MASTER) vw[u].store(w + i, k);
     vp[u].store(p + i, k);
@@ -313,14 +352,16 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8 a) {
       *(GANET_GLOBAL Byte8 *)(r + i) =
           __builtin_bit_cast(Byte8, (unsigned long long)orr[0] | (unsigned long long)orr[1] << 32);
     } else {
-      for (int j = 0; j < (int)k; ++j) {
-        m[i + j] = (unsigned char)(om[j >> 2] >> (8 * (j & 3)));
-        r[i + j] = (unsigned char)(orr[j >> 2] >> (8 * (j & 3)));
-      }
+#pragma unroll
+      for (int j = 0; j < kVec8; ++j)
+        if (j < k) {
+          m[i + j] = (unsigned char)(om[j >> 2] >> (8 * (j & 3)));
+          r[i + j] = (unsigned char)(orr[j >> 2] >> (8 * (j & 3)));
+        }
     }
     if (i % kBlock == 0) {
-      ((GANET_GLOBAL float *)ms)[i / kBlock] = tm / 448.0f;
-      ((GANET_GLOBAL float *)rs)[i / kBlock] = tr / 448.0f;
+      ((GANET_GLOBAL float *)ms)[i / kBlock] = tm * (1.0f / 448.0f);
+      ((GANET_GLOBAL float *)rs)[i / kBlock] = tr * (1.0f / 448.0f);
     }
   }
 }
@@ -328,10 +369,11 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8 a) {
 // ---------------------------------------------------------------------------------------------
 // The norm of all gradients
 // ---------------------------------------------------------------------------------------------
-// Squares are summed in float64: float32 would overflow at |g| = 1.8e19 and lose the small
-// gradients of a long sum, and the conversion and the addition hide behind the loads.  Each
-// workgroup leaves one partial sum, a second launch adds them in their order: the same inputs give
-// the same bits.
+// A vector's squares (4 or 8) are added in float32, the vectors in float64: float32 alone would lose
+// the small gradients of a long sum, and float64 for every value makes the conversions the bound.
+// Where float32 is no safe place for a vector's squares (a sum past 2^100, or under 2^-100 and not
+// zero) that vector is added in float64.  Each workgroup leaves one partial sum, a second launch adds
+// them in their order: the same inputs give the same bits.
 constexpr int kTensorsN = 128;
 struct ArgsN {
   const void *grad[kTensorsN];
@@ -346,6 +388,18 @@ static_assert(sizeof(ArgsN) <= 4096, "kernel arguments");
 constexpr int kUnrollN = 4;
 
 template <typename T, int N>
+__device__ __forceinline__ double squares(const Vec<T, N> &v) {
+  float s = 0.0f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) s = fmaf(v.get(k), v.get(k), s);
+  if (s > 0x1p-100f && s < 0x1p100f) return (double)s;
+  double d = 0.0;                    // also the way of zeros, infinities and NaN
+#pragma unroll
+  for (int k = 0; k < N; ++k) d = fma((double)v.get(k), (double)v.get(k), d);
+  return d;
+}
+
+template <typename T, int N>
 __device__ __forceinline__ double sum_squares(const T *g, long long n) {
   double s[kUnrollN] = {0, 0, 0, 0};
   long long i = (long long)threadIdx.x * N;
@@ -355,21 +409,12 @@ __device__ __forceinline__ double sum_squares(const T *g, long long n) {
 #pragma unroll
     for (int u = 0; u < kUnrollN; ++u) v[u].load(g + i + u * step);
 #pragma unroll
-    for (int u = 0; u < kUnrollN; ++u)
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const double d = (double)v[u].get(k);
-        s[u] = fma(d, d, s[u]);
-      }
+    for (int u = 0; u < kUnrollN; ++u) s[u] += squares(v[u]);
   }
   for (; i < n; i += step) {
     Vec<T, N> v;
     v.load(g + i, n - i);
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const double d = (double)v.get(k);
-      s[0] = fma(d, d, s[0]);
-    }
+    s[0] += squares(v);
   }
   return (s[0] + s[1]) + (s[2] + s[3]);
 }

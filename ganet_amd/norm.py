@@ -48,68 +48,60 @@ def _rows_stride(t):
 
 
 class _Layout(object):
-    """How a tensor's channels lie in memory: `outer` rows or images, `inner` positions each."""
+    """How a tensor's channels lie in memory, in the order that the tensor itself suggests:
+    `outer` rows (inner = 1) or images of `inner` positions, `stride` values apart."""
+    __slots__ = ("x", "dim", "C", "positions", "outer", "inner", "stride", "channels_last")
 
-    def __init__(self, shape, channel_dim):
-        dim = channel_dim + len(shape) if channel_dim < 0 else channel_dim
-        if not 0 <= dim < len(shape):
+    def __init__(self, x, channel_dim):
+        shape = x.shape
+        dims = len(shape)
+        dim = channel_dim + dims if channel_dim < 0 else channel_dim
+        if not 0 <= dim < dims:
             raise IndexError("layer_norm: channel_dim %d of a %d-dimensional tensor"
-                             % (channel_dim, len(shape)))
-        self.shape, self.dim, self.C = shape, dim, shape[dim]
-        if self.C < 1:
+                             % (channel_dim, dims))
+        C = shape[dim]
+        if C < 1:
             raise ValueError("layer_norm: no channels in %s" % (tuple(shape),))
-        self.positions = 1
-        for d, size in enumerate(shape):
-            if d != dim:
-                self.positions *= size
-        self.inner = 1
-        for size in shape[dim + 1:]:
-            self.inner *= size
-
-    def choose(self, x):
-        """Takes x's own order where the kernels have it.  Returns (x, values between rows or
-        images); sets `rows` and `channels_last`."""
-        self.channels_last = self.dim == 1 and _is_channels_last(x)
-        self.rows = self.channels_last or self.inner <= 1
-        return self.fit(x)
+        self.dim, self.C = dim, C
+        self.positions = n = x.numel() // C
+        self.channels_last = False
+        inner = 1
+        if dim != dims - 1 and n:
+            for size in shape[dim + 1:]:
+                inner *= size
+            if dim == 1 and inner > 1 and _is_channels_last(x):
+                self.channels_last, inner = True, 1
+        self.inner, self.outer = inner, n // inner
+        self.x, self.stride = self.fit(x)
 
     def fit(self, t):
-        """`t` in the chosen order, copied where it is in another."""
-        if self.channels_last:
-            if not _is_channels_last(t):
-                t = t.contiguous(memory_format=torch.channels_last)
-            return t, self.C
-        if self.rows:
-            if self.dim == len(self.shape) - 1:
-                stride = _rows_stride(t)
-                if stride is not None:
-                    return t, stride
-            return t.contiguous(), self.C
+        """(t in this order, values between its rows or images), copied where it is in another."""
         one = self.C * self.inner
-        if self.dim == 1 and t.shape[0] > 0 and t[0].is_contiguous() and (
-                t.shape[0] == 1 or t.stride(0) >= one):
-            return t, t.stride(0) if t.shape[0] > 1 else one
+        if self.channels_last:
+            return (t if _is_channels_last(t)
+                    else t.contiguous(memory_format=torch.channels_last)), one
+        if t.is_contiguous():
+            return t, one
+        if self.dim == t.dim() - 1:
+            stride = _rows_stride(t)
+            if stride is not None:
+                return t, stride
+        elif self.dim == 1 and t.shape[0] > 0 and t[0].is_contiguous():
+            if t.shape[0] == 1:
+                return t, one
+            if t.stride(0) >= one:
+                return t, t.stride(0)
         return t.contiguous(), one
 
-    def empty(self, dtype, device):
-        return torch.empty(self.shape, dtype=dtype, device=device,
-                           memory_format=torch.channels_last if self.channels_last
-                           else torch.contiguous_format)
-
-    def params(self, dtype, weight_dtype, eps):
-        p = _lib.LayerNormParams()
-        p.C, p.dtype, p.weight_dtype, p.eps = self.C, _DTYPES[dtype], _DTYPES[weight_dtype], eps
-        p.inner = 1 if self.rows else self.inner
-        p.outer = self.positions // p.inner if self.positions else 0
-        p.y_stride = self.C * p.inner
-        return p
+    def like(self, x):
+        """An output of the input's memory format."""
+        if self.channels_last:
+            return torch.empty_like(x, memory_format=torch.channels_last)
+        return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
-def _check(x, tensors, C):
-    if not x.is_cuda:
-        raise NotImplementedError
-    if x.dtype not in _DTYPES:
-        raise TypeError("layer_norm: unsupported dtype %s" % x.dtype)
+def _weight_dtype(x, tensors, C):
+    """The (one) dtype of weight and bias, the input's without them; checks them."""
     dtype = None
     for name, t in tensors:
         if t is None:
@@ -118,13 +110,24 @@ def _check(x, tensors, C):
             raise TypeError("layer_norm: unsupported dtype %s of the %s" % (t.dtype, name))
         if dtype is not None and t.dtype != dtype:
             raise TypeError("layer_norm: weight and bias of unlike dtypes")
-        if t.device != x.device:
+        if t.get_device() != x.get_device():
             raise ValueError("layer_norm: %s on %s, input on %s" % (name, t.device, x.device))
-        if tuple(t.shape) != (C,):
+        if t.dim() != 1 or t.numel() != C:
             raise ValueError("layer_norm: %s of shape %s for %d channels"
                              % (name, tuple(t.shape), C))
         dtype = t.dtype
     return dtype or x.dtype
+
+
+def _check_input(x):
+    if not x.is_cuda:
+        raise NotImplementedError
+    if x.dtype not in _DTYPES:
+        raise TypeError("layer_norm: unsupported dtype %s" % x.dtype)
+
+
+def _dense(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def _ptr(t):
@@ -132,26 +135,24 @@ def _ptr(t):
 
 
 def _forward(input, weight, bias, eps, channel_dim, stats):
-    lay = _Layout(input.shape, channel_dim)
-    wdtype = _check(input, (("weight", weight), ("bias", bias)), lay.C)
+    lay = _Layout(input, channel_dim)
+    _check_input(input)
+    wdtype = _weight_dtype(input, (("weight", weight), ("bias", bias)), lay.C)
     if not eps >= 0:
         raise ValueError("layer_norm: eps %r" % (eps,))
     L = _lib.lib()
-    x, stride = lay.choose(input)
-    weight = weight.contiguous() if weight is not None else None
-    bias = bias.contiguous() if bias is not None else None
-    p = lay.params(x.dtype, wdtype, eps)
-    p.x_stride = stride
-    with torch.cuda.device(x.device):
-        out = lay.empty(x.dtype, x.device)
-        mean = rstd = None
-        if stats:
-            mean, rstd = torch.empty((2, lay.positions), dtype=torch.float32,
-                                     device=x.device).unbind(0)
-        rc = L.ganet_layer_norm_forward(
-            x.data_ptr(), _ptr(weight), _ptr(bias), out.data_ptr(), _ptr(mean), _ptr(rstd),
-            ctypes.byref(p), torch.cuda.current_stream(x.device).cuda_stream)
-    _lib.check(rc, "ganet_layer_norm_forward")
+    x, weight, bias = lay.x, _dense(weight), _dense(bias)
+    p = _lib.LayerNormParams(lay.outer, lay.inner, lay.stride, lay.C * lay.inner, 0, lay.C,
+                             _DTYPES[x.dtype], _DTYPES[wdtype], eps)
+    out = lay.like(x)
+    mean = rstd = None
+    if stats:
+        mean = torch.empty(lay.positions, dtype=torch.float32, device=x.device)
+        rstd = torch.empty_like(mean)
+    rc = _lib.call(x.get_device(), L.ganet_layer_norm_forward, x.data_ptr(), _ptr(weight),
+                   _ptr(bias), out.data_ptr(), _ptr(mean), _ptr(rstd), ctypes.byref(p))
+    if rc:
+        _lib.check(rc, "ganet_layer_norm_forward")
     return out, mean, rstd
 
 
@@ -168,15 +169,17 @@ def layer_norm_backward(input, weight, grad_output, mean, rstd, channel_dim=-1,
     """Raw backward: (grad_input, grad_weight, grad_bias), None for what is not asked for.
     grad_input has the memory format of `input`; grad_weight and grad_bias are [C] of the weight's
     dtype (the input's without a weight)."""
-    lay = _Layout(input.shape, channel_dim)
+    lay = _Layout(input, channel_dim)
     if not grad_output.is_cuda:
         raise NotImplementedError
-    wdtype = _check(input, (("weight", weight),), lay.C)
+    _check_input(input)
+    wdtype = _weight_dtype(input, (("weight", weight),), lay.C)
     if grad_output.shape != input.shape:
         raise ValueError("layer_norm: grad_output of shape %s for an input of shape %s"
                          % (tuple(grad_output.shape), tuple(input.shape)))
+    index = input.get_device()
     for t in (grad_output, mean, rstd):
-        if t.device != input.device:
+        if t.get_device() != index:
             raise ValueError("layer_norm: tensors on %s and %s" % (t.device, input.device))
     for t in (mean, rstd):
         if t.dtype != torch.float32 or t.numel() != lay.positions or not t.is_contiguous():
@@ -184,28 +187,28 @@ def layer_norm_backward(input, weight, grad_output, mean, rstd, channel_dim=-1,
     if not (need_input or need_weight or need_bias):
         return None, None, None
     L = _lib.lib()
-    x, x_stride = lay.choose(input)
-    grad, g_stride = lay.fit(grad_output.to(x.dtype))
-    weight = weight.contiguous() if weight is not None else None
-    p = lay.params(x.dtype, wdtype, 0.0)
-    p.x_stride, p.g_stride = x_stride, g_stride
+    x, weight = lay.x, _dense(weight)
+    grad, g_stride = lay.fit(grad_output if grad_output.dtype == x.dtype
+                             else grad_output.to(x.dtype))
+    p = _lib.LayerNormParams(lay.outer, lay.inner, lay.stride, lay.C * lay.inner, g_stride, lay.C,
+                             _DTYPES[x.dtype], _DTYPES[wdtype], 0.0)
+    at = ctypes.byref(p)
     gx = gw = gb = ws = None
     nbytes = 0
-    with torch.cuda.device(x.device):
-        if need_input:
-            gx = lay.empty(x.dtype, x.device)
-        if need_weight:
-            gw = torch.empty(lay.C, dtype=wdtype, device=x.device)
-        if need_bias:
-            gb = torch.empty(lay.C, dtype=wdtype, device=x.device)
-        if need_weight or need_bias:
-            nbytes = L.ganet_layer_norm_backward_workspace_bytes(ctypes.byref(p))
-            ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=x.device)
-        rc = L.ganet_layer_norm_backward(
-            x.data_ptr(), _ptr(weight), grad.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
-            _ptr(gx), _ptr(gw), _ptr(gb), ctypes.byref(p), _ptr(ws), nbytes,
-            torch.cuda.current_stream(x.device).cuda_stream)
-    _lib.check(rc, "ganet_layer_norm_backward")
+    if need_input:
+        gx = lay.like(x)
+    if need_weight:
+        gw = torch.empty(lay.C, dtype=wdtype, device=x.device)
+    if need_bias:
+        gb = torch.empty(lay.C, dtype=wdtype, device=x.device)
+    if need_weight or need_bias:
+        nbytes = L.ganet_layer_norm_backward_workspace_bytes(at)
+        ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=x.device)
+    rc = _lib.call(index, L.ganet_layer_norm_backward, x.data_ptr(), _ptr(weight),
+                   grad.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _ptr(gx), _ptr(gw),
+                   _ptr(gb), at, _ptr(ws), nbytes)
+    if rc:
+        _lib.check(rc, "ganet_layer_norm_backward")
     return gx, gw, gb
 
 

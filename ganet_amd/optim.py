@@ -17,6 +17,9 @@ weights too).  CPU tensors raise NotImplementedError.
 """
 import ctypes
 import math
+from array import array
+from itertools import chain
+from operator import attrgetter
 
 import torch
 
@@ -24,6 +27,12 @@ from . import _lib
 from .dcn import _DTYPES
 
 BLOCK = _lib.GANET_STATE_BLOCK
+
+
+# Attribute reads of a whole list, at C speed: a model's step checks every tensor of every list,
+# and on the host that is what a step over many small tensors costs.
+_ptrs, _sizes, _gpus = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
+_dtypes, _shapes, _plain = attrgetter("dtype"), attrgetter("shape"), torch.Tensor.is_contiguous
 
 
 def _dense(t):
@@ -47,22 +56,25 @@ def _same_order(a, b):
     return all(x == y for x, y, n in zip(a.stride(), b.stride(), a.shape) if n != 1)
 
 
-def _one(tensors, what, device, dtype=None):
-    """Checks that a list's tensors share one device and dtype; returns the dtype."""
-    for t in tensors:
-        if not t.is_cuda:
+def _one(tensors, what, index, dtype=None):
+    """Checks that a list's tensors share one GPU and dtype; returns the dtype."""
+    gpus = set(map(_gpus, tensors))
+    if gpus != {index} or index < 0:
+        if -1 in gpus:
             raise NotImplementedError
-        if dtype is None:
-            dtype = t.dtype
-        if t.dtype != dtype:
-            raise TypeError("adamw: %s of dtypes %s and %s in one call" % (what, dtype, t.dtype))
-        if t.device != device:
-            raise ValueError("adamw: %s on %s and %s in one call" % (what, device, t.device))
-    return dtype
+        raise ValueError("adamw: %s on GPUs %s, parameters on %d" % (what, sorted(gpus), index))
+    found = set(map(_dtypes, tensors))
+    if len(found) != 1 or (dtype is not None and dtype not in found):
+        raise TypeError("adamw: %s of dtypes %s%s" % (
+            what, ", ".join(map(str, found)), "" if dtype is None else ", expected %s" % dtype))
+    return found.pop()
 
 
-def _in_order(params, others, what):
-    for p, t in zip(params, others):
+def _like_params(params, shapes, plain, tensors, what):
+    """Checks that `tensors` have the parameters' shapes and memory order."""
+    if list(map(_shapes, tensors)) == shapes and plain and all(map(_plain, tensors)):
+        return
+    for p, t in zip(params, tensors):
         if not _same_order(p, t):
             raise ValueError("adamw: %s of shape %s and strides %s for a parameter of shape %s and "
                              "strides %s" % (what, tuple(t.shape), t.stride(), tuple(p.shape),
@@ -78,43 +90,53 @@ def _step(params, grads, avgs, seconds, avg_scales, second_scales, bits, step, l
             raise ValueError("adamw: %d %s for %d parameters" % (len(ts), what, n))
     if n == 0:
         return
-    device = params[0].device
-    pdtype = _one(params, "parameters", device)
-    gdtype = _one(grads, "gradients", device)
+    index = params[0].get_device()
+    pdtype = _one(params, "parameters", index)
+    gdtype = _one(grads, "gradients", index)
     for t in (pdtype, gdtype):
         if t not in _DTYPES:
             raise TypeError("adamw: unsupported dtype %s" % t)
     state = torch.float32 if bits == 32 else torch.float8_e4m3fn
-    _one(avgs, "states", device, state)
-    _one(seconds, "states", device, state)
+    _one(avgs, "states", index, state)
+    _one(seconds, "states", index, state)
+    shapes, plain = list(map(_shapes, params)), all(map(_plain, params))
+    if not plain:
+        for p in params:
+            if not _dense(p):
+                raise ValueError("adamw: a parameter of shape %s and strides %s is not dense"
+                                 % (tuple(p.shape), p.stride()))
+    _like_params(params, shapes, plain, avgs, "a state")
+    _like_params(params, shapes, plain, seconds, "a state")
+    sizes = list(map(_sizes, params))
+    none = [0] * n
+    columns = [list(map(_ptrs, params)), None, list(map(_ptrs, avgs)), list(map(_ptrs, seconds)),
+               none, none, none, sizes]
+    written = columns[0] + columns[2] + columns[3]
     if masters is not None:
         if pdtype == torch.float32:
             raise TypeError("adamw: masters of float32 parameters")
-        _one(masters, "masters", device, torch.float32)
-        _in_order(params, masters, "a master")
-    for p in params:
-        if not _dense(p):
-            raise ValueError("adamw: a parameter of shape %s and strides %s is not dense"
-                             % (tuple(p.shape), p.stride()))
-    _in_order(params, avgs, "a state")
-    _in_order(params, seconds, "a state")
+        _one(masters, "masters", index, torch.float32)
+        _like_params(params, shapes, plain, masters, "a master")
+        columns[6] = list(map(_ptrs, masters))
+        written += columns[6]
     if bits == 8:
-        for ts in (avg_scales, second_scales):
-            _one(ts, "scales", device, torch.float32)
-            for p, t in zip(params, ts):
-                if t.numel() != -(-p.numel() // BLOCK) or not t.is_contiguous():
-                    raise ValueError("adamw: a dense scale for each %d values of a parameter "
-                                     "is wanted" % BLOCK)
-    ordered = []                               # gradients in their parameters' order
-    for p, g in zip(params, grads):
-        if g.shape != p.shape:
-            raise ValueError("adamw: a gradient of shape %s for a parameter of shape %s"
-                             % (tuple(g.shape), tuple(p.shape)))
-        if not _same_order(p, g):
-            g = torch.empty_like(p, dtype=gdtype).copy_(g)
-        ordered.append(g)
-    written = [t.data_ptr() for ts in (params, avgs, seconds, masters) if ts is not None
-               for t in ts if t.numel()]
+        blocks = [-(-k // BLOCK) for k in sizes]
+        for at, ts in ((4, avg_scales), (5, second_scales)):
+            _one(ts, "scales", index, torch.float32)
+            if list(map(_sizes, ts)) != blocks or not all(map(_plain, ts)):
+                raise ValueError("adamw: a dense scale for each %d values of a parameter is wanted"
+                                 % BLOCK)
+            columns[at] = list(map(_ptrs, ts))
+        written += columns[4] + columns[5]
+    # gradients in their parameters' order
+    if list(map(_shapes, grads)) != shapes:
+        raise ValueError("adamw: a gradient's shape is not its parameter's")
+    if not (plain and all(map(_plain, grads))):
+        grads = [g if _same_order(p, g) else torch.empty_like(p, dtype=gdtype).copy_(g)
+                 for p, g in zip(params, grads)]
+    columns[1] = list(map(_ptrs, grads))
+    if 0 in sizes:                              # these have no address
+        written = [address for address in written if address]
     if len(set(written)) != len(written):
         raise ValueError("adamw: a tensor is in the lists twice")
 
@@ -123,38 +145,28 @@ def _step(params, grads, avgs, seconds, avg_scales, second_scales, bits, step, l
     h.skip_nonfinite = 1 if skip_nonfinite else 0
     h.beta1, h.beta2, h.eps, h.weight_decay = betas[0], betas[1], eps, weight_decay
     h.seed = int(seed) & 0xFFFFFFFF
-    held = []
     if torch.is_tensor(step):
-        h.step_device = _scalar(step, torch.int64, device, "step", held)
+        h.step_device = _scalar(step, torch.int64, index, "step")
     else:
         h.step = int(step)
     if torch.is_tensor(lr):
-        h.lr_device = _scalar(lr, torch.float32, device, "lr", held)
+        h.lr_device = _scalar(lr, torch.float32, index, "lr")
     else:
         h.lr = lr
     if grad_stats is not None:
         if (grad_stats.dtype != torch.float32 or grad_stats.numel() != 4
-                or grad_stats.device != device or not grad_stats.is_contiguous()):
+                or grad_stats.get_device() != index or not grad_stats.is_contiguous()):
             raise ValueError("adamw: grad_stats is the float32 [4] tensor of grad_norm")
         h.grad_stats = grad_stats.data_ptr()
-    words = []
-    for i in range(n):
-        words += (params[i].data_ptr(), ordered[i].data_ptr(), avgs[i].data_ptr(),
-                  seconds[i].data_ptr(),
-                  avg_scales[i].data_ptr() if avg_scales is not None else 0,
-                  second_scales[i].data_ptr() if second_scales is not None else 0,
-                  masters[i].data_ptr() if masters is not None else 0, params[i].numel())
-    table = (ctypes.c_uint64 * len(words))(*words)
-    with torch.cuda.device(device):
-        rc = _lib.lib().ganet_adamw_step(ctypes.byref(table), n, ctypes.byref(h),
-                                         torch.cuda.current_stream(device).cuda_stream)
-    _lib.check(rc, "ganet_adamw_step")
+    table = array("Q", chain.from_iterable(zip(*columns)))       # rows of ganet_step_tensor
+    rc = _lib.call(index, _lib.lib().ganet_adamw_step, table.buffer_info()[0], n, ctypes.byref(h))
+    if rc:
+        _lib.check(rc, "ganet_adamw_step")
 
 
-def _scalar(t, dtype, device, what, held):
-    if t.dtype != dtype or t.numel() != 1 or t.device != device:
-        raise ValueError("adamw: %s as a tensor is one %s on %s" % (what, dtype, device))
-    held.append(t)
+def _scalar(t, dtype, index, what):
+    if t.dtype != dtype or t.numel() != 1 or t.get_device() != index:
+        raise ValueError("adamw: %s as a tensor is one %s on GPU %d" % (what, dtype, index))
     return t.data_ptr()
 
 
@@ -203,36 +215,37 @@ def grad_norm(grads, max_norm=None, inv_scale=1.0, out=None):
     grads = list(grads)
     if out is None and not grads:
         raise ValueError("grad_norm: no gradients")
-    device = grads[0].device if grads else out.device
-    dense = []
-    for g in grads:
-        if not g.is_cuda:
+    index = (grads[0] if grads else out).get_device()
+    gpus = set(map(_gpus, grads)) or {index}
+    if gpus != {index} or index < 0:
+        if -1 in gpus:
             raise NotImplementedError
-        if g.dtype not in _DTYPES:
-            raise TypeError("grad_norm: unsupported dtype %s" % g.dtype)
-        if g.device != device:
-            raise ValueError("grad_norm: gradients on %s and %s" % (device, g.device))
-        dense.append(g if _dense(g) else g.contiguous())
+        raise ValueError("grad_norm: gradients on GPUs %s" % sorted(gpus))
+    if not all(map(_plain, grads)):
+        grads = [g if _dense(g) else g.contiguous() for g in grads]
+    try:
+        dtypes = array("i", [_DTYPES[t] for t in map(_dtypes, grads)])
+    except KeyError as e:
+        raise TypeError("grad_norm: unsupported dtype %s" % e.args[0])
     max_norm = math.inf if max_norm is None else float(max_norm)
     if not max_norm >= 0 or not math.isfinite(inv_scale):
         raise ValueError("grad_norm: max_norm %r, inv_scale %r" % (max_norm, inv_scale))
     L = _lib.lib()
-    n = len(dense)
-    ptrs = (ctypes.c_void_p * max(n, 1))(*[g.data_ptr() for g in dense])
-    numel = (ctypes.c_int64 * max(n, 1))(*[g.numel() for g in dense])
-    dtypes = (ctypes.c_int32 * max(n, 1))(*[_DTYPES[g.dtype] for g in dense])
-    with torch.cuda.device(device):
-        if out is None:
-            out = torch.empty(4, dtype=torch.float32, device=device)
-        elif (out.dtype != torch.float32 or out.numel() != 4 or out.device != device
-              or not out.is_contiguous()):
-            raise ValueError("grad_norm: out is a float32 [4] tensor on the gradients' device")
-        nbytes = L.ganet_grad_norm_workspace_bytes(numel, n)
-        ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
-        rc = L.ganet_grad_norm(ptrs, numel, dtypes, n, max_norm, inv_scale, out.data_ptr(),
-                               ws.data_ptr(), nbytes,
-                               torch.cuda.current_stream(device).cuda_stream)
-    _lib.check(rc, "ganet_grad_norm")
+    n = len(grads)
+    ptrs, numel = array("Q", map(_ptrs, grads)), array("q", map(_sizes, grads))
+    if out is None:
+        out = torch.empty(4, dtype=torch.float32, device=grads[0].device)
+    elif (out.dtype != torch.float32 or out.numel() != 4 or out.get_device() != index
+          or not out.is_contiguous()):
+        raise ValueError("grad_norm: out is a float32 [4] tensor on the gradients' device")
+    sizes = numel.buffer_info()[0]
+    nbytes = L.ganet_grad_norm_workspace_bytes(sizes, n)
+    ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=out.device)
+    rc = _lib.call(index, L.ganet_grad_norm, ptrs.buffer_info()[0], sizes,
+                   dtypes.buffer_info()[0], n, max_norm, inv_scale, out.data_ptr(), ws.data_ptr(),
+                   nbytes)
+    if rc:
+        _lib.check(rc, "ganet_grad_norm")
     return out
 
 
