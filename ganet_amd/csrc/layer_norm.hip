@@ -292,13 +292,26 @@ __global__ __launch_bounds__(kBwdThreads) void ln_rows_bwd(Args a) {
   extern __shared__ __align__(16) float sums[];      // [groups][columns], for the end
   const int l = (int)threadIdx.x % LANES;
   const int group = (int)threadIdx.x / LANES;
-  float w[NV][N], dw[NV][N], db[NV][N];
+  // Weights stay in registers, or, where a lane has 16 columns or more, in LDS.
+  constexpr bool LDS_W = NV * N >= 16;
+  constexpr int COLS = LANES * NV * N;
+  __shared__ __align__(16) float w_lds[LDS_W ? COLS : 1];
+  float w_reg[LDS_W ? 1 : NV][N], dw[NV][N], db[NV][N];
+  if constexpr (LDS_W) {
+    for (int c = threadIdx.x; c < COLS; c += kBwdThreads) w_lds[c] = c < a.C ? load_weight(a.w, a.wdtype, c, 1.0f) : 0.0f;
+    __syncthreads();
+  }
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    load_weights<N>(a.w, a.wdtype, (v * LANES + l) * N, a.C, 1.0f, w[v]);
+    if constexpr (!LDS_W) load_weights<N>(a.w, a.wdtype, (v * LANES + l) * N, a.C, 1.0f, w_reg[v]);
 #pragma unroll
     for (int k = 0; k < N; ++k) dw[v][k] = db[v][k] = 0.0f;
   }
+  // `at`: l, but not known to be the same in every row, or the loads would move out of the loop and
+  // into registers again
+  auto weight = [&](int at, int v, int k) {
+    return LDS_W ? w_lds[(v * LANES + at) * N + k] : w_reg[LDS_W ? 0 : v][k];
+  };
   Vec<T, N> x[NV], g[NV];
   float mean, rstd;
   auto fetch = [&](long long row) {
@@ -317,7 +330,7 @@ __global__ __launch_bounds__(kBwdThreads) void ln_rows_bwd(Args a) {
       }
     }
   };
-  constexpr bool AHEAD = NV * N <= 8;                // more fill the 128 registers by themselves
+  constexpr bool AHEAD = !LDS_W;                     // 16 columns fill the 128 registers by themselves
   const long long step = (long long)gridDim.x * ROWS;
   const long long first = (long long)blockIdx.x * ROWS;
   if (AHEAD) fetch(first + group);
@@ -334,13 +347,20 @@ __global__ __launch_bounds__(kBwdThreads) void ln_rows_bwd(Args a) {
     const float mu = mean, rs = rstd;
     if (AHEAD && base + step < a.outer) fetch(row + step);
     float s1 = 0.0f, s2 = 0.0f;
+    int at = l;
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
+    for (int v = 0; v < NV; ++v) {
+      // a vector after the other: widened all at once they would not fit the registers
+      if (NV > 1) {
+        xr[v].forget();
+        gr[v].forget();
+        asm volatile("" : "+v"(s1), "+v"(s2), "+v"(at));
+      }
 #pragma unroll
       for (int k = 0; k < N; ++k) {
         // zero past the row's end: grad_y is zero there
         const float xh = (xr[v].get(k) - mu) * rs, dy = gr[v].get(k);
-        const float wa = dy * w[v][k];
+        const float wa = dy * weight(at, v, k);
         s1 += wa;
         s2 += wa * xh;
         if constexpr (SUMS) {
@@ -348,6 +368,7 @@ __global__ __launch_bounds__(kBwdThreads) void ln_rows_bwd(Args a) {
           db[v][k] += dy;
         }
       }
+    }
     if (!a.y) continue;
     float m1, m2;
     if constexpr (LANES <= 64) {
@@ -375,18 +396,16 @@ __global__ __launch_bounds__(kBwdThreads) void ln_rows_bwd(Args a) {
     if (row >= a.outer) continue;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
+      const int c = (v * LANES + l) * N;
       xr[v].forget();
       gr[v].forget();
-    }
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int c = (v * LANES + l) * N;
+      if (NV > 1) asm volatile("" : "+v"(at));
       if (c >= a.C) continue;
       Vec<T, N> d;
 #pragma unroll
       for (int k = 0; k < N; ++k) {
         const float xh = (xr[v].get(k) - mu) * rs;
-        d.set(k, rs * (gr[v].get(k) * w[v][k] - m1 - xh * m2));
+        d.set(k, rs * (gr[v].get(k) * weight(at, v, k) - m1 - xh * m2));
       }
       d.store((T *)a.y + row * a.ys + c, a.C - c);
     }
@@ -394,7 +413,6 @@ __global__ __launch_bounds__(kBwdThreads) void ln_rows_bwd(Args a) {
   if constexpr (SUMS) {
     // The row groups' sums meet in LDS, [groups][columns], the weight's and then the bias's (64 KiB
     // at most), and are added in their order.
-    constexpr int COLS = LANES * NV * N;
     constexpr int GROUPS = LANES < 64 ? kBwdThreads / 64 : ROWS;
     const int mine = LANES < 64 ? (int)threadIdx.x / 64 : group;
     float *out = a.partial + (long long)blockIdx.x * 2 * a.C;
@@ -548,7 +566,7 @@ template <typename T, int VB, int NC, int WAVES, bool SUMS>
 __global__ __launch_bounds__(64 * WAVES) void ln_planes_bwd(Args a, int tiles, int nc) {
   typedef Plane<T, VB, NC, WAVES> P;
   constexpr int N = P::N;
-  __shared__ __align__(16) float part[2][2][WAVES][16][N];
+  __shared__ __align__(16) float part[2][WAVES][16][2 * N];
   __shared__ float weights[P::SLOTS * NC];
   const int c0 = (int)(threadIdx.x >> 4) * nc;
   for (int c = threadIdx.x; c < a.C; c += P::THREADS) weights[c] = load_weight(a.w, a.wdtype, c, 1.0f);
@@ -576,9 +594,9 @@ __global__ __launch_bounds__(64 * WAVES) void ln_planes_bwd(Args a, int tiles, i
     Vec<float, N> mean, rstd;
     mean.load(a.mean + img * a.inner + pos);
     rstd.load(a.rstd + img * a.inner + pos);
-    float m1[N], m2[N];
+    float m[2 * N];                                  // sums of a, of a xh
 #pragma unroll
-    for (int j = 0; j < N; ++j) m1[j] = m2[j] = 0.0f;
+    for (int j = 0; j < 2 * N; ++j) m[j] = 0.0f;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       if (k < nc) {
@@ -586,8 +604,8 @@ __global__ __launch_bounds__(64 * WAVES) void ln_planes_bwd(Args a, int tiles, i
 #pragma unroll
         for (int j = 0; j < N; ++j) {
           const float xh = (vx[k].get(j) - mean.v[j]) * rstd.v[j], dy = vg[k].get(j);
-          m1[j] += dy * w;
-          m2[j] += dy * w * xh;
+          m[j] += dy * w;
+          m[N + j] += dy * w * xh;
           if constexpr (SUMS) {
             const float counted = j >= own ? dy : 0.0f;
             dw[k] += counted * xh;
@@ -598,8 +616,9 @@ __global__ __launch_bounds__(64 * WAVES) void ln_planes_bwd(Args a, int tiles, i
     }
     if (!a.y) continue;
     // two sets of part: the next tile's sums do not wait for this one's readers
-    slots_sum<N, WAVES>(m1, part[turn][0]);
-    slots_sum<N, WAVES>(m2, part[turn][1]);
+    slots_sum<2 * N, WAVES>(m, part[turn]);
+#pragma unroll
+    for (int j = 0; j < 2 * N; ++j) m[j] *= a.inv_c;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       vx[k].forget();
@@ -614,7 +633,7 @@ __global__ __launch_bounds__(64 * WAVES) void ln_planes_bwd(Args a, int tiles, i
 #pragma unroll
         for (int j = 0; j < N; ++j) {
           const float xh = (vx[k].get(j) - mean.v[j]) * rstd.v[j];
-          o.set(j, rstd.v[j] * (vg[k].get(j) * w - m1[j] * a.inv_c - xh * (m2[j] * a.inv_c)));
+          o.set(j, rstd.v[j] * (vg[k].get(j) * w - m[j] - xh * m[N + j]));
         }
         o.store(dx + k * a.inner);
       }
@@ -717,8 +736,11 @@ int with_type(int dtype, F &&f) {
 }
 
 // ---- which kernel ----
-// Rows: the narrowest of these that holds C, i.e. LANES * NV vectors of 16 bytes.
-template <typename T, typename F>
+// Rows: the narrowest of these that holds C, i.e. LANES * NV vectors of 16 bytes.  Forward: one
+// wavefront a row as long as possible, no barrier.  Backward: one vector a lane as long as possible,
+// the registers hold the columns' sums and the next row (rows of 4096 bf16 on 256 lanes of two
+// vectors, without the next row: 76 us for 16384 of them; on 512 lanes of one: ROWS512).
+template <bool BACKWARD, typename T, typename F>
 int with_row_shape(int C, F &&f) {
   const int vecs = (C + kN<T> - 1) / kN<T>;
 #define GANET_ROW(LANES, NV) \
@@ -730,9 +752,15 @@ int with_row_shape(int C, F &&f) {
   GANET_ROW(16, 1);
   GANET_ROW(32, 1);
   GANET_ROW(64, 1);
-  GANET_ROW(64, 2);
-  GANET_ROW(256, 1);
-  GANET_ROW(256, 2);
+  if constexpr (BACKWARD) {
+    GANET_ROW(128, 1);
+    GANET_ROW(256, 1);
+    GANET_ROW(512, 1);
+  } else {
+    GANET_ROW(64, 2);
+    GANET_ROW(256, 1);
+    GANET_ROW(256, 2);
+  }
   GANET_ROW(1024, 1);
   GANET_ROW(1024, 2);
   if constexpr (sizeof(T) == 4) GANET_ROW(1024, 4);
@@ -775,7 +803,7 @@ int backward_blocks(const ganet_layer_norm_params *p) {
   with_type(p->dtype, [&](auto t) {
     typedef decltype(t) T;
     if (p->inner == 1)
-      return with_row_shape<T>(p->C, [&](auto lanes, auto) {
+      return with_row_shape<true, T>(p->C, [&](auto lanes, auto) {
         const long long need = (p->outer + kBwdThreads / lanes.value - 1) / (kBwdThreads / lanes.value);
         blocks = (int)(need < 256 ? need : 256);
         return GANET_OK;
@@ -799,7 +827,7 @@ int backward_blocks(const ganet_layer_norm_params *p) {
 template <typename T>
 int launch_forward(const ganet_layer_norm_params *p, const Args &a, hipStream_t s) {
   if (p->inner == 1)
-    return with_row_shape<T>(p->C, [&](auto lanes, auto nv) {
+    return with_row_shape<false, T>(p->C, [&](auto lanes, auto nv) {
       constexpr int L = lanes.value, NV = nv.value;
       constexpr int threads = L > 256 ? L : 256, rows = threads / L;
       // four vectors of a lane in flight once that still leaves 4 workgroups a CU
@@ -836,7 +864,7 @@ int launch_forward(const ganet_layer_norm_params *p, const Args &a, hipStream_t 
 template <typename T, bool SUMS>
 int launch_backward(const ganet_layer_norm_params *p, const Args &a, int blocks, hipStream_t s) {
   if (p->inner == 1)
-    return with_row_shape<T>(p->C, [&](auto lanes, auto nv) {
+    return with_row_shape<true, T>(p->C, [&](auto lanes, auto nv) {
       constexpr int L = lanes.value, NV = nv.value;
       constexpr int groups = L < 64 ? kBwdThreads / 64 : kBwdThreads / L;
       constexpr size_t room = SUMS ? (size_t)groups * L * NV * kN<T> * sizeof(float) : 0;

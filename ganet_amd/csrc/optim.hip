@@ -20,12 +20,29 @@ using ganet_vec::Vec;
 
 constexpr int kThreads = 256;
 
-// Which of the (at most 64) tensors of a launch a workgroup belongs to: `first` holds the number
-// of the first chunk of each, ascending.
-__device__ __forceinline__ int find_tensor(const int *first, int count, int chunk) {
+// The tensors of a launch: PTRS addresses each, the number of its first chunk, and how many values
+// its last chunk holds (whole chunks precede it, so no length is needed).
+template <int PTRS, int MOST>
+struct Table {
+  static constexpr int most = MOST;
+  void *ptr[PTRS][MOST];
+  int first[MOST + 1];               // [count]: all chunks
+  unsigned short tail[MOST];
+  int count;
+};
+
+// The tensor of a workgroup's chunk: the last that starts at or before it (a tensor without values
+// has no chunk and starts where its successor does).
+template <typename Tab>
+__device__ __forceinline__ int find_tensor(const Tab &tab, int chunk) {
   const int lane = threadIdx.x & 63;
-  const unsigned long long below = __ballot(lane < count && first[lane < count ? lane : 0] <= chunk);
-  return __builtin_amdgcn_readfirstlane(__popcll(below) - 1);
+  int t = -1;
+#pragma unroll
+  for (int base = 0; base < Tab::most; base += 64) {
+    const int i = base + lane < Tab::most ? base + lane : Tab::most - 1;
+    t += __popcll(__ballot(base + lane < tab.count && tab.first[i] <= chunk));
+  }
+  return __builtin_amdgcn_readfirstlane(t);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -75,35 +92,29 @@ __device__ __forceinline__ bool coefficients(const Hyper &h, Coef &c) {
   return true;
 }
 
-constexpr int kTensors32 = 64;
+enum { kParam, kGrad, kAvg, kSecond, kMaster32 };
+template <bool MASTER>
 struct Args32 {
-  void *param[kTensors32];
-  const void *grad[kTensors32];
-  float *m[kTensors32];
-  float *v[kTensors32];
-  float *master[kTensors32];
-  long long n[kTensors32];
-  int first[kTensors32];
-  int count;
+  Table<MASTER ? 5 : 4, MASTER ? 82 : 98> t;
   Hyper h;
 };
-static_assert(sizeof(Args32) <= 4096, "kernel arguments");
+static_assert(sizeof(Args32<true>) <= 4096 && sizeof(Args32<false>) <= 4096, "kernel arguments");
 
 constexpr int kVec32 = 4;       // values of a lane's vector
 constexpr int kUnroll32 = 4;    // vectors of a lane: 16 loads in flight
 constexpr int kChunk32 = kThreads * kVec32 * kUnroll32;
 
 template <typename TP, typename TG, bool MASTER>
-__global__ __launch_bounds__(kThreads) void adamw32_kernel(Args32 a) {
+__global__ __launch_bounds__(kThreads) void adamw32_kernel(Args32<MASTER> a) {
   Coef c;
   if (!coefficients(a.h, c)) return;
-  const int t = find_tensor(a.first, a.count, (int)blockIdx.x);
-  const long long at = (long long)((int)blockIdx.x - a.first[t]) * kChunk32;
-  const long long left = a.n[t] - at;
-  TP *p = (TP *)a.param[t] + at;
-  const TG *g = (const TG *)a.grad[t] + at;
-  float *m = a.m[t] + at, *v = a.v[t] + at;
-  float *w = MASTER ? a.master[t] + at : nullptr;
+  const int t = find_tensor(a.t, (int)blockIdx.x);
+  const long long at = (long long)((int)blockIdx.x - a.t.first[t]) * kChunk32;
+  const int left = (int)blockIdx.x + 1 == a.t.first[t + 1] ? a.t.tail[t] : kChunk32;
+  TP *p = (TP *)a.t.ptr[kParam][t] + at;
+  const TG *g = (const TG *)a.t.ptr[kGrad][t] + at;
+  float *m = (float *)a.t.ptr[kAvg][t] + at, *v = (float *)a.t.ptr[kSecond][t] + at;
+  float *w = MASTER ? (float *)a.t.ptr[MASTER ? kMaster32 : 0][t] + at : nullptr;
 
   Vec<TP, kVec32> vp[kUnroll32];
   Vec<TG, kVec32> vg[kUnroll32];
@@ -152,24 +163,17 @@ __global__ __launch_bounds__(kThreads) void adamw32_kernel(Args32 a) {
 // half of e4m3's spacing (2^-4), and rounding to nearest would stop it for good.  An r above zero
 // never becomes zero (m over a zero r would be a step of m / eps).
 constexpr int kBlock = GANET_STATE_BLOCK;
-constexpr int kTensors8 = 56;
+enum { kAvgScale = 4, kSecondScale, kMaster8 };
+template <bool MASTER>
 struct Args8 {
-  void *param[kTensors8];
-  const void *grad[kTensors8];
-  unsigned char *m[kTensors8];
-  unsigned char *r[kTensors8];
-  float *ms[kTensors8];
-  float *rs[kTensors8];
-  float *master[kTensors8];
-  long long n[kTensors8];
-  int first[kTensors8];
-  int count, tensor0;          // the first tensor's place in the whole list
+  Table<MASTER ? 7 : 6, MASTER ? 62 : 70> t;
+  int tensor0;                 // the first tensor's place in the whole list
   Hyper h;
 };
-static_assert(sizeof(Args8) <= 4096, "kernel arguments");
+static_assert(sizeof(Args8<true>) <= 4096 && sizeof(Args8<false>) <= 4096, "kernel arguments");
 
-constexpr int kVec8 = 8;                            // values of a lane: 32 lanes hold a block
-constexpr int kUnroll8 = 2;
+constexpr int kVec8 = 4;                            // values of a lane: a wavefront holds a block
+constexpr int kUnroll8 = 4;
 constexpr int kChunk8 = kThreads * kVec8 * kUnroll8; // a whole number of blocks
 
 __device__ __forceinline__ unsigned mix32(unsigned x) {
@@ -194,44 +198,45 @@ __device__ __forceinline__ unsigned max3(unsigned a, unsigned b, unsigned c) {
   const unsigned m = b > c ? b : c;
   return a > m ? a : m;
 }
-// The largest of 32 lanes' values
+// The largest of a wavefront's values, in a scalar register
 __device__ __forceinline__ unsigned block_max(unsigned v) {
   auto with = [&](unsigned o) { v = v > o ? v : o; };
   with((unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true));
   with((unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true));
   with((unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true));
   with((unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, true));
-  with((unsigned)__builtin_amdgcn_ds_swizzle((int)v, 0x401F));
-  return v;
+  with((unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, true));   // row 0 -> 1, 2 -> 3
+  with((unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, true));   // row 1 -> 2 and 3
+  return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
 }
 constexpr unsigned kInf = 0x7F800000u;
 
 template <typename TP, typename TG, bool MASTER>
-__global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8 a) {
+__global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8<MASTER> a) {
   Coef c;
   if (!coefficients(a.h, c)) return;
-  const int t = find_tensor(a.first, a.count, (int)blockIdx.x);
-  const long long at = (long long)((int)blockIdx.x - a.first[t]) * kChunk8;
-  const long long left = a.n[t] - at;
-  TP *p = (TP *)a.param[t] + at;
-  const TG *g = (const TG *)a.grad[t] + at;
-  unsigned char *m = a.m[t] + at, *r = a.r[t] + at;
+  const int t = find_tensor(a.t, (int)blockIdx.x);
+  const long long at = (long long)((int)blockIdx.x - a.t.first[t]) * kChunk8;
+  const int left = (int)blockIdx.x + 1 == a.t.first[t + 1] ? a.t.tail[t] : kChunk8;
+  TP *p = (TP *)a.t.ptr[kParam][t] + at;
+  const TG *g = (const TG *)a.t.ptr[kGrad][t] + at;
+  unsigned char *m = (unsigned char *)a.t.ptr[kAvg][t] + at, *r = (unsigned char *)a.t.ptr[kSecond][t] + at;
   const long long block0 = at / kBlock;
-  float *ms = a.ms[t] + block0, *rs = a.rs[t] + block0;
-  float *w = MASTER ? a.master[t] + at : nullptr;
+  float *ms = (float *)a.t.ptr[kAvgScale][t] + block0, *rs = (float *)a.t.ptr[kSecondScale][t] + block0;
+  float *w = MASTER ? (float *)a.t.ptr[MASTER ? kMaster8 : 0][t] + at : nullptr;
   const unsigned key = mix32(c.key + (unsigned)(a.tensor0 + t) * 0x85EBCA6Bu);
-  typedef unsigned char Byte8 __attribute__((ext_vector_type(8), aligned(1)));
+  typedef unsigned char Byte4 __attribute__((ext_vector_type(4), aligned(1)));
 
   Vec<TP, kVec8> vp[kUnroll8];
   Vec<TG, kVec8> vg[kUnroll8];
   Vec<float, kVec8> vw[kUnroll8];
-  unsigned vm[kUnroll8][2], vr[kUnroll8][2];
+  unsigned vm[kUnroll8], vr[kUnroll8];
   float sm[kUnroll8], sr[kUnroll8];
 #pragma unroll
   for (int u = 0; u < kUnroll8; ++u) {
     const int i = (u * kThreads + (int)threadIdx.x) * kVec8;
-    const long long k = left - i;
-    vm[u][0] = vm[u][1] = vr[u][0] = vr[u][1] = 0;
+    const int k = left - i;
+    vm[u] = vr[u] = 0;
     sm[u] = sr[u] = 0.0f;
     vg[u].zero();
     if (k <= 0) continue;
@@ -243,27 +248,21 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8 a) {
     sm[u] = ((const GANET_GLOBAL float *)ms)[i / kBlock];
     sr[u] = ((const GANET_GLOBAL float *)rs)[i / kBlock];
     if (k >= kVec8) {
-      const Byte8 bm = *(const GANET_GLOBAL Byte8 *)(m + i);
-      const Byte8 br = *(const GANET_GLOBAL Byte8 *)(r + i);
-      const unsigned long long wm = __builtin_bit_cast(unsigned long long, bm);
-      const unsigned long long wr = __builtin_bit_cast(unsigned long long, br);
-      vm[u][0] = (unsigned)wm;
-      vm[u][1] = (unsigned)(wm >> 32);
-      vr[u][0] = (unsigned)wr;
-      vr[u][1] = (unsigned)(wr >> 32);
+      vm[u] = __builtin_bit_cast(unsigned, __builtin_nontemporal_load((const GANET_GLOBAL Byte4 *)(m + i)));
+      vr[u] = __builtin_bit_cast(unsigned, __builtin_nontemporal_load((const GANET_GLOBAL Byte4 *)(r + i)));
     } else {
 #pragma unroll
       for (int j = 0; j < kVec8; ++j)
         if (j < k) {
-          vm[u][j >> 2] |= (unsigned)m[i + j] << (8 * (j & 3));
-          vr[u][j >> 2] |= (unsigned)r[i + j] << (8 * (j & 3));
+          vm[u] |= (unsigned)m[i + j] << (8 * j);
+          vr[u] |= (unsigned)r[i + j] << (8 * j);
         }
     }
   }
 #pragma unroll
   for (int u = 0; u < kUnroll8; ++u) {
     const int i = (u * kThreads + (int)threadIdx.x) * kVec8;
-    const long long k = left - i;
+    const int k = left - i;
     float nm[kVec8], nr[kVec8];
     // Magnitudes are compared as integers: the order is the same, and what is not finite comes out
     // on top.
@@ -271,10 +270,8 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8 a) {
     const float b1s = a.h.b1 * sm[u];
 #pragma unroll
     for (int j = 0; j < kVec8; j += 2) {
-      const auto m2 = (j & 2) ? __builtin_amdgcn_cvt_pk_f32_fp8(vm[u][j >> 2], true)
-                              : __builtin_amdgcn_cvt_pk_f32_fp8(vm[u][j >> 2], false);
-      const auto r2 = (j & 2) ? __builtin_amdgcn_cvt_pk_f32_fp8(vr[u][j >> 2], true)
-                              : __builtin_amdgcn_cvt_pk_f32_fp8(vr[u][j >> 2], false);
+      const auto m2 = j ? __builtin_amdgcn_cvt_pk_f32_fp8(vm[u], true) : __builtin_amdgcn_cvt_pk_f32_fp8(vm[u], false);
+      const auto r2 = j ? __builtin_amdgcn_cvt_pk_f32_fp8(vr[u], true) : __builtin_amdgcn_cvt_pk_f32_fp8(vr[u], false);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float gr = vg[u].get(j + e) * c.gscale;
@@ -311,17 +308,17 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8 a) {
     const float ir = tr > 0.0f ? 448.0f * __builtin_amdgcn_rcpf(tr) : 0.0f;
     if (k <= 0) continue;               // after the exchanges between a block's lanes
     const unsigned bkey = mix32(key + (unsigned)(block0 + i / kBlock) * 0xC2B2AE35u);
-    unsigned om[2] = {0, 0}, orr[2] = {0, 0};
+    unsigned om = 0, orr = 0;
     auto value = [&](auto J) {
       constexpr int j = J.value;
       unsigned h = bkey + (unsigned)((i + j) % kBlock) * 0x9E3779B1u;
       h ^= h >> 16;
       h *= 0xBB67AE85u;
       h ^= h >> 15;
-      om[j >> 2] = to_e4m3<(j & 3)>(__builtin_amdgcn_fmed3f(nm[j] * im, -448.0f, 448.0f), h << 16, om[j >> 2]);
+      om = to_e4m3<j>(__builtin_amdgcn_fmed3f(nm[j] * im, -448.0f, 448.0f), h << 16, om);
       // above zero and below e4m3's smallest: the smallest
-      orr[j >> 2] = to_e4m3<(j & 3)>(
-          __builtin_amdgcn_fmed3f(nr[j] * ir, nr[j] > 0.0f ? 0x1p-9f : 0.0f, 448.0f), h & 0xFFFF0000u, orr[j >> 2]);
+      orr = to_e4m3<j>(__builtin_amdgcn_fmed3f(nr[j] * ir, nr[j] > 0.0f ? 0x1p-9f : 0.0f, 448.0f),
+                       h & 0xFFFF0000u, orr);
       const float old = MASTER ? vw[u].get(j) : vp[u].get(j);
       const float part = nm[j] * __builtin_amdgcn_rcpf(fmaf(nr[j], c.rbc2, a.h.eps));
       const float now = fmaf(-c.lr_c, part, old * c.decay);
@@ -332,31 +329,25 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8 a) {
     value(std::integral_constant<int, 1>());
     value(std::integral_constant<int, 2>());
     value(std::integral_constant<int, 3>());
-    value(std::integral_constant<int, 4>());
-    value(std::integral_constant<int, 5>());
-    value(std::integral_constant<int, 6>());
-    value(std::integral_constant<int, 7>());
     if (bad) {
 #pragma unroll
       for (int j = 0; j < kVec8; ++j)
         if (bad >> j & 1) {
-          om[j >> 2] |= 0x7Fu << (8 * (j & 3));
-          orr[j >> 2] |= 0x7Fu << (8 * (j & 3));
+          om |= 0x7Fu << (8 * j);
+          orr |= 0x7Fu << (8 * j);
         }
     }
     if constexpr (MASTER) vw[u].store(w + i, k);
     vp[u].store(p + i, k);
     if (k >= kVec8) {
-      *(GANET_GLOBAL Byte8 *)(m + i) =
-          __builtin_bit_cast(Byte8, (unsigned long long)om[0] | (unsigned long long)om[1] << 32);
-      *(GANET_GLOBAL Byte8 *)(r + i) =
-          __builtin_bit_cast(Byte8, (unsigned long long)orr[0] | (unsigned long long)orr[1] << 32);
+      __builtin_nontemporal_store(__builtin_bit_cast(Byte4, om), (GANET_GLOBAL Byte4 *)(m + i));
+      __builtin_nontemporal_store(__builtin_bit_cast(Byte4, orr), (GANET_GLOBAL Byte4 *)(r + i));
     } else {
 #pragma unroll
       for (int j = 0; j < kVec8; ++j)
         if (j < k) {
-          m[i + j] = (unsigned char)(om[j >> 2] >> (8 * (j & 3)));
-          r[i + j] = (unsigned char)(orr[j >> 2] >> (8 * (j & 3)));
+          m[i + j] = (unsigned char)(om >> (8 * j));
+          r[i + j] = (unsigned char)(orr >> (8 * j));
         }
     }
     if (i % kBlock == 0) {
@@ -374,14 +365,15 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8 a) {
 // Where float32 is no safe place for a vector's squares (a sum past 2^100, or under 2^-100 and not
 // zero) that vector is added in float64.  Each workgroup leaves one partial sum, a second launch adds
 // them in their order: the same inputs give the same bits.
-constexpr int kTensorsN = 128;
+// The list's entries are packed to 12 bytes, so that a launch takes 320 tensors: a lower and an
+// upper address word (48 bits), the first chunk (16 bits), the last chunk's values (30) and the type.
+constexpr int kTensorsN = 320;
 struct ArgsN {
-  const void *grad[kTensorsN];
-  long long n[kTensorsN];
-  int first[kTensorsN];
-  unsigned char dtype[kTensorsN];
+  unsigned low[kTensorsN];
+  unsigned high_first[kTensorsN];
+  unsigned tail_type[kTensorsN];
   int count;
-  long long chunk;
+  unsigned chunks, chunk;
   double *partial;
 };
 static_assert(sizeof(ArgsN) <= 4096, "kernel arguments");
@@ -427,21 +419,23 @@ __device__ __forceinline__ double wave_sum(double v) {
 
 __global__ __launch_bounds__(kThreads) void grad_norm_kernel(ArgsN a) {
   const int lane = threadIdx.x & 63;
-  int t = find_tensor(a.first, a.count < 64 ? a.count : 64, (int)blockIdx.x);
-  if (a.count > 64) {
-    const unsigned long long below =
-        __ballot(lane + 64 < a.count && a.first[lane + 64 < a.count ? lane + 64 : 0] <= (int)blockIdx.x);
-    t = __builtin_amdgcn_readfirstlane(t + __popcll(below));
-  }
-  const long long at = (long long)((int)blockIdx.x - a.first[t]) * a.chunk;
-  const long long n = a.n[t] - at < a.chunk ? a.n[t] - at : a.chunk;
+  int t = -1;
+#pragma unroll
+  for (int base = 0; base < kTensorsN; base += 64)
+    t += __popcll(__ballot(base + lane < a.count && (a.high_first[base + lane] & 0xFFFF) <= blockIdx.x));
+  t = __builtin_amdgcn_readfirstlane(t);
+  const unsigned first = a.high_first[t] & 0xFFFF, type = a.tail_type[t] >> 30;
+  const unsigned next = t + 1 < a.count ? a.high_first[t + 1] & 0xFFFF : a.chunks;
+  const char *g = (const char *)((unsigned long long)(a.high_first[t] >> 16) << 32 | a.low[t]);
+  const long long at = (long long)(blockIdx.x - first) * a.chunk;
+  const long long n = blockIdx.x + 1 == next ? a.tail_type[t] & 0x3FFFFFFF : a.chunk;
   double s;
-  if (a.dtype[t] == GANET_F32)
-    s = sum_squares<float, 4>((const float *)a.grad[t] + at, n);
-  else if (a.dtype[t] == GANET_BF16)
-    s = sum_squares<bf16_t, 8>((const bf16_t *)a.grad[t] + at, n);
+  if (type == GANET_F32)
+    s = sum_squares<float, 4>((const float *)g + at, n);
+  else if (type == GANET_BF16)
+    s = sum_squares<bf16_t, 8>((const bf16_t *)g + at, n);
   else
-    s = sum_squares<f16_t, 8>((const f16_t *)a.grad[t] + at, n);
+    s = sum_squares<f16_t, 8>((const f16_t *)g + at, n);
   __shared__ double part[kThreads / 64];
   s = wave_sum(s);
   if (lane == 0) part[threadIdx.x >> 6] = s;
@@ -479,7 +473,7 @@ __global__ __launch_bounds__(kFinish) void grad_norm_finish_kernel(const double 
 // ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
-constexpr long long kMostValues = 1ll << 40;      // of one tensor: no sum below overflows
+constexpr long long kMostValues = 1ll << 40;      // of one tensor
 constexpr long long kMostBlocks = 1ll << 23;      // of one launch: its threads stay below 2^32
 
 bool dtype_ok(int d) { return d == GANET_F32 || d == GANET_BF16 || d == GANET_F16; }
@@ -498,30 +492,39 @@ int with_types(int pd, int gd, bool master, F &&f) {
   return master ? grad(f16_t(), std::true_type()) : grad(f16_t(), std::false_type());
 }
 
-// Takes the list in launches of at most `most` tensors; chunk numbers into args.first.  A tensor
-// without values keeps its place and gets no chunk (its successor starts at the same number, and a
-// workgroup takes the last tensor that starts at or before its own).
-template <typename Args, typename Fill, typename Launch>
-int in_launches(const ganet_step_tensor *ts, int count, int most, long long chunk, Args &args, Fill &&fill,
+// Takes the list in launches; `ptr(x, k)` is the k-th address of a tensor.
+template <int PTRS, int MOST, typename Ptr, typename Launch>
+int in_launches(const ganet_step_tensor *ts, int count, long long chunk, Table<PTRS, MOST> &tab, Ptr &&ptr,
                 Launch &&launch) {
-  int i = 0;
-  while (i < count) {
+  for (int i = 0; i < count;) {
+    const int start = i;
     int k = 0;
     long long blocks = 0;
-    for (; i < count && k < most; ++i, ++k) {
-      const long long need = (ts[i].n + chunk - 1) / chunk;
+    for (; i < count && k < MOST; ++i, ++k) {
+      const long long n = ts[i].n, need = (n + chunk - 1) / chunk;
       if (need > kMostBlocks) return GANET_ERR_UNSUPPORTED;
       if (blocks + need > kMostBlocks) break;
-      args.first[k] = (int)blocks;
-      fill(k, ts[i], i);
+      tab.first[k] = (int)blocks;
+      tab.tail[k] = (unsigned short)(n - (need - 1) * chunk);      // not read where need == 0
+      for (int j = 0; j < PTRS; ++j) tab.ptr[j][k] = ptr(ts[i], j);
       blocks += need;
     }
+    tab.first[k] = (int)blocks;
+    tab.count = k;
     if (blocks == 0) continue;
-    args.count = k;
-    const int rc = launch((unsigned)blocks);
+    const int rc = launch((unsigned)blocks, start);
     if (rc != GANET_OK) return rc;
   }
   return GANET_OK;
+}
+
+void *address(const ganet_step_tensor &x, int k) {
+  switch (k) {
+    case kParam: return x.param;
+    case kGrad: return const_cast<void *>(x.grad);
+    case kAvg: return x.exp_avg;
+    default: return x.second;
+  }
 }
 
 }  // namespace
@@ -574,49 +577,36 @@ extern "C" int ganet_adamw_step(const ganet_step_tensor *tensors, int count, con
   h.lr_dev = p->lr_device;
 
   hipStream_t s = (hipStream_t)stream;
-  if (!small) {
-    Args32 a;
-    a.h = h;
-    return in_launches(
-        tensors, count, kTensors32, kChunk32, a,
-        [&](int k, const ganet_step_tensor &x, int) {
-          a.param[k] = x.param;
-          a.grad[k] = x.grad;
-          a.m[k] = (float *)x.exp_avg;
-          a.v[k] = (float *)x.second;
-          a.master[k] = x.master;
-          a.n[k] = x.n;
-        },
-        [&](unsigned blocks) {
-          return with_types(p->param_dtype, p->grad_dtype, master, [&](auto tp, auto tg, auto tm) {
-            adamw32_kernel<decltype(tp), decltype(tg), decltype(tm)::value>
-                <<<dim3(blocks), dim3(kThreads), 0, s>>>(a);
+  return with_types(p->param_dtype, p->grad_dtype, master, [&](auto tp, auto tg, auto tm) {
+    typedef decltype(tp) TP;
+    typedef decltype(tg) TG;
+    constexpr bool M = decltype(tm)::value;
+    if (!small) {
+      Args32<M> a;
+      a.h = h;
+      return in_launches(
+          tensors, count, kChunk32, a.t,
+          [](const ganet_step_tensor &x, int k) { return k == kMaster32 ? (void *)x.master : address(x, k); },
+          [&](unsigned blocks, int) {
+            adamw32_kernel<TP, TG, M><<<dim3(blocks), dim3(kThreads), 0, s>>>(a);
             return ganet_check_launch();
           });
-        });
-  }
-  Args8 a;
-  a.h = h;
-  return in_launches(
-      tensors, count, kTensors8, kChunk8, a,
-      [&](int k, const ganet_step_tensor &x, int i) {
-        if (k == 0) a.tensor0 = i;
-        a.param[k] = x.param;
-        a.grad[k] = x.grad;
-        a.m[k] = (unsigned char *)x.exp_avg;
-        a.r[k] = (unsigned char *)x.second;
-        a.ms[k] = x.exp_avg_scale;
-        a.rs[k] = x.second_scale;
-        a.master[k] = x.master;
-        a.n[k] = x.n;
-      },
-      [&](unsigned blocks) {
-        return with_types(p->param_dtype, p->grad_dtype, master, [&](auto tp, auto tg, auto tm) {
-          adamw8_kernel<decltype(tp), decltype(tg), decltype(tm)::value>
-              <<<dim3(blocks), dim3(kThreads), 0, s>>>(a);
+    }
+    Args8<M> a;
+    a.h = h;
+    return in_launches(
+        tensors, count, kChunk8, a.t,
+        [](const ganet_step_tensor &x, int k) {
+          if (k == kAvgScale) return (void *)x.exp_avg_scale;
+          if (k == kSecondScale) return (void *)x.second_scale;
+          return k == kMaster8 ? (void *)x.master : address(x, k);
+        },
+        [&](unsigned blocks, int start) {
+          a.tensor0 = start;
+          adamw8_kernel<TP, TG, M><<<dim3(blocks), dim3(kThreads), 0, s>>>(a);
           return ganet_check_launch();
         });
-      });
+  });
 }
 
 // ---- norm ----
@@ -633,8 +623,11 @@ long long norm_chunk(const int64_t *numel, int count) {
 int norm_list_ok(const int64_t *numel, int count) {
   if (count < 0 || count > (1 << 20)) return GANET_ERR_BAD_SHAPE;
   if (count > 0 && !numel) return GANET_ERR_NULL;
-  for (int i = 0; i < count; ++i)
-    if (numel[i] < 0 || numel[i] > kMostValues) return GANET_ERR_BAD_SHAPE;
+  long long total = 0;                 // below 2^40: a chunk's length fits its 30 bits
+  for (int i = 0; i < count; ++i) {
+    if (numel[i] < 0 || numel[i] > kMostValues || total + numel[i] > kMostValues) return GANET_ERR_BAD_SHAPE;
+    total += numel[i];
+  }
   return GANET_OK;
 }
 }  // namespace
@@ -661,20 +654,24 @@ extern "C" int ganet_grad_norm(const void *const *grads, const int64_t *numel, c
   if (workspace_bytes < ganet_grad_norm_workspace_bytes(numel, count)) return GANET_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
   ArgsN a;
-  a.chunk = norm_chunk(numel, count);
+  const long long chunk = norm_chunk(numel, count);
+  a.chunk = (unsigned)chunk;
   long long done = 0;
   for (int i = 0; i < count;) {
     int k = 0;
     long long blocks = 0;
-    for (; i < count && k < kTensorsN; ++i, ++k) {     // at most 2048 chunks beside one a tensor
-      a.grad[k] = grads[i];
-      a.n[k] = numel[i];
-      a.dtype[k] = (unsigned char)dtypes[i];
-      a.first[k] = (int)blocks;
-      blocks += (numel[i] + a.chunk - 1) / a.chunk;
+    for (; i < count && k < kTensorsN; ++i, ++k) {     // 2048 chunks and one a tensor at most: 16 bits hold them
+      const long long need = (numel[i] + chunk - 1) / chunk;
+      const unsigned long long at = (unsigned long long)grads[i];
+      if (at >> 48) return GANET_ERR_UNSUPPORTED;      // no device address
+      a.low[k] = (unsigned)at;
+      a.high_first[k] = (unsigned)(at >> 32) << 16 | (unsigned)blocks;
+      a.tail_type[k] = (unsigned)dtypes[i] << 30 | (need ? (unsigned)(numel[i] - (need - 1) * chunk) : 0);
+      blocks += need;
     }
     if (blocks == 0) continue;
     a.count = k;
+    a.chunks = (unsigned)blocks;
     a.partial = (double *)workspace + done;
     grad_norm_kernel<<<dim3((unsigned)blocks), dim3(kThreads), 0, s>>>(a);
     const int rc = ganet_check_launch();
