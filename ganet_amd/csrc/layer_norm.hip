@@ -461,24 +461,59 @@ struct Plane {
   static constexpr int THREADS = 64 * WAVES;
 };
 
-// s[N] of each lane, added over the workgroup's slots, in every lane.
-template <int N, int WAVES>
-__device__ __forceinline__ void slots_sum(float (&s)[N], float (*part)[16][N]) {
+// s[M] of each lane, added over the workgroup's slots, in every lane.  First over a wavefront's four
+// rows, two values an exchange, so that each row is left with a quarter of the values; these go
+// through LDS, where a lane adds what it holds over the wavefronts; then the rows hand each other
+// their quarters back.  For M = 16 and 8 wavefronts: 24 exchanges and 9 LDS accesses of 16 bytes
+// without conflicts (every lane summing everything: 32 exchanges through LDS and 36 accesses, bf16
+// backward 32x256x40x100 61 us instead of PLANES16).
+template <int M, int WAVES>
+__device__ __forceinline__ void slots_sum(float (&s)[M], float (*part)[64][M / 4]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int Q = M / 4;
 #pragma unroll
-  for (int k = 0; k < N; ++k) s[k] = ganet_vec::rows_sum(s[k]);
-  if (lane < 16) {
+  for (int i = 0; i < 2 * Q; ++i) {
+    ganet_vec::swap_halves(s[i], s[i + 2 * Q]);
+    s[i] += s[i + 2 * Q];
+  }
 #pragma unroll
-    for (int k = 0; k < N; ++k) part[wave][lane][k] = s[k];
+  for (int i = 0; i < Q; ++i) {
+    ganet_vec::swap_rows(s[i], s[i + Q]);
+    s[i] += s[i + Q];                   // rows: values i, i + Q, i + 2 Q, i + 3 Q
+    part[wave][lane][i] = s[i];
   }
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < N; ++k) s[k] = 0.0f;
+  for (int i = 0; i < Q; ++i) s[i] = part[0][lane][i];
 #pragma unroll
-  for (int i = 0; i < WAVES; ++i)
+  for (int w = 1; w < WAVES; ++w)
 #pragma unroll
-    for (int k = 0; k < N; ++k) s[k] += part[i][lane & 15][k];
+    for (int i = 0; i < Q; ++i) s[i] += part[w][lane][i];
+#pragma unroll
+  for (int i = 0; i < Q; ++i) {
+    s[i + Q] = s[i];
+    ganet_vec::swap_rows(s[i], s[i + Q]);
+  }
+#pragma unroll
+  for (int i = 0; i < 2 * Q; ++i) {
+    s[i + 2 * Q] = s[i];
+    ganet_vec::swap_halves(s[i], s[i + 2 * Q]);
+  }
 }
+
+// The tiles of a workgroup.  Workgroups go to the eight XCDs in turn, and each XCD has an L2 of its
+// own: it gets an eighth of the tiles, neighbours one after another, so that the cache lines that two
+// tiles share (planes start at any address) meet in one L2.
+struct Share {
+  long long end, step, at;
+  __device__ __forceinline__ explicit Share(long long tiles) {
+    const long long per = (tiles + 7) / 8, from = (blockIdx.x & 7) * per;
+    at = from + (blockIdx.x >> 3);
+    end = from + per < tiles ? from + per : tiles;
+    step = (gridDim.x + 7 - (blockIdx.x & 7)) >> 3;
+  }
+  __device__ __forceinline__ long long first() const { return at; }
+};
 
 // Where a lane's N positions begin.  A vector that would pass the plane's end is moved back to end
 // there (the plane holds N positions at least): every lane then loads and stores whole vectors; the
@@ -495,12 +530,14 @@ template <typename T, int VB, int NC, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void ln_planes_fwd(Args a, int tiles, int nc) {
   typedef Plane<T, VB, NC, WAVES> P;
   constexpr int N = P::N;
-  __shared__ __align__(16) float part[2][WAVES][16][N];
+  __shared__ __align__(16) float part[2][WAVES][64][N / 4];
   __shared__ float weights[2][P::SLOTS * NC];
   int own;
-  const long long img = blockIdx.x / tiles;
-  const long long pos = plane_position<N>(
-      (long long)(blockIdx.x % tiles) * P::TILE + (threadIdx.x & 15) * N, a.inner, own);
+  const Share share(a.outer * tiles);
+  const long long i = share.first();
+  if (i >= share.end) return;
+  const long long img = i / tiles;
+  const long long pos = plane_position<N>((i % tiles) * P::TILE + (threadIdx.x & 15) * N, a.inner, own);
   const int c0 = (int)(threadIdx.x >> 4) * nc;       // nc <= NC channels of a slot
   const T *x = (const T *)a.x + img * a.xs + (long long)c0 * a.inner + pos;
   Vec<T, N> v[NC];
@@ -547,7 +584,7 @@ __global__ __launch_bounds__(64 * WAVES) void ln_planes_fwd(Args a, int tiles, i
       Vec<T, N> o;
 #pragma unroll
       for (int j = 0; j < N; ++j) o.set(j, (v[k].get(j) - mean[j]) * rstd[j] * w + b);
-      o.store(y + k * a.inner);
+      o.store_kept(y + k * a.inner);
     }
   }
   if (threadIdx.x < 16 && a.mean) {
@@ -562,11 +599,12 @@ __global__ __launch_bounds__(64 * WAVES) void ln_planes_fwd(Args a, int tiles, i
   }
 }
 
+// Backward: 16 wavefronts a CU (128 registers), however they are grouped.
 template <typename T, int VB, int NC, int WAVES, bool SUMS>
-__global__ __launch_bounds__(64 * WAVES) void ln_planes_bwd(Args a, int tiles, int nc) {
+__global__ __launch_bounds__(64 * WAVES, 4) void ln_planes_bwd(Args a, int tiles, int nc) {
   typedef Plane<T, VB, NC, WAVES> P;
   constexpr int N = P::N;
-  __shared__ __align__(16) float part[2][WAVES][16][2 * N];
+  __shared__ __align__(16) float part[2][WAVES][64][N / 2];
   __shared__ float weights[P::SLOTS * NC];
   const int c0 = (int)(threadIdx.x >> 4) * nc;
   for (int c = threadIdx.x; c < a.C; c += P::THREADS) weights[c] = load_weight(a.w, a.wdtype, c, 1.0f);
@@ -575,7 +613,8 @@ __global__ __launch_bounds__(64 * WAVES) void ln_planes_bwd(Args a, int tiles, i
 #pragma unroll
   for (int k = 0; k < NC; ++k) dw[k] = db[k] = 0.0f;
   int turn = 0;
-  for (long long i = blockIdx.x; i < a.outer * tiles; i += gridDim.x, turn ^= 1) {
+  const Share share(a.outer * tiles);
+  for (long long i = share.first(); i < share.end; i += share.step, turn ^= 1) {
     int own;
     const long long img = i / tiles;
     const long long pos = plane_position<N>((i % tiles) * P::TILE + (threadIdx.x & 15) * N, a.inner, own);
@@ -591,9 +630,11 @@ __global__ __launch_bounds__(64 * WAVES) void ln_planes_bwd(Args a, int tiles, i
         vg[k].load(g + k * a.inner);
       }
     }
-    Vec<float, N> mean, rstd;
-    mean.load(a.mean + img * a.inner + pos);
+    Vec<float, N> shift, rstd;                       // xh = x rstd - mean rstd
+    shift.load(a.mean + img * a.inner + pos);
     rstd.load(a.rstd + img * a.inner + pos);
+#pragma unroll
+    for (int j = 0; j < N; ++j) shift.v[j] *= -rstd.v[j];
     float m[2 * N];                                  // sums of a, of a xh
 #pragma unroll
     for (int j = 0; j < 2 * N; ++j) m[j] = 0.0f;
@@ -603,9 +644,10 @@ __global__ __launch_bounds__(64 * WAVES) void ln_planes_bwd(Args a, int tiles, i
         const float w = c0 + k < a.C ? weights[c0 + k] : 0.0f;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-          const float xh = (vx[k].get(j) - mean.v[j]) * rstd.v[j], dy = vg[k].get(j);
-          m[j] += dy * w;
-          m[N + j] += dy * w * xh;
+          const float xh = fmaf(vx[k].get(j), rstd.v[j], shift.v[j]), dy = vg[k].get(j);
+          const float wa = dy * w;
+          m[j] += wa;
+          m[N + j] = fmaf(wa, xh, m[N + j]);
           if constexpr (SUMS) {
             const float counted = j >= own ? dy : 0.0f;
             dw[k] += counted * xh;
@@ -632,10 +674,10 @@ __global__ __launch_bounds__(64 * WAVES) void ln_planes_bwd(Args a, int tiles, i
         Vec<T, N> o;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-          const float xh = (vx[k].get(j) - mean.v[j]) * rstd.v[j];
+          const float xh = fmaf(vx[k].get(j), rstd.v[j], shift.v[j]);
           o.set(j, rstd.v[j] * (vg[k].get(j) * w - m[j] - xh * m[N + j]));
         }
-        o.store(dx + k * a.inner);
+        o.store_kept(dx + k * a.inner);
       }
     }
   }
@@ -780,18 +822,14 @@ int with_plane_shape(const ganet_layer_norm_params *p, F &&f) {
              std::integral_constant<int, WAVES>())
   GANET_PLANE(16, 4, 4);
   GANET_PLANE(16, 8, 4);
-  if constexpr (!BACKWARD) {
+  if constexpr (BACKWARD) {
+    GANET_PLANE(16, 8, 8);
+    GANET_PLANE(16, 8, 16);
+    GANET_PLANE(8, 16, 16);
+  } else {
     GANET_PLANE(16, 16, 4);
     GANET_PLANE(16, 32, 4);
     GANET_PLANE(16, 32, 8);
-  } else if constexpr (sizeof(T) == 4) {
-    GANET_PLANE(16, 16, 4);
-    GANET_PLANE(16, 16, 8);
-    GANET_PLANE(8, 32, 8);
-  } else {
-    GANET_PLANE(16, 8, 8);
-    GANET_PLANE(8, 16, 8);
-    GANET_PLANE(8, 32, 8);
   }
 #undef GANET_PLANE
   return f(std::integral_constant<int, kAny>(), std::integral_constant<int, 1>(), std::integral_constant<int, 1>());
@@ -815,7 +853,7 @@ int backward_blocks(const ganet_layer_norm_params *p) {
       } else {
         typedef Plane<T, vb.value, nc.value, waves.value> P;
         const long long need = p->outer * tiles_of(p, P::TILE);
-        const int most = waves.value == 8 ? 256 : 512;        // two wavefronts a SIMD
+        const int most = 256 * 16 / waves.value;              // sixteen wavefronts a CU
         blocks = (int)(need < most ? need : most);
       }
       return GANET_OK;
@@ -854,7 +892,7 @@ int launch_forward(const ganet_layer_norm_params *p, const Args &a, hipStream_t 
       const long long tiles = tiles_of(p, P::TILE);
       if (p->outer * tiles > kMostBlocks) return (int)GANET_ERR_UNSUPPORTED;
       ln_planes_fwd<T, vb.value, nc.value, waves.value>
-          <<<dim3((unsigned)(p->outer * tiles)), dim3(P::THREADS), 0, s>>>(a, (int)tiles,
+          <<<dim3((unsigned)((p->outer * tiles + 7) / 8 * 8)), dim3(P::THREADS), 0, s>>>(a, (int)tiles,
                                                                           (p->C + P::SLOTS - 1) / P::SLOTS);
     }
     return ganet_check_launch();

@@ -63,6 +63,9 @@ struct Vec {
   __device__ __forceinline__ void store(T *p) const {
     __builtin_nontemporal_store((Mem)v, (GANET_GLOBAL Mem *)(p));
   }
+  // ... or may come again (a line that a neighbour shares)
+  __device__ __forceinline__ void load_kept(const T *p) { v = *(const GANET_GLOBAL Mem *)(p); }
+  __device__ __forceinline__ void store_kept(T *p) const { *(GANET_GLOBAL Mem *)(p) = (Mem)v; }
   // To the compiler the values may have changed here: it widens them again afterwards (one
   // instruction a value at most) instead of keeping the wide ones, twice the registers.
   __device__ __forceinline__ void forget() {
@@ -98,46 +101,40 @@ struct Vec {
   }
 };
 
-// ---- lane exchanges without LDS: groups of 2, 4, 8 and 16 lanes by DPP, 32 by a swizzle, 64 by
-// the row broadcasts' counterpart (ds_bpermute) --------------------------------------------------
+// ---- sums over lanes without LDS: DPP within a row of 16, then gfx950's row and half swaps --------
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
   return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xf, 0xf, true));
 }
-// the value of a partner lane; applied for 2, 4, ... W each lane has met all W of its group
-template <int W>
-__device__ __forceinline__ float partner(float v) {
-  if constexpr (W == 2) return dpp<0xB1>(v);         // quad_perm [1,0,3,2]
-  if constexpr (W == 4) return dpp<0x4E>(v);         // quad_perm [2,3,0,1]
-  if constexpr (W == 8) return dpp<0x141>(v);        // row_half_mirror
-  if constexpr (W == 16) return dpp<0x140>(v);       // row_mirror
-  if constexpr (W == 32)
-    return __uint_as_float(__builtin_amdgcn_ds_swizzle(__float_as_uint(v), 0x401F));  // lane ^ 16
-  return __shfl_xor(v, 32);
+// a's odd rows of 16 lanes change places with b's even ones: a = {a0, b0, a2, b2}, b = {a1, b1, a3, b3}
+__device__ __forceinline__ void swap_rows(float &a, float &b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  a = __uint_as_float(r[0]);
+  b = __uint_as_float(r[1]);
 }
+// a's upper 32 lanes change places with b's lower ones: a = {a_low, b_low}, b = {a_high, b_high}
+__device__ __forceinline__ void swap_halves(float &a, float &b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  a = __uint_as_float(r[0]);
+  b = __uint_as_float(r[1]);
+}
+// The sum over each group of W neighbouring lanes, in all of them.
 template <int W>
 __device__ __forceinline__ float group_sum(float v) {
-  if constexpr (W >= 2) v += partner<2>(v);
-  if constexpr (W >= 4) v += partner<4>(v);
-  if constexpr (W >= 8) v += partner<8>(v);
-  if constexpr (W >= 16) v += partner<16>(v);
-  if constexpr (W >= 32) v += partner<32>(v);
-  if constexpr (W >= 64) v += partner<64>(v);
-  return v;
-}
-// The sum over the four rows of 16 lanes of a wavefront, in each of them.
-__device__ __forceinline__ float rows_sum(float v) {
-  v += partner<32>(v);
-  return v + partner<64>(v);
-}
-template <int W>
-__device__ __forceinline__ float group_max(float v) {   // of values that are not NaN
-  if constexpr (W >= 2) v = fmaxf(v, partner<2>(v));
-  if constexpr (W >= 4) v = fmaxf(v, partner<4>(v));
-  if constexpr (W >= 8) v = fmaxf(v, partner<8>(v));
-  if constexpr (W >= 16) v = fmaxf(v, partner<16>(v));
-  if constexpr (W >= 32) v = fmaxf(v, partner<32>(v));
-  if constexpr (W >= 64) v = fmaxf(v, partner<64>(v));
+  if constexpr (W >= 2) v += dpp<0xB1>(v);      // quad_perm [1,0,3,2]
+  if constexpr (W >= 4) v += dpp<0x4E>(v);      // quad_perm [2,3,0,1]
+  if constexpr (W >= 8) v += dpp<0x141>(v);     // row_half_mirror
+  if constexpr (W >= 16) v += dpp<0x140>(v);    // row_mirror
+  if constexpr (W >= 32) {
+    float o = v;
+    swap_rows(v, o);
+    v += o;
+  }
+  if constexpr (W >= 64) {
+    float o = v;
+    swap_halves(v, o);
+    v += o;
+  }
   return v;
 }
 
