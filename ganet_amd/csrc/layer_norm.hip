@@ -209,8 +209,8 @@ __device__ __forceinline__ float row_sum(float v, float *part, int slot) {
   }
 }
 
-// Forward.  R rows of a lane are loaded before the first is worked on: 64 bytes a lane in flight
-// where rows are plenty.
+// Forward.  R rows of a lane are loaded before the first is worked on.  The accesses are ordinary
+// ones: marked as not coming again (as elsewhere here) they cost 2 to 5 % in this kernel.
 template <typename T, int LANES, int NV, int R>
 __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_rows_fwd(Args a) {
   constexpr int N = kN<T>;
@@ -227,7 +227,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_rows_fwd(Args a)
     for (int v = 0; v < NV; ++v) {
       const int c = (v * LANES + l) * N;
       if (row < a.outer && c < a.C)
-        x[r][v].load((const T *)a.x + row * a.xs + c, a.C - c);
+        x[r][v].load_kept((const T *)a.x + row * a.xs + c, a.C - c);
       else
         x[r][v].zero();
     }
@@ -269,7 +269,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_rows_fwd(Args a)
       Vec<T, N> y;
 #pragma unroll
       for (int k = 0; k < N; ++k) y.set(k, (x[r][v].get(k) - mean) * rstd * w[v][k] + b[v][k]);
-      y.store((T *)a.y + row * a.ys + c, a.C - c);
+      y.store_kept((T *)a.y + row * a.ys + c, a.C - c);
     }
     if (l == 0 && a.mean) {
       a.mean[row] = mean;
@@ -407,7 +407,7 @@ __global__ __launch_bounds__(kBwdThreads) void ln_rows_bwd(Args a) {
         const float xh = (xr[v].get(k) - mu) * rs;
         d.set(k, rs * (gr[v].get(k) * weight(at, v, k) - m1 - xh * m2));
       }
-      d.store((T *)a.y + row * a.ys + c, a.C - c);
+      d.store_kept((T *)a.y + row * a.ys + c, a.C - c);
     }
   }
   if constexpr (SUMS) {
@@ -694,15 +694,15 @@ __global__ __launch_bounds__(64 * WAVES, 4) void ln_planes_bwd(Args a, int tiles
   }
 }
 
-// Adds the workgroups' sums: 32 channels a workgroup (whole 128-byte lines), its 32 half wavefronts
-// take every 32nd of the `n` <= 512 partial rows, eight loads at a time: latency is all there is.
-// blockIdx.y: 0 the weight's gradient, 1 the bias's.
+// Adds the workgroups' sums: 16 channels a workgroup, its 64 groups of 16 lanes take every 64th of
+// the `n` partial rows, eight loads at a time: latency is all there is.  blockIdx.y: 0 the weight's
+// gradient, 1 the bias's.
 constexpr int kFinish = 1024;
-constexpr int kFinishCols = 32;
+constexpr int kFinishCols = 16;
 __global__ __launch_bounds__(kFinish) void ln_finish(const float *partial, int n, int C, void *dw, void *db,
                                                      int dtype) {
   constexpr int SLOTS = kFinish / kFinishCols;
-  __shared__ float part[SLOTS][kFinishCols];
+  __shared__ float part[kFinish / 64][kFinishCols];
   const int col = threadIdx.x % kFinishCols, slot = threadIdx.x / kFinishCols;
   const int c = blockIdx.x * kFinishCols + col;
   void *out = blockIdx.y ? db : dw;
@@ -716,12 +716,18 @@ __global__ __launch_bounds__(kFinish) void ln_finish(const float *partial, int n
 #pragma unroll
     for (int u = 0; u < 8; ++u) s += f[u];
   }
-  part[slot][col] = s;
+  float o = s;
+  ganet_vec::swap_rows(s, o);
+  s += o;
+  o = s;
+  ganet_vec::swap_halves(s, o);
+  s += o;
+  if ((threadIdx.x & 63) < kFinishCols) part[threadIdx.x >> 6][col] = s;
   __syncthreads();
   if (slot != 0 || c >= C) return;
   s = 0.0f;
 #pragma unroll
-  for (int i = 0; i < SLOTS; ++i) s += part[i][col];
+  for (int i = 0; i < kFinish / 64; ++i) s += part[i][col];
   if (dtype == GANET_F32)
     store1((float *)out + c, s);
   else if (dtype == GANET_BF16)
@@ -778,10 +784,12 @@ int with_type(int dtype, F &&f) {
 }
 
 // ---- which kernel ----
-// Rows: the narrowest of these that holds C, i.e. LANES * NV vectors of 16 bytes.  Forward: one
-// wavefront a row as long as possible, no barrier.  Backward: one vector a lane as long as possible,
-// the registers hold the columns' sums and the next row (rows of 4096 bf16 on 256 lanes of two
-// vectors, without the next row: 76 us for 16384 of them; on 512 lanes of one: ROWS512).
+// Rows: the narrowest of these that holds C, i.e. LANES * NV vectors of 16 bytes.  Forward: a
+// wavefront a row while two vectors a lane do; then four vectors a lane rather than more wavefronts at
+// the barriers for 16-bit values (2048 rows of 16384: 512 lanes of four 33 us, 1024 of two 39 us),
+// the other way round for float32 (8192 rows of 4096: 256 lanes of four 54 us, 1024 of one 48 us).
+// Backward: one vector a lane as long as possible, the registers hold the columns' sums and the next
+// row (16384 rows of 4096 bf16: 512 lanes of one 70 us, 256 of two, without the next row, 76 us).
 template <bool BACKWARD, typename T, typename F>
 int with_row_shape(int C, F &&f) {
   const int vecs = (C + kN<T> - 1) / kN<T>;
@@ -803,9 +811,14 @@ int with_row_shape(int C, F &&f) {
     GANET_ROW(256, 1);
     GANET_ROW(256, 2);
   }
-  GANET_ROW(1024, 1);
-  GANET_ROW(1024, 2);
-  if constexpr (sizeof(T) == 4) GANET_ROW(1024, 4);
+  if constexpr (!BACKWARD && sizeof(T) == 2) {
+    GANET_ROW(256, 4);
+    GANET_ROW(512, 4);
+  } else {
+    GANET_ROW(1024, 1);
+    GANET_ROW(1024, 2);
+    if constexpr (sizeof(T) == 4) GANET_ROW(1024, 4);
+  }
 #undef GANET_ROW
   return GANET_ERR_UNSUPPORTED;           // past GANET_LAYER_NORM_MAX_C
 }
@@ -868,17 +881,16 @@ int launch_forward(const ganet_layer_norm_params *p, const Args &a, hipStream_t 
     return with_row_shape<false, T>(p->C, [&](auto lanes, auto nv) {
       constexpr int L = lanes.value, NV = nv.value;
       constexpr int threads = L > 256 ? L : 256, rows = threads / L;
-      // four vectors of a lane in flight once that still leaves 4 workgroups a CU
-      constexpr int R = NV == 1 ? 4 : (NV == 2 ? 2 : 1);
+      // Two rows a lane (all their loads first, the weights read once for both) where that leaves
+      // half of the chip's threads busy: 512000 rows of 64 bf16 24 us (one: 27, four: 26).
+      constexpr int R = 2;
       const long long many = (p->outer + rows * R - 1) / (rows * R);
-      const bool deep = R > 1 && L <= 64 && many >= 1024;
+      const bool deep = many * threads >= 256 * 1024;
       const long long blocks = deep ? many : (p->outer + rows - 1) / rows;
       if (blocks > kMostBlocks) return (int)GANET_ERR_UNSUPPORTED;
-      if constexpr (R > 1 && L <= 64) {
-        if (deep) {
-          ln_rows_fwd<T, L, NV, R><<<dim3((unsigned)blocks), dim3(threads), 0, s>>>(a);
-          return ganet_check_launch();
-        }
+      if (deep) {
+        ln_rows_fwd<T, L, NV, R><<<dim3((unsigned)blocks), dim3(threads), 0, s>>>(a);
+        return ganet_check_launch();
       }
       ln_rows_fwd<T, L, NV, 1><<<dim3((unsigned)blocks), dim3(threads), 0, s>>>(a);
       return ganet_check_launch();

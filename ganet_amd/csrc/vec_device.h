@@ -63,9 +63,20 @@ struct Vec {
   __device__ __forceinline__ void store(T *p) const {
     __builtin_nontemporal_store((Mem)v, (GANET_GLOBAL Mem *)(p));
   }
-  // ... or may come again (a line that a neighbour shares)
-  __device__ __forceinline__ void load_kept(const T *p) { v = *(const GANET_GLOBAL Mem *)(p); }
+  // ... or is read by what follows, or shares its lines with a neighbour
+  __device__ __forceinline__ void load_kept(const T *p, long long k) {
+    if (k >= N)
+      v = *(const GANET_GLOBAL Mem *)(p);
+    else
+      load(p, k);
+  }
   __device__ __forceinline__ void store_kept(T *p) const { *(GANET_GLOBAL Mem *)(p) = (Mem)v; }
+  __device__ __forceinline__ void store_kept(T *p, long long k) const {
+    if (k >= N)
+      store_kept(p);
+    else
+      store(p, k);
+  }
   // To the compiler the values may have changed here: it widens them again afterwards (one
   // instruction a value at most) instead of keeping the wide ones, twice the registers.
   __device__ __forceinline__ void forget() {
