@@ -215,6 +215,20 @@ def lib():
     return _lib
 
 
+def tensor_lists():
+    """The host extension that reads lists of tensors (csrc/tensor_lists.cpp)."""
+    global tensor_lists
+    try:
+        from . import _tensor_lists as module
+    except ImportError as e:
+        raise RuntimeError("ganet_amd: _tensor_lists.so is missing or does not load (%s) - build it "
+                           "with `python -m ganet_amd.build`" % e)
+
+    def tensor_lists():
+        return module
+    return module
+
+
 def call(index, fn, *args):
     """fn(*args, stream) with GPU `index` current, on torch's current stream there.  The device
     guard and the stream object cost 3 us a call: both are left out where they change nothing."""

@@ -6,6 +6,7 @@ GPU box with the source snapshot.  hipcc cross-compiles without a GPU.
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -30,6 +31,28 @@ SOURCES = ["api.hip", "decode.hip", "deform_conv.hip", "deform_conv_cts.hip", "d
 
 def _newer(a, b):
     return (not os.path.exists(b)) or os.path.getmtime(a) > os.path.getmtime(b)
+
+
+LISTS = os.path.join(HERE, "_tensor_lists.so")
+
+
+def build_lists(force=False, verbose=False):
+    """The host extension ganet_amd/_tensor_lists.so (csrc/tensor_lists.cpp, no GPU code)."""
+    src = os.path.join(CSRC, "tensor_lists.cpp")
+    if not force and not _newer(src, LISTS):
+        return LISTS
+    import sysconfig
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI]
+    cmd += ["-isystem" + p for p in include_paths()] + ["-I" + sysconfig.get_paths()["include"]]
+    cmd += [src, "-o", LISTS] + ["-L" + p for p in library_paths()]
+    cmd += ["-ltorch_python", "-ltorch_cpu", "-lc10"]
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.check_call(cmd)
+    return LISTS
 
 
 def _variant_flags():
@@ -67,7 +90,7 @@ def build_lib(force=False, verbose=False):
         # the library is newer than everything it is built from: on the GPU box the
         # objects do not travel (.gpurunignore) but the library does, and is used as it is
         return LIB
-    objs, relink = [], force or not os.path.exists(LIB)
+    objs, jobs, relink = [], [], force or not os.path.exists(LIB)
     # flags named after one source file only rebuild that file; the rest are the product's objects
     only = {"-DGANET_RING": "deform_conv_ring.hip", "-DGANET_STREAM": "deform_conv_stream.hip",
             "-DGANET_DECODE": "decode.hip", "-DGANET_TAPS": "deform_conv.hip"}
@@ -88,8 +111,10 @@ def build_lib(force=False, verbose=False):
             cmd = [hipcc] + COMMON + extra + PER_FILE.get(src, []) + ["-c", s, "-o", o]
             if verbose:
                 print(" ".join(cmd))
-            subprocess.check_call(cmd)
+            jobs.append(cmd)
             relink = True
+    with ThreadPoolExecutor(min(8, int(os.environ.get("MAX_JOBS", 8)))) as pool:
+        list(pool.map(subprocess.check_call, jobs))
     if relink:
         cmd = [hipcc, "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", LIB] + objs
         if verbose:
@@ -100,3 +125,4 @@ def build_lib(force=False, verbose=False):
 
 if __name__ == "__main__":
     print(build_lib(force="--force" in sys.argv, verbose=True))
+    print(build_lists(force="--force" in sys.argv, verbose=True))

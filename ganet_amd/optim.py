@@ -29,8 +29,6 @@ from .dcn import _DTYPES
 BLOCK = _lib.GANET_STATE_BLOCK
 
 
-# Attribute reads of a whole list, at C speed: a model's step checks every tensor of every list,
-# and on the host that is what a step over many small tensors costs.
 _ptrs, _sizes, _gpus = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
 _dtypes, _shapes, _plain = attrgetter("dtype"), attrgetter("shape"), torch.Tensor.is_contiguous
 
@@ -81,15 +79,15 @@ def _like_params(params, shapes, plain, tensors, what):
                                              p.stride()))
 
 
-def _step(params, grads, avgs, seconds, avg_scales, second_scales, bits, step, lr, betas, eps,
-          weight_decay, masters, grad_stats, skip_nonfinite, seed):
+def _table(params, grads, avgs, seconds, avg_scales, second_scales, masters, bits):
+    """(GPU, parameters' dtype, gradients' dtype, rows of ganet_step_tensor, what they point into):
+    any order of memory, and the errors of what cannot be stepped.  Plain lists (contiguous, nothing
+    wrong) do not come here: _lib.tensor_lists().step reads them."""
     n = len(params)
     for what, ts in (("gradients", grads), ("exp_avgs", avgs), ("second moments", seconds),
                      ("masters", masters), ("scales", avg_scales), ("scales", second_scales)):
         if ts is not None and len(ts) != n:
             raise ValueError("adamw: %d %s for %d parameters" % (len(ts), what, n))
-    if n == 0:
-        return
     index = params[0].get_device()
     pdtype = _one(params, "parameters", index)
     gdtype = _one(grads, "gradients", index)
@@ -139,12 +137,26 @@ def _step(params, grads, avgs, seconds, avg_scales, second_scales, bits, step, l
         written = [address for address in written if address]
     if len(set(written)) != len(written):
         raise ValueError("adamw: a tensor is in the lists twice")
+    rows = array("Q", chain.from_iterable(zip(*columns))).tobytes()
+    return index, _DTYPES[pdtype], _DTYPES[gdtype], rows, grads
 
-    h = _lib.AdamwParams()
-    h.param_dtype, h.grad_dtype, h.state_bits = _DTYPES[pdtype], _DTYPES[gdtype], bits
-    h.skip_nonfinite = 1 if skip_nonfinite else 0
-    h.beta1, h.beta2, h.eps, h.weight_decay = betas[0], betas[1], eps, weight_decay
-    h.seed = int(seed) & 0xFFFFFFFF
+
+def _step(params, grads, avgs, seconds, avg_scales, second_scales, bits, step, lr, betas, eps,
+          weight_decay, masters, grad_stats, skip_nonfinite, seed):
+    n = len(params)
+    lists = (params, grads, avgs, seconds, avg_scales, second_scales, masters)
+    found = _lib.tensor_lists().step(*lists, BLOCK)
+    if (found is not None and max(found[1:3]) < 3 and found[3] == (0 if bits == 32 else 3)
+            and not (masters is not None and found[1] == 0)):
+        index, ptype, gtype, _, rows = found
+    elif n or any(lists[1:]):
+        if not n:
+            raise ValueError("adamw: no parameters")
+        index, ptype, gtype, rows, grads = _table(*lists, bits)
+    else:
+        return
+    h = _lib.AdamwParams(ptype, gtype, bits, 1 if skip_nonfinite else 0, 0, int(seed) & 0xFFFFFFFF,
+                         0, 0.0, betas[0], betas[1], eps, weight_decay)
     if torch.is_tensor(step):
         h.step_device = _scalar(step, torch.int64, index, "step")
     else:
@@ -158,8 +170,7 @@ def _step(params, grads, avgs, seconds, avg_scales, second_scales, bits, step, l
                 or grad_stats.get_device() != index or not grad_stats.is_contiguous()):
             raise ValueError("adamw: grad_stats is the float32 [4] tensor of grad_norm")
         h.grad_stats = grad_stats.data_ptr()
-    table = array("Q", chain.from_iterable(zip(*columns)))       # rows of ganet_step_tensor
-    rc = _lib.call(index, _lib.lib().ganet_adamw_step, table.buffer_info()[0], n, ctypes.byref(h))
+    rc = _lib.call(index, _lib.lib().ganet_adamw_step, rows, n, ctypes.byref(h))
     if rc:
         _lib.check(rc, "ganet_adamw_step")
 
@@ -213,6 +224,33 @@ def grad_norm(grads, max_norm=None, inv_scale=1.0, out=None):
     0 where the norm is not finite.  Nothing waits for the device; adamw_step and
     adamw_step_8bit take the tensor as grad_stats.  Gradients of several dtypes may be mixed."""
     grads = list(grads)
+    n = len(grads)
+    found = _lib.tensor_lists().grads(grads)
+    if found is not None:
+        index, ptrs, numel, dtypes = found
+    else:
+        index, ptrs, numel, dtypes, grads = _read_grads(grads, out)
+    max_norm = math.inf if max_norm is None else float(max_norm)
+    if not max_norm >= 0 or not math.isfinite(inv_scale):
+        raise ValueError("grad_norm: max_norm %r, inv_scale %r" % (max_norm, inv_scale))
+    L = _lib.lib()
+    if out is None:
+        out = torch.empty(4, dtype=torch.float32, device=grads[0].device)
+    elif (out.dtype != torch.float32 or out.numel() != 4 or out.get_device() != index
+          or not out.is_contiguous()):
+        raise ValueError("grad_norm: out is a float32 [4] tensor on the gradients' device")
+    nbytes = L.ganet_grad_norm_workspace_bytes(numel, n)
+    ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=out.device)
+    rc = _lib.call(index, L.ganet_grad_norm, ptrs, numel, dtypes, n, max_norm, inv_scale,
+                   out.data_ptr(), ws.data_ptr(), nbytes)
+    if rc:
+        _lib.check(rc, "ganet_grad_norm")
+    return out
+
+
+def _read_grads(grads, out):
+    """(GPU, addresses, sizes, dtypes, tensors) of gradients that are not all contiguous, and the
+    errors of what is none."""
     if out is None and not grads:
         raise ValueError("grad_norm: no gradients")
     index = (grads[0] if grads else out).get_device()
@@ -221,32 +259,13 @@ def grad_norm(grads, max_norm=None, inv_scale=1.0, out=None):
         if -1 in gpus:
             raise NotImplementedError
         raise ValueError("grad_norm: gradients on GPUs %s" % sorted(gpus))
-    if not all(map(_plain, grads)):
-        grads = [g if _dense(g) else g.contiguous() for g in grads]
+    grads = [g if _dense(g) else g.contiguous() for g in grads]
     try:
         dtypes = array("i", [_DTYPES[t] for t in map(_dtypes, grads)])
     except KeyError as e:
         raise TypeError("grad_norm: unsupported dtype %s" % e.args[0])
-    max_norm = math.inf if max_norm is None else float(max_norm)
-    if not max_norm >= 0 or not math.isfinite(inv_scale):
-        raise ValueError("grad_norm: max_norm %r, inv_scale %r" % (max_norm, inv_scale))
-    L = _lib.lib()
-    n = len(grads)
-    ptrs, numel = array("Q", map(_ptrs, grads)), array("q", map(_sizes, grads))
-    if out is None:
-        out = torch.empty(4, dtype=torch.float32, device=grads[0].device)
-    elif (out.dtype != torch.float32 or out.numel() != 4 or out.get_device() != index
-          or not out.is_contiguous()):
-        raise ValueError("grad_norm: out is a float32 [4] tensor on the gradients' device")
-    sizes = numel.buffer_info()[0]
-    nbytes = L.ganet_grad_norm_workspace_bytes(sizes, n)
-    ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=out.device)
-    rc = _lib.call(index, L.ganet_grad_norm, ptrs.buffer_info()[0], sizes,
-                   dtypes.buffer_info()[0], n, max_norm, inv_scale, out.data_ptr(), ws.data_ptr(),
-                   nbytes)
-    if rc:
-        _lib.check(rc, "ganet_grad_norm")
-    return out
+    return (index, array("Q", map(_ptrs, grads)).tobytes(), array("q", map(_sizes, grads)).tobytes(),
+            dtypes.tobytes(), grads)
 
 
 class AdamW(torch.optim.Optimizer):
