@@ -18,13 +18,12 @@ LIB, OBJ_DIR = _PRODUCT_LIB, _PRODUCT_OBJ
 ARCH = "gfx950"
 COMMON = ["-O3", "--offload-arch=" + ARCH, "-fPIC", "-std=c++17",
           "-I" + os.path.join(ROOT, "include"), "-I" + CSRC,
-          "-Wall", "-Wno-unused-function"]
+          "-Wall", "-Wno-unused-function",
+          # hipcc makes packed float32 instructions of ordinary float code; some of their forms
+          # give wrong lanes now and then on gfx950, so they are switched off
+          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # decode.hip must round like numpy / CPython: no fused multiply-add contraction.
-# hipcc makes packed float32 instructions of ordinary float code; some of their forms give wrong
-# lanes now and then on gfx950, so they are switched off.
-NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-PER_FILE = {"decode.hip": ["-ffp-contract=off"], "lane_format.hip": ["-ffp-contract=off"],
-            "layer_norm.hip": NO_PACKED, "optim.hip": NO_PACKED}
+PER_FILE = {"decode.hip": ["-ffp-contract=off"], "lane_format.hip": ["-ffp-contract=off"]}
 SOURCES = ["api.hip", "decode.hip", "deform_conv.hip", "deform_conv_cts.hip", "deform_conv_stream.hip", "deform_conv_ring.hip",
            "deform_conv_bwd.hip", "lane_format.hip", "layer_norm.hip", "optim.hip"]
 
