@@ -215,18 +215,29 @@ def lib():
     return _lib
 
 
-def tensor_lists():
-    """The host extension that reads lists of tensors (csrc/tensor_lists.cpp)."""
-    global tensor_lists
+def host():
+    """The host extension (csrc/host_calls.cpp): the plain case of small or many-tensor calls."""
+    global host
     try:
-        from . import _tensor_lists as module
+        from . import _host as module
     except ImportError as e:
-        raise RuntimeError("ganet_amd: _tensor_lists.so is missing or does not load (%s) - build it "
-                           "with `python -m ganet_amd.build`" % e)
+        raise RuntimeError("ganet_amd: _host.so is missing or does not load (%s) - build it with "
+                           "`python -m ganet_amd.build`" % e)
 
-    def tensor_lists():
+    def host():
         return module
     return module
+
+
+_ADDRESSES = {}
+
+
+def address(name):
+    """The address of an entry point of the library."""
+    found = _ADDRESSES.get(name)
+    if found is None:
+        found = _ADDRESSES[name] = ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value
+    return found
 
 
 def call(index, fn, *args):
@@ -234,18 +245,18 @@ def call(index, fn, *args):
     guard and the stream object cost 3 us a call: both are left out where they change nothing."""
     import torch
     if torch.cuda.current_device() == index:
-        return fn(*args, _raw_stream(index))
+        return fn(*args, raw_stream(index))
     with torch.cuda.device(index):
-        return fn(*args, _raw_stream(index))
+        return fn(*args, raw_stream(index))
 
 
-def _raw_stream(index):
+def raw_stream(index):
+    """The address of torch's current stream on a GPU, without a Stream object around it."""
     import torch
-    global _raw_stream
-    # the address alone, without a Stream object around it
-    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    global raw_stream
+    raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
         lambda i: torch.cuda.current_stream(i).cuda_stream)
-    return _raw_stream(index)
+    return raw_stream(index)
 
 
 def status_string(status):

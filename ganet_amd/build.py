@@ -32,26 +32,27 @@ def _newer(a, b):
     return (not os.path.exists(b)) or os.path.getmtime(a) > os.path.getmtime(b)
 
 
-LISTS = os.path.join(HERE, "_tensor_lists.so")
+HOST = os.path.join(HERE, "_host.so")
 
 
-def build_lists(force=False, verbose=False):
-    """The host extension ganet_amd/_tensor_lists.so (csrc/tensor_lists.cpp, no GPU code)."""
-    src = os.path.join(CSRC, "tensor_lists.cpp")
-    if not force and not _newer(src, LISTS):
-        return LISTS
+def build_host(force=False, verbose=False):
+    """The host extension ganet_amd/_host.so (csrc/host_calls.cpp, no GPU code)."""
+    src = os.path.join(CSRC, "host_calls.cpp")
+    header = os.path.join(ROOT, "include", "ganet_hip.h")
+    if not force and not _newer(src, HOST) and not _newer(header, HOST):
+        return HOST
     import sysconfig
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall",
            "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI]
     cmd += ["-isystem" + p for p in include_paths()] + ["-I" + sysconfig.get_paths()["include"]]
-    cmd += [src, "-o", LISTS] + ["-L" + p for p in library_paths()]
+    cmd += ["-I" + os.path.dirname(header), src, "-o", HOST] + ["-L" + p for p in library_paths()]
     cmd += ["-ltorch_python", "-ltorch_cpu", "-lc10"]
     if verbose:
         print(" ".join(cmd))
     subprocess.check_call(cmd)
-    return LISTS
+    return HOST
 
 
 def _variant_flags():
@@ -124,4 +125,4 @@ def build_lib(force=False, verbose=False):
 
 if __name__ == "__main__":
     print(build_lib(force="--force" in sys.argv, verbose=True))
-    print(build_lists(force="--force" in sys.argv, verbose=True))
+    print(build_host(force="--force" in sys.argv, verbose=True))

@@ -1,0 +1,301 @@
+// Host only: the plain case of the training operators' calls (ganet_amd/optim.py, norm.py) without
+// Python in between.
+//
+// A step checks every tensor of every list (GPU, type, shape, order, address): in Python that is
+// some 40 ns an attribute, 100 us for the seven lists of a 62-tensor model, as long as the step
+// itself.  Here it is a few.  The functions only accept the plain case - one GPU, one type a list,
+// everything contiguous and of its parameter's shape, nothing twice - and return None for anything
+// else; Python then looks again, copies what can be copied and names what is wrong.
+#include <ATen/ops/empty.h>
+#include <ATen/ops/empty_like.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <vector>
+
+#include "ganet_hip.h"
+
+namespace {
+
+enum { kFloat32 = 0, kBFloat16 = 1, kFloat16 = 2, kE4M3 = 3, kOther = -1 };
+
+int code(at::ScalarType t) {
+  switch (t) {
+    case at::kFloat: return kFloat32;
+    case at::kBFloat16: return kBFloat16;
+    case at::kHalf: return kFloat16;
+    case at::kFloat8_e4m3fn: return kE4M3;
+    default: return kOther;
+  }
+}
+
+// The i-th tensor of a list or tuple, null where it is none.
+const at::Tensor *item(PyObject *list, Py_ssize_t i) {
+  PyObject *o = PyList_Check(list) ? PyList_GET_ITEM(list, i) : PyTuple_GET_ITEM(list, i);
+  return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr;
+}
+Py_ssize_t length(PyObject *list) {
+  if (PyList_Check(list)) return PyList_GET_SIZE(list);
+  return PyTuple_Check(list) ? PyTuple_GET_SIZE(list) : -1;
+}
+
+PyObject *bytes(const void *p, size_t n) {
+  return PyBytes_FromStringAndSize(static_cast<const char *>(p), static_cast<Py_ssize_t>(n));
+}
+
+// step(params, grads, avgs, seconds, avg_scales, second_scales, masters, block) ->
+// (gpu, parameter type, gradient type, state type, rows of ganet_step_tensor) or None
+PyObject *step(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  if (nargs != 8) {
+    PyErr_SetString(PyExc_TypeError, "step() takes 8 arguments");
+    return nullptr;
+  }
+  const long block = PyLong_AsLong(args[7]);
+  if (block < 1) {
+    if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "step(): block");
+    return nullptr;
+  }
+  try {
+    const Py_ssize_t n = length(args[0]);
+    if (n < 1) Py_RETURN_NONE;
+    std::vector<std::uint64_t> rows(static_cast<size_t>(n) * 8, 0);
+    std::vector<std::uint64_t> written;
+    int types[7] = {kOther, kOther, kOther, kOther, kOther, kOther, kOther};
+    int gpu = -1;
+    for (int k = 0; k < 7; ++k) {
+      if (args[k] == Py_None) {
+        if (k < 4) Py_RETURN_NONE;
+        continue;
+      }
+      if (length(args[k]) != n) Py_RETURN_NONE;
+      for (Py_ssize_t i = 0; i < n; ++i) {
+        const at::Tensor *t = item(args[k], i), *p = item(args[0], i);
+        if (!t || !p || !t->is_cuda() || t->layout() != at::kStrided || !t->is_contiguous()) Py_RETURN_NONE;
+        const int type = code(t->scalar_type()), at = static_cast<int>(t->get_device());
+        if (i == 0) types[k] = type;
+        if (i == 0 && k == 0) gpu = at;
+        if (type == kOther || type != types[k] || at != gpu) Py_RETURN_NONE;
+        const std::int64_t values = p->numel();
+        if (k == 4 || k == 5) {
+          if (t->numel() != (values + block - 1) / block) Py_RETURN_NONE;
+        } else if (!t->sizes().equals(p->sizes())) {
+          Py_RETURN_NONE;
+        }
+        const auto address = reinterpret_cast<std::uint64_t>(t->data_ptr());
+        rows[i * 8 + k] = address;
+        if (k == 0) rows[i * 8 + 7] = static_cast<std::uint64_t>(values);
+        if (k != 1 && values) written.push_back(address);
+      }
+    }
+    std::sort(written.begin(), written.end());
+    if (std::adjacent_find(written.begin(), written.end()) != written.end()) Py_RETURN_NONE;
+    if (types[2] != types[3] || (args[6] != Py_None && types[6] != kFloat32)) Py_RETURN_NONE;
+    for (int k = 4; k < 6; ++k)
+      if ((args[k] == Py_None) != (types[2] != kE4M3) || (args[k] != Py_None && types[k] != kFloat32))
+        Py_RETURN_NONE;
+    return Py_BuildValue("iiiiN", gpu, types[0], types[1], types[2], bytes(rows.data(), rows.size() * 8));
+  } catch (const std::exception &) {   // a tensor without storage: Python's own reading names it
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+}
+
+// grads(list) -> (gpu, addresses, sizes, types) or None
+PyObject *grads(PyObject *, PyObject *list) {
+  try {
+    const Py_ssize_t n = length(list);
+    if (n < 1) Py_RETURN_NONE;
+    std::vector<std::uint64_t> address(n);
+    std::vector<std::int64_t> size(n);
+    std::vector<std::int32_t> type(n);
+    int gpu = -1;
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      const at::Tensor *t = item(list, i);
+      if (!t || !t->is_cuda() || t->layout() != at::kStrided || !t->is_contiguous()) Py_RETURN_NONE;
+      type[i] = code(t->scalar_type());
+      if (i == 0) gpu = static_cast<int>(t->get_device());
+      if (type[i] == kOther || type[i] == kE4M3 || t->get_device() != gpu) Py_RETURN_NONE;
+      address[i] = reinterpret_cast<std::uint64_t>(t->data_ptr());
+      size[i] = t->numel();
+    }
+    return Py_BuildValue("iNNN", gpu, bytes(address.data(), n * 8), bytes(size.data(), n * 8),
+                         bytes(type.data(), n * 4));
+  } catch (const std::exception &) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+}
+
+// ---- layer norm -----------------------------------------------------------------------------
+// The calls of ganet_amd/norm.py where tensors lie as the kernels take them: in Python the outputs,
+// the parameters and the checks of a small call cost more than its kernel.
+
+struct Where {        // how a tensor's channels lie in memory
+  std::int64_t outer, inner, channels;
+  bool channels_last;
+};
+
+// False where the order is another than rows, an NCHW map or a channels_last one.
+bool place(const at::Tensor &x, std::int64_t dim, Where &w) {
+  const std::int64_t dims = x.dim();
+  if (dim < 0) dim += dims;
+  if (dim < 0 || dim >= dims || x.numel() == 0) return false;
+  w.channels = x.size(dim);
+  w.channels_last = false;
+  w.inner = 1;
+  if (x.is_contiguous()) {
+    for (std::int64_t d = dim + 1; d < dims; ++d) w.inner *= x.size(d);
+  } else if (dims == 4 && dim == 1 && x.is_contiguous(at::MemoryFormat::ChannelsLast)) {
+    w.channels_last = true;
+  } else {
+    return false;
+  }
+  w.outer = x.numel() / w.channels / w.inner;
+  return true;
+}
+bool like(const at::Tensor &t, const at::Tensor &x, const Where &w) {
+  if (!t.is_cuda() || t.get_device() != x.get_device() || t.scalar_type() != x.scalar_type() ||
+      !t.sizes().equals(x.sizes()))
+    return false;
+  return w.channels_last ? t.is_contiguous(at::MemoryFormat::ChannelsLast) : t.is_contiguous();
+}
+const at::Tensor *tensor(PyObject *o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
+// A weight or None: false where it is neither or not [channels] on x's GPU.
+bool weight(PyObject *o, const at::Tensor &x, const Where &w, const at::Tensor *&t, int &type) {
+  t = nullptr;
+  if (o == Py_None) return true;
+  t = tensor(o);
+  if (!t || !t->is_cuda() || t->get_device() != x.get_device() || t->dim() != 1 || t->numel() != w.channels ||
+      !t->is_contiguous())
+    return false;
+  const int c = code(t->scalar_type());
+  if (c == kOther || c == kE4M3 || (type != kOther && c != type)) return false;
+  type = c;
+  return true;
+}
+at::Tensor empty_like(const at::Tensor &x, const Where &w) {
+  return at::empty(x.sizes(), x.options().requires_grad(false),
+                   w.channels_last ? at::MemoryFormat::ChannelsLast : at::MemoryFormat::Contiguous);
+}
+ganet_layer_norm_params parameters(const Where &w, int type, int weight_type, float eps) {
+  ganet_layer_norm_params p = {};
+  p.outer = w.outer;
+  p.inner = w.inner;
+  p.x_stride = p.y_stride = p.g_stride = w.channels * w.inner;
+  p.C = static_cast<std::int32_t>(w.channels);
+  p.dtype = type;
+  p.weight_dtype = weight_type;
+  p.eps = eps;
+  return p;
+}
+void *address(PyObject *o) { return PyLong_AsVoidPtr(o); }
+void *data(const at::Tensor *t) { return t ? t->data_ptr() : nullptr; }
+PyObject *wrapped(const at::Tensor &t) {
+  if (t.defined()) return THPVariable_Wrap(t);
+  Py_RETURN_NONE;
+}
+
+// layer_norm_forward(entry point, x, weight, bias, eps, channel_dim, stats, stream) ->
+// (y, mean, rstd), the entry point's status where it is not 0, or None
+PyObject *layer_norm_forward(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  if (nargs != 8) {
+    PyErr_SetString(PyExc_TypeError, "layer_norm_forward() takes 8 arguments");
+    return nullptr;
+  }
+  const double eps = PyFloat_AsDouble(args[4]);
+  const long dim = PyLong_AsLong(args[5]);
+  const int stats = PyObject_IsTrue(args[6]);
+  auto entry = reinterpret_cast<decltype(&ganet_layer_norm_forward)>(address(args[0]));
+  void *stream = address(args[7]);
+  if (PyErr_Occurred()) return nullptr;
+  try {
+    const at::Tensor *x = tensor(args[1]), *w, *b;
+    Where at;
+    int weight_type = kOther;
+    if (!x || !x->is_cuda() || !entry || !place(*x, dim, at) || at.channels > INT32_MAX) Py_RETURN_NONE;
+    const int type = code(x->scalar_type());
+    if (type == kOther || type == kE4M3 || !weight(args[2], *x, at, w, weight_type) ||
+        !weight(args[3], *x, at, b, weight_type))
+      Py_RETURN_NONE;
+    const auto p = parameters(at, type, weight_type == kOther ? type : weight_type, static_cast<float>(eps));
+    const at::Tensor y = empty_like(*x, at);
+    at::Tensor mean, rstd;
+    if (stats) {
+      mean = at::empty({at.outer * at.inner}, x->options().dtype(at::kFloat).requires_grad(false));
+      rstd = at::empty_like(mean);
+    }
+    const int rc = entry(data(x), data(w), data(b), y.data_ptr(),
+                         stats ? mean.data_ptr<float>() : nullptr, stats ? rstd.data_ptr<float>() : nullptr, &p, stream);
+    if (rc) return PyLong_FromLong(rc);
+    return Py_BuildValue("NNN", wrapped(y), wrapped(mean), wrapped(rstd));
+  } catch (const std::exception &e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
+// layer_norm_backward(workspace query, entry point, x, weight, grad, mean, rstd, channel_dim,
+// need_input + 2 need_weight + 4 need_bias, stream) -> (grad_x, grad_weight, grad_bias), a status, or None
+PyObject *layer_norm_backward(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  if (nargs != 10) {
+    PyErr_SetString(PyExc_TypeError, "layer_norm_backward() takes 10 arguments");
+    return nullptr;
+  }
+  auto query = reinterpret_cast<decltype(&ganet_layer_norm_backward_workspace_bytes)>(address(args[0]));
+  auto entry = reinterpret_cast<decltype(&ganet_layer_norm_backward)>(address(args[1]));
+  const long dim = PyLong_AsLong(args[7]), need = PyLong_AsLong(args[8]);
+  void *stream = address(args[9]);
+  if (PyErr_Occurred()) return nullptr;
+  try {
+    const at::Tensor *x = tensor(args[2]), *g = tensor(args[4]), *mean = tensor(args[5]), *rstd = tensor(args[6]), *w;
+    Where at;
+    int weight_type = kOther;
+    if (!x || !g || !mean || !rstd || !x->is_cuda() || !query || !entry || need < 1 || need > 7 ||
+        !place(*x, dim, at) || at.channels > INT32_MAX || !like(*g, *x, at))
+      Py_RETURN_NONE;
+    const int type = code(x->scalar_type());
+    if (type == kOther || type == kE4M3 || !weight(args[3], *x, at, w, weight_type)) Py_RETURN_NONE;
+    for (const at::Tensor *t : {mean, rstd})
+      if (!t->is_cuda() || t->get_device() != x->get_device() || t->scalar_type() != at::kFloat ||
+          t->numel() != at.outer * at.inner || !t->is_contiguous())
+        Py_RETURN_NONE;
+    if (weight_type == kOther) weight_type = type;
+    const auto p = parameters(at, type, weight_type, 0.0f);
+    const auto plain = (w ? w : x)->options().requires_grad(false);
+    at::Tensor gx, gw, gb, ws;
+    size_t bytes = 0;
+    if (need & 1) gx = empty_like(*x, at);
+    if (need & 2) gw = at::empty({at.channels}, plain);
+    if (need & 4) gb = at::empty({at.channels}, plain);
+    if (need & 6) {
+      bytes = query(&p);
+      ws = at::empty({static_cast<std::int64_t>(std::max<size_t>(bytes, 256))}, plain.dtype(at::kByte));
+    }
+    auto out = [](const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; };
+    const int rc = entry(data(x), data(w), data(g), mean->data_ptr<float>(), rstd->data_ptr<float>(), out(gx), out(gw),
+                         out(gb), &p, out(ws), bytes, stream);
+    if (rc) return PyLong_FromLong(rc);
+    return Py_BuildValue("NNN", wrapped(gx), wrapped(gw), wrapped(gb));
+  } catch (const std::exception &e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
+PyMethodDef methods[] = {
+    {"step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(step)), METH_FASTCALL,
+     "The table of an AdamW step over plain lists of tensors, or None."},
+    {"grads", grads, METH_O, "Addresses, sizes and types of a plain list of gradients, or None."},
+    {"layer_norm_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(layer_norm_forward)),
+     METH_FASTCALL, "Layer norm's forward on tensors in the kernels' order, or None."},
+    {"layer_norm_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(layer_norm_backward)),
+     METH_FASTCALL, "Layer norm's backward on tensors in the kernels' order, or None."},
+    {nullptr, nullptr, 0, nullptr}};
+
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Reads lists of tensors at C speed.", -1, methods,
+                      nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__host(void) { return PyModule_Create(&module); }

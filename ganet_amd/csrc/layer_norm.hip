@@ -739,7 +739,7 @@ __global__ __launch_bounds__(kFinish) void ln_finish(const float *partial, int n
 // ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
-constexpr long long kMostBlocks = 1ll << 22;      // of one launch: its threads stay below 2^32
+constexpr long long kMostThreads = 1ll << 31;     // of one launch
 
 bool dtype_ok(int d) { return d == GANET_F32 || d == GANET_BF16 || d == GANET_F16; }
 
@@ -886,23 +886,37 @@ int launch_forward(const ganet_layer_norm_params *p, const Args &a, hipStream_t 
       constexpr int R = 2;
       const long long many = (p->outer + rows * R - 1) / (rows * R);
       const bool deep = many * threads >= 256 * 1024;
-      const long long blocks = deep ? many : (p->outer + rows - 1) / rows;
-      if (blocks > kMostBlocks) return (int)GANET_ERR_UNSUPPORTED;
-      if (deep) {
-        ln_rows_fwd<T, L, NV, R><<<dim3((unsigned)blocks), dim3(threads), 0, s>>>(a);
-        return ganet_check_launch();
+      const long long most = kMostThreads / threads * (deep ? rows * R : rows);    // rows of a launch
+      Args part = a;
+      for (long long at = 0; at < p->outer; at += most) {
+        part.outer = p->outer - at < most ? p->outer - at : most;
+        part.x = (const T *)a.x + at * a.xs;
+        part.y = (T *)a.y + at * a.ys;
+        part.mean = a.mean ? a.mean + at : nullptr;
+        part.rstd = a.rstd ? a.rstd + at : nullptr;
+        if (deep)
+          ln_rows_fwd<T, L, NV, R><<<dim3((unsigned)((part.outer + rows * R - 1) / (rows * R))), dim3(threads), 0, s>>>(part);
+        else
+          ln_rows_fwd<T, L, NV, 1><<<dim3((unsigned)((part.outer + rows - 1) / rows)), dim3(threads), 0, s>>>(part);
+        const int rc = ganet_check_launch();
+        if (rc != GANET_OK) return rc;
       }
-      ln_rows_fwd<T, L, NV, 1><<<dim3((unsigned)blocks), dim3(threads), 0, s>>>(a);
-      return ganet_check_launch();
+      return (int)GANET_OK;
     });
   return with_plane_shape<false, T>(p, [&](auto vb, auto nc, auto waves) {
-    if constexpr (vb.value == kAny) {
+    auto any = [&] {
       const long long work = p->outer * tiles_of(p, kTile);
       ln_planes_any_fwd<T><<<dim3((unsigned)(work < 8192 ? work : 8192)), dim3(kThreads), 0, s>>>(a);
+    };
+    if constexpr (vb.value == kAny) {
+      any();
     } else {
       typedef Plane<T, vb.value, nc.value, waves.value> P;
       const long long tiles = tiles_of(p, P::TILE);
-      if (p->outer * tiles > kMostBlocks) return (int)GANET_ERR_UNSUPPORTED;
+      if (p->outer * tiles > kMostThreads / P::THREADS - 8) {    // more than a launch takes
+        any();
+        return ganet_check_launch();
+      }
       ln_planes_fwd<T, vb.value, nc.value, waves.value>
           <<<dim3((unsigned)((p->outer * tiles + 7) / 8 * 8)), dim3(P::THREADS), 0, s>>>(a, (int)tiles,
                                                                           (p->C + P::SLOTS - 1) / P::SLOTS);

@@ -135,11 +135,20 @@ def _ptr(t):
 
 
 def _forward(input, weight, bias, eps, channel_dim, stats):
+    if not eps >= 0:
+        raise ValueError("layer_norm: eps %r" % (eps,))
+    index = input.get_device()
+    if index >= 0 and torch.cuda.current_device() == index:
+        out = _lib.host().layer_norm_forward(_lib.address("ganet_layer_norm_forward"), input, weight,
+                                             bias, eps, channel_dim, stats, _lib.raw_stream(index))
+        if type(out) is tuple:
+            return out
+        if out is not None:
+            _lib.check(out, "ganet_layer_norm_forward")
+    # another order of memory, nothing to do, or something wrong
     lay = _Layout(input, channel_dim)
     _check_input(input)
     wdtype = _weight_dtype(input, (("weight", weight), ("bias", bias)), lay.C)
-    if not eps >= 0:
-        raise ValueError("layer_norm: eps %r" % (eps,))
     L = _lib.lib()
     x, weight, bias = lay.x, _dense(weight), _dense(bias)
     p = _lib.LayerNormParams(lay.outer, lay.inner, lay.stride, lay.C * lay.inner, 0, lay.C,
@@ -169,6 +178,17 @@ def layer_norm_backward(input, weight, grad_output, mean, rstd, channel_dim=-1,
     """Raw backward: (grad_input, grad_weight, grad_bias), None for what is not asked for.
     grad_input has the memory format of `input`; grad_weight and grad_bias are [C] of the weight's
     dtype (the input's without a weight)."""
+    index = input.get_device()
+    if index >= 0 and torch.cuda.current_device() == index:
+        out = _lib.host().layer_norm_backward(
+            _lib.address("ganet_layer_norm_backward_workspace_bytes"),
+            _lib.address("ganet_layer_norm_backward"), input, weight, grad_output, mean, rstd,
+            channel_dim, bool(need_input) + 2 * bool(need_weight) + 4 * bool(need_bias),
+            _lib.raw_stream(index))
+        if type(out) is tuple:
+            return out
+        if out is not None:
+            _lib.check(out, "ganet_layer_norm_backward")
     lay = _Layout(input, channel_dim)
     if not grad_output.is_cuda:
         raise NotImplementedError
@@ -177,7 +197,6 @@ def layer_norm_backward(input, weight, grad_output, mean, rstd, channel_dim=-1,
     if grad_output.shape != input.shape:
         raise ValueError("layer_norm: grad_output of shape %s for an input of shape %s"
                          % (tuple(grad_output.shape), tuple(input.shape)))
-    index = input.get_device()
     for t in (grad_output, mean, rstd):
         if t.get_device() != index:
             raise ValueError("layer_norm: tensors on %s and %s" % (t.device, input.device))

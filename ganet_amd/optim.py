@@ -82,7 +82,7 @@ def _like_params(params, shapes, plain, tensors, what):
 def _table(params, grads, avgs, seconds, avg_scales, second_scales, masters, bits):
     """(GPU, parameters' dtype, gradients' dtype, rows of ganet_step_tensor, what they point into):
     any order of memory, and the errors of what cannot be stepped.  Plain lists (contiguous, nothing
-    wrong) do not come here: _lib.tensor_lists().step reads them."""
+    wrong) do not come here: _lib.host().step reads them."""
     n = len(params)
     for what, ts in (("gradients", grads), ("exp_avgs", avgs), ("second moments", seconds),
                      ("masters", masters), ("scales", avg_scales), ("scales", second_scales)):
@@ -145,7 +145,7 @@ def _step(params, grads, avgs, seconds, avg_scales, second_scales, bits, step, l
           weight_decay, masters, grad_stats, skip_nonfinite, seed):
     n = len(params)
     lists = (params, grads, avgs, seconds, avg_scales, second_scales, masters)
-    found = _lib.tensor_lists().step(*lists, BLOCK)
+    found = _lib.host().step(*lists, BLOCK)
     if (found is not None and max(found[1:3]) < 3 and found[3] == (0 if bits == 32 else 3)
             and not (masters is not None and found[1] == 0)):
         index, ptype, gtype, _, rows = found
@@ -225,7 +225,7 @@ def grad_norm(grads, max_norm=None, inv_scale=1.0, out=None):
     adamw_step_8bit take the tensor as grad_stats.  Gradients of several dtypes may be mixed."""
     grads = list(grads)
     n = len(grads)
-    found = _lib.tensor_lists().grads(grads)
+    found = _lib.host().grads(grads)
     if found is not None:
         index, ptrs, numel, dtypes = found
     else:
@@ -300,6 +300,15 @@ class AdamW(torch.optim.Optimizer):
         self.seed, self.min_8bit_size, self.capturable = seed, min_8bit_size, capturable
         self.grad_stats = None
 
+    def __getstate__(self):
+        """Copies and pickles keep the options too (torch's own state has the groups only)."""
+        kept = super(AdamW, self).__getstate__()
+        for name in ("state_bits", "master_weights", "max_grad_norm", "skip_nonfinite", "seed",
+                     "min_8bit_size", "capturable"):
+            kept[name] = getattr(self, name)
+        kept["grad_stats"] = None
+        return kept
+
     def _init_state(self, p, fresh):
         """First step of a parameter.  `fresh`: the step counters made in this call, by device."""
         if not p.is_cuda:
@@ -308,8 +317,6 @@ class AdamW(torch.optim.Optimizer):
             raise TypeError("AdamW: unsupported dtype %s" % p.dtype)
         if not _dense(p):
             raise ValueError("AdamW: a parameter of strides %s is not dense" % (p.stride(),))
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("AdamW: make one step before the capture")
         st = self.state[p]
         if self.capturable:
             if p.device not in fresh:
@@ -337,6 +344,12 @@ class AdamW(torch.optim.Optimizer):
             return loss
         if any(p.grad.is_sparse for _, p in every):
             raise RuntimeError("AdamW: sparse gradients")
+        if every[0][1].is_cuda and torch.cuda.is_current_stream_capturing():
+            # the number of the step would be part of the graph, a new state its memory
+            if not self.capturable:
+                raise RuntimeError("AdamW: a captured step needs capturable=True")
+            if any("step" not in self.state.get(p, ()) for _, p in every):
+                raise RuntimeError("AdamW: make one step before the capture")
         if grad_stats is None and self.max_grad_norm is not None:
             grad_stats = grad_norm([p.grad for _, p in every], self.max_grad_norm)
         self.grad_stats = grad_stats

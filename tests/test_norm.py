@@ -418,3 +418,13 @@ def test_offsets_past_32_bits():
     planes[1, :, -70:] = part[0]
     y, mean, rstd = norm.layer_norm_forward(planes, part[1], part[2], channel_dim=1)
     check_forward(part[0], part[1], part[2], 1e-5, 0, y[1, :, -70:], mean[-70:], rstd[-70:])
+
+
+@gpu
+def test_more_rows_than_a_launch_takes():
+    """One channel, 2^31 + rows: every output is its bias."""
+    n = (1 << 31) + 70001
+    x = torch.ones(n, 1, dtype=torch.bfloat16, device="cuda")
+    b = torch.full((1,), 0.75, dtype=torch.bfloat16, device="cuda")
+    y = norm.layer_norm(x, None, b)
+    assert float(y.min()) == float(y.max()) == 0.75

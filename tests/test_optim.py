@@ -8,6 +8,7 @@ parameter is off by 16 u (|p| + lr' / denominator (|b1 m0| + |(1 - b1) g|)), and
 type for its rounding.  The norm is summed in float64 and rounded once: 2^-23 relative.
 A value held in 8 bits is one of the two e4m3 values around it, each with the probability that keeps
 the mean; which one is a function of the random word, tested against that word's own definition."""
+import copy
 import ctypes
 import math
 
@@ -553,10 +554,15 @@ def test_optimizer_matches_the_raw_calls_and_reloads(bits, master):
             if torch.is_tensor(value):
                 assert o2.state[q][name].dtype == value.dtype
                 assert o2.state[q][name].data_ptr() != value.data_ptr()
+    copied = copy.deepcopy(o2)                       # options and states go along
+    assert (copied.state_bits, copied.max_grad_norm, copied.seed) == (bits, 0.5, 11)
     for _ in range(2):
         for m, opt in ((model, o), (twin, o2)):
             backward(m)
             opt.step()
+    for p in copied.param_groups[0]["params"]:
+        p.grad = torch.ones_like(p)
+    copied.step()
     for p, q in zip(model.parameters(), twin.parameters()):
         assert torch.equal(p, q)
 
@@ -582,10 +588,12 @@ def test_captured_step_counts_on(bits):
                 t.grad.copy_(g)
 
     fill()
-    with pytest.raises(RuntimeError):
-        graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph):
-            o.step()
+    plain = optim.AdamW(model.parameters(), **kw)
+    for opt in (o, plain):                           # no state yet; a number that would not count on
+        with pytest.raises(RuntimeError):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                opt.step()
     o.step()
     e.step()
     torch.cuda.synchronize()
