@@ -466,7 +466,7 @@ struct Plane {
 // through LDS, where a lane adds what it holds over the wavefronts; then the rows hand each other
 // their quarters back.  For M = 16 and 8 wavefronts: 24 exchanges and 9 LDS accesses of 16 bytes
 // without conflicts (every lane summing everything: 32 exchanges through LDS and 36 accesses, bf16
-// backward 32x256x40x100 61 us instead of PLANES16).
+// backward 32x256x40x100 61 us instead of 50).
 template <int M, int WAVES>
 __device__ __forceinline__ void slots_sum(float (&s)[M], float (*part)[64][M / 4]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -825,7 +825,11 @@ int with_row_shape(int C, F &&f) {
 
 long long tiles_of(const ganet_layer_norm_params *p, int tile) { return (p->inner + tile - 1) / tile; }
 
-// Planes: the fewest registers that hold C; a forward keeps one map, a backward two.
+// Planes.  Forward: 16 channels a slot, as many wavefronts as C takes (bf16 128x64x40x100: one
+// wavefront 22 us, four with four channels a slot 31 us; 8x1024x40x100: 28 us with this and with half
+// the wavefronts).  Backward, which keeps two maps and the channels' sums: eight channels a slot, and
+// four where 16-bit values make eight positions a lane (32x256x40x100: 45 us, with eight 50 us;
+// float32 with its four positions the other way round, 75 and 72 us).
 enum { kAny = 0 };
 template <bool BACKWARD, typename T, typename F>
 int with_plane_shape(const ganet_layer_norm_params *p, F &&f) {
@@ -833,16 +837,23 @@ int with_plane_shape(const ganet_layer_norm_params *p, F &&f) {
   if (p->C <= 4 * (WAVES) * (NC) && p->inner >= (VB) / (int)sizeof(T))                                                                          \
     return f(std::integral_constant<int, VB>(), std::integral_constant<int, NC>(),                      \
              std::integral_constant<int, WAVES>())
-  GANET_PLANE(16, 4, 4);
-  GANET_PLANE(16, 8, 4);
-  if constexpr (BACKWARD) {
-    GANET_PLANE(16, 8, 8);
+  if constexpr (!BACKWARD) {
+    GANET_PLANE(16, 16, 1);
+    GANET_PLANE(16, 16, 2);
+    GANET_PLANE(16, 16, 4);
+    GANET_PLANE(16, 16, 8);
+    GANET_PLANE(16, 16, 16);
+  } else {
+    GANET_PLANE(16, 4, 4);
+    if constexpr (sizeof(T) == 2) {
+      GANET_PLANE(16, 4, 8);
+      GANET_PLANE(16, 4, 16);
+    } else {
+      GANET_PLANE(16, 8, 4);
+      GANET_PLANE(16, 8, 8);
+    }
     GANET_PLANE(16, 8, 16);
     GANET_PLANE(8, 16, 16);
-  } else {
-    GANET_PLANE(16, 16, 4);
-    GANET_PLANE(16, 32, 4);
-    GANET_PLANE(16, 32, 8);
   }
 #undef GANET_PLANE
   return f(std::integral_constant<int, kAny>(), std::integral_constant<int, 1>(), std::integral_constant<int, 1>());

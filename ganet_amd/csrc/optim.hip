@@ -100,27 +100,31 @@ struct Args32 {
 };
 static_assert(sizeof(Args32<true>) <= 4096 && sizeof(Args32<false>) <= 4096, "kernel arguments");
 
-constexpr int kVec32 = 4;       // values of a lane's vector
-constexpr int kUnroll32 = 4;    // vectors of a lane: 16 loads in flight
-constexpr int kChunk32 = kThreads * kVec32 * kUnroll32;
+// A lane takes U vectors of 4 values: four (16 loads in flight) where there is work for the whole
+// chip, one where a list is so short that its chunks would not be four a CU (one weight of 114688
+// values, the launch alone: 6.4 us with four, 4.0 with one).
+constexpr int kVec32 = 4;
+constexpr int kDeep = 4;
+constexpr long long kFew = 4 * 256;               // chunks
+constexpr int chunk32(int u) { return kThreads * kVec32 * u; }
 
-template <typename TP, typename TG, bool MASTER>
+template <typename TP, typename TG, bool MASTER, int U>
 __global__ __launch_bounds__(kThreads) void adamw32_kernel(Args32<MASTER> a) {
   Coef c;
   if (!coefficients(a.h, c)) return;
   const int t = find_tensor(a.t, (int)blockIdx.x);
-  const long long at = (long long)((int)blockIdx.x - a.t.first[t]) * kChunk32;
-  const int left = (int)blockIdx.x + 1 == a.t.first[t + 1] ? a.t.tail[t] : kChunk32;
+  const long long at = (long long)((int)blockIdx.x - a.t.first[t]) * chunk32(U);
+  const int left = (int)blockIdx.x + 1 == a.t.first[t + 1] ? a.t.tail[t] : chunk32(U);
   TP *p = (TP *)a.t.ptr[kParam][t] + at;
   const TG *g = (const TG *)a.t.ptr[kGrad][t] + at;
   float *m = (float *)a.t.ptr[kAvg][t] + at, *v = (float *)a.t.ptr[kSecond][t] + at;
   float *w = MASTER ? (float *)a.t.ptr[MASTER ? kMaster32 : 0][t] + at : nullptr;
 
-  Vec<TP, kVec32> vp[kUnroll32];
-  Vec<TG, kVec32> vg[kUnroll32];
-  Vec<float, kVec32> vm[kUnroll32], vv[kUnroll32], vw[kUnroll32];
+  Vec<TP, kVec32> vp[U];
+  Vec<TG, kVec32> vg[U];
+  Vec<float, kVec32> vm[U], vv[U], vw[U];
 #pragma unroll
-  for (int u = 0; u < kUnroll32; ++u) {
+  for (int u = 0; u < U; ++u) {
     const int i = (u * kThreads + (int)threadIdx.x) * kVec32;
     if (i < left) {
       vg[u].load(g + i, left - i);
@@ -133,7 +137,7 @@ __global__ __launch_bounds__(kThreads) void adamw32_kernel(Args32<MASTER> a) {
     }
   }
 #pragma unroll
-  for (int u = 0; u < kUnroll32; ++u) {
+  for (int u = 0; u < U; ++u) {
     const int i = (u * kThreads + (int)threadIdx.x) * kVec32;
     if (i >= left) continue;
 #pragma unroll
@@ -172,9 +176,8 @@ struct Args8 {
 };
 static_assert(sizeof(Args8<true>) <= 4096 && sizeof(Args8<false>) <= 4096, "kernel arguments");
 
-constexpr int kVec8 = 4;                            // values of a lane: a wavefront holds a block
-constexpr int kUnroll8 = 4;
-constexpr int kChunk8 = kThreads * kVec8 * kUnroll8; // a whole number of blocks
+constexpr int kVec8 = 4;                          // values of a lane: a wavefront holds a block
+constexpr int chunk8(int u) { return kThreads * kVec8 * u; }   // a whole number of blocks
 
 __device__ __forceinline__ unsigned mix32(unsigned x) {
   x ^= x >> 16;
@@ -211,13 +214,13 @@ __device__ __forceinline__ unsigned block_max(unsigned v) {
 }
 constexpr unsigned kInf = 0x7F800000u;
 
-template <typename TP, typename TG, bool MASTER>
+template <typename TP, typename TG, bool MASTER, int U>
 __global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8<MASTER> a) {
   Coef c;
   if (!coefficients(a.h, c)) return;
   const int t = find_tensor(a.t, (int)blockIdx.x);
-  const long long at = (long long)((int)blockIdx.x - a.t.first[t]) * kChunk8;
-  const int left = (int)blockIdx.x + 1 == a.t.first[t + 1] ? a.t.tail[t] : kChunk8;
+  const long long at = (long long)((int)blockIdx.x - a.t.first[t]) * chunk8(U);
+  const int left = (int)blockIdx.x + 1 == a.t.first[t + 1] ? a.t.tail[t] : chunk8(U);
   TP *p = (TP *)a.t.ptr[kParam][t] + at;
   const TG *g = (const TG *)a.t.ptr[kGrad][t] + at;
   unsigned char *m = (unsigned char *)a.t.ptr[kAvg][t] + at, *r = (unsigned char *)a.t.ptr[kSecond][t] + at;
@@ -227,13 +230,13 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8<MASTER> a) {
   const unsigned key = mix32(c.key + (unsigned)(a.tensor0 + t) * 0x85EBCA6Bu);
   typedef unsigned char Byte4 __attribute__((ext_vector_type(4), aligned(1)));
 
-  Vec<TP, kVec8> vp[kUnroll8];
-  Vec<TG, kVec8> vg[kUnroll8];
-  Vec<float, kVec8> vw[kUnroll8];
-  unsigned vm[kUnroll8], vr[kUnroll8];
-  float sm[kUnroll8], sr[kUnroll8];
+  Vec<TP, kVec8> vp[U];
+  Vec<TG, kVec8> vg[U];
+  Vec<float, kVec8> vw[U];
+  unsigned vm[U], vr[U];
+  float sm[U], sr[U];
 #pragma unroll
-  for (int u = 0; u < kUnroll8; ++u) {
+  for (int u = 0; u < U; ++u) {
     const int i = (u * kThreads + (int)threadIdx.x) * kVec8;
     const int k = left - i;
     vm[u] = vr[u] = 0;
@@ -260,7 +263,7 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8<MASTER> a) {
     }
   }
 #pragma unroll
-  for (int u = 0; u < kUnroll8; ++u) {
+  for (int u = 0; u < U; ++u) {
     const int i = (u * kThreads + (int)threadIdx.x) * kVec8;
     const int k = left - i;
     float nm[kVec8], nr[kVec8];
@@ -577,35 +580,43 @@ extern "C" int ganet_adamw_step(const ganet_step_tensor *tensors, int count, con
   h.lr_dev = p->lr_device;
 
   hipStream_t s = (hipStream_t)stream;
+  long long chunks = 0;
+  for (int i = 0; i < count; ++i) chunks += (tensors[i].n + chunk32(kDeep) - 1) / chunk32(kDeep);
+  const bool deep = chunks >= kFew;
   return with_types(p->param_dtype, p->grad_dtype, master, [&](auto tp, auto tg, auto tm) {
     typedef decltype(tp) TP;
     typedef decltype(tg) TG;
     constexpr bool M = decltype(tm)::value;
-    if (!small) {
-      Args32<M> a;
+    auto step = [&](auto u) {
+      constexpr int U = u.value;
+      if (!small) {
+        Args32<M> a;
+        a.h = h;
+        return in_launches(
+            tensors, count, chunk32(U), a.t,
+            [](const ganet_step_tensor &x, int k) { return k == kMaster32 ? (void *)x.master : address(x, k); },
+            [&](unsigned blocks, int) {
+              adamw32_kernel<TP, TG, M, U><<<dim3(blocks), dim3(kThreads), 0, s>>>(a);
+              return ganet_check_launch();
+            });
+      }
+      Args8<M> a;
       a.h = h;
       return in_launches(
-          tensors, count, kChunk32, a.t,
-          [](const ganet_step_tensor &x, int k) { return k == kMaster32 ? (void *)x.master : address(x, k); },
-          [&](unsigned blocks, int) {
-            adamw32_kernel<TP, TG, M><<<dim3(blocks), dim3(kThreads), 0, s>>>(a);
+          tensors, count, chunk8(U), a.t,
+          [](const ganet_step_tensor &x, int k) {
+            if (k == kAvgScale) return (void *)x.exp_avg_scale;
+            if (k == kSecondScale) return (void *)x.second_scale;
+            return k == kMaster8 ? (void *)x.master : address(x, k);
+          },
+          [&](unsigned blocks, int start) {
+            a.tensor0 = start;
+            adamw8_kernel<TP, TG, M, U><<<dim3(blocks), dim3(kThreads), 0, s>>>(a);
             return ganet_check_launch();
           });
-    }
-    Args8<M> a;
-    a.h = h;
-    return in_launches(
-        tensors, count, kChunk8, a.t,
-        [](const ganet_step_tensor &x, int k) {
-          if (k == kAvgScale) return (void *)x.exp_avg_scale;
-          if (k == kSecondScale) return (void *)x.second_scale;
-          return k == kMaster8 ? (void *)x.master : address(x, k);
-        },
-        [&](unsigned blocks, int start) {
-          a.tensor0 = start;
-          adamw8_kernel<TP, TG, M><<<dim3(blocks), dim3(kThreads), 0, s>>>(a);
-          return ganet_check_launch();
-        });
+    };
+    if (deep) return step(std::integral_constant<int, kDeep>());
+    return step(std::integral_constant<int, 1>());
   });
 }
 
