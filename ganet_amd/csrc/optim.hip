@@ -100,63 +100,52 @@ struct Args32 {
 };
 static_assert(sizeof(Args32<true>) <= 4096 && sizeof(Args32<false>) <= 4096, "kernel arguments");
 
-// A lane takes U vectors of 4 values: four (16 loads in flight) where there is work for the whole
-// chip, one where a list is so short that its chunks would not be four a CU (one weight of 114688
-// values, the launch alone: 6.4 us with four, 4.0 with one).
-constexpr int kVec32 = 4;
-constexpr int kDeep = 4;
-constexpr long long kFew = 4 * 256;               // chunks
-constexpr int chunk32(int u) { return kThreads * kVec32 * u; }
+// A lane takes one vector of 4 values, a workgroup 1024: many short workgroups keep more loads and
+// stores under way than few with several vectors a lane (100 M float32 values: one vector 471 us,
+// two 479, four 492; 114688 values: 4.0 us and 6.4 with four).
+constexpr int kVec = 4;
+constexpr int kChunk = kThreads * kVec;
 
-template <typename TP, typename TG, bool MASTER, int U>
+template <typename TP, typename TG, bool MASTER>
 __global__ __launch_bounds__(kThreads) void adamw32_kernel(Args32<MASTER> a) {
   Coef c;
   if (!coefficients(a.h, c)) return;
   const int t = find_tensor(a.t, (int)blockIdx.x);
-  const long long at = (long long)((int)blockIdx.x - a.t.first[t]) * chunk32(U);
-  const int left = (int)blockIdx.x + 1 == a.t.first[t + 1] ? a.t.tail[t] : chunk32(U);
+  const long long at = (long long)((int)blockIdx.x - a.t.first[t]) * kChunk;
+  const int left = (int)blockIdx.x + 1 == a.t.first[t + 1] ? a.t.tail[t] : kChunk;
   TP *p = (TP *)a.t.ptr[kParam][t] + at;
   const TG *g = (const TG *)a.t.ptr[kGrad][t] + at;
   float *m = (float *)a.t.ptr[kAvg][t] + at, *v = (float *)a.t.ptr[kSecond][t] + at;
   float *w = MASTER ? (float *)a.t.ptr[MASTER ? kMaster32 : 0][t] + at : nullptr;
 
-  Vec<TP, kVec32> vp[U];
-  Vec<TG, kVec32> vg[U];
-  Vec<float, kVec32> vm[U], vv[U], vw[U];
+  const int i = (int)threadIdx.x * kVec, k = left - i;
+  if (k <= 0) return;
+  Vec<TP, kVec> vp;
+  Vec<TG, kVec> vg;
+  Vec<float, kVec> vm, vv, vw;
+  vg.load(g + i, k);
+  vm.load(m + i, k);
+  vv.load(v + i, k);
+  if constexpr (MASTER)
+    vw.load(w + i, k);
+  else
+    vp.load(p + i, k);
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int i = (u * kThreads + (int)threadIdx.x) * kVec32;
-    if (i < left) {
-      vg[u].load(g + i, left - i);
-      vm[u].load(m + i, left - i);
-      vv[u].load(v + i, left - i);
-      if constexpr (MASTER)
-        vw[u].load(w + i, left - i);
-      else
-        vp[u].load(p + i, left - i);
-    }
+  for (int j = 0; j < kVec; ++j) {
+    const float gr = vg.get(j) * c.gscale;
+    const float mm = a.h.b1 * vm.get(j) + a.h.omb1 * gr;
+    const float sq = a.h.b2 * vv.get(j) + a.h.omb2 * (gr * gr);
+    const float old = MASTER ? vw.get(j) : vp.get(j);
+    const float now = old * c.decay - c.lr_c * (mm / (sqrtf(sq) * c.rbc2 + a.h.eps));
+    vm.set(j, mm);
+    vv.set(j, sq);
+    if constexpr (MASTER) vw.set(j, now);
+    vp.set(j, now);   // 16-bit weights: rounded once, to nearest
   }
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int i = (u * kThreads + (int)threadIdx.x) * kVec32;
-    if (i >= left) continue;
-#pragma unroll
-    for (int k = 0; k < kVec32; ++k) {
-      const float gr = vg[u].get(k) * c.gscale;
-      const float mm = a.h.b1 * vm[u].get(k) + a.h.omb1 * gr;
-      const float sq = a.h.b2 * vv[u].get(k) + a.h.omb2 * (gr * gr);
-      const float old = MASTER ? vw[u].get(k) : vp[u].get(k);
-      const float now = old * c.decay - c.lr_c * (mm / (sqrtf(sq) * c.rbc2 + a.h.eps));
-      vm[u].set(k, mm);
-      vv[u].set(k, sq);
-      if constexpr (MASTER) vw[u].set(k, now);
-      vp[u].set(k, now);   // 16-bit weights: rounded once, to nearest
-    }
-    vm[u].store(m + i, left - i);
-    vv[u].store(v + i, left - i);
-    if constexpr (MASTER) vw[u].store(w + i, left - i);
-    vp[u].store(p + i, left - i);
-  }
+  vm.store(m + i, k);
+  vv.store(v + i, k);
+  if constexpr (MASTER) vw.store(w + i, k);
+  vp.store(p + i, k);
 }
 
 // ---- states in 8 bits -------------------------------------------------------------------------
@@ -176,8 +165,7 @@ struct Args8 {
 };
 static_assert(sizeof(Args8<true>) <= 4096 && sizeof(Args8<false>) <= 4096, "kernel arguments");
 
-constexpr int kVec8 = 4;                          // values of a lane: a wavefront holds a block
-constexpr int chunk8(int u) { return kThreads * kVec8 * u; }   // a whole number of blocks
+static_assert(kBlock == 64 * kVec, "a wavefront holds a block");
 
 __device__ __forceinline__ unsigned mix32(unsigned x) {
   x ^= x >> 16;
@@ -214,13 +202,13 @@ __device__ __forceinline__ unsigned block_max(unsigned v) {
 }
 constexpr unsigned kInf = 0x7F800000u;
 
-template <typename TP, typename TG, bool MASTER, int U>
+template <typename TP, typename TG, bool MASTER>
 __global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8<MASTER> a) {
   Coef c;
   if (!coefficients(a.h, c)) return;
   const int t = find_tensor(a.t, (int)blockIdx.x);
-  const long long at = (long long)((int)blockIdx.x - a.t.first[t]) * chunk8(U);
-  const int left = (int)blockIdx.x + 1 == a.t.first[t + 1] ? a.t.tail[t] : chunk8(U);
+  const long long at = (long long)((int)blockIdx.x - a.t.first[t]) * kChunk;
+  const int left = (int)blockIdx.x + 1 == a.t.first[t + 1] ? a.t.tail[t] : kChunk;
   TP *p = (TP *)a.t.ptr[kParam][t] + at;
   const TG *g = (const TG *)a.t.ptr[kGrad][t] + at;
   unsigned char *m = (unsigned char *)a.t.ptr[kAvg][t] + at, *r = (unsigned char *)a.t.ptr[kSecond][t] + at;
@@ -230,133 +218,125 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8<MASTER> a) {
   const unsigned key = mix32(c.key + (unsigned)(a.tensor0 + t) * 0x85EBCA6Bu);
   typedef unsigned char Byte4 __attribute__((ext_vector_type(4), aligned(1)));
 
-  Vec<TP, kVec8> vp[U];
-  Vec<TG, kVec8> vg[U];
-  Vec<float, kVec8> vw[U];
-  unsigned vm[U], vr[U];
-  float sm[U], sr[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int i = (u * kThreads + (int)threadIdx.x) * kVec8;
-    const int k = left - i;
-    vm[u] = vr[u] = 0;
-    sm[u] = sr[u] = 0.0f;
-    vg[u].zero();
-    if (k <= 0) continue;
-    vg[u].load(g + i, k);
+  const int i = (int)threadIdx.x * kVec, k = left - i;
+  Vec<TP, kVec> vp;
+  Vec<TG, kVec> vg;
+  Vec<float, kVec> vw;
+  unsigned vm = 0, vr = 0;
+  float sm = 0.0f, sr = 0.0f;
+  vg.zero();
+  if (k > 0) {
+    vg.load(g + i, k);
     if constexpr (MASTER)
-      vw[u].load(w + i, k);
+      vw.load(w + i, k);
     else
-      vp[u].load(p + i, k);
-    sm[u] = ((const GANET_GLOBAL float *)ms)[i / kBlock];
-    sr[u] = ((const GANET_GLOBAL float *)rs)[i / kBlock];
-    if (k >= kVec8) {
-      vm[u] = __builtin_bit_cast(unsigned, __builtin_nontemporal_load((const GANET_GLOBAL Byte4 *)(m + i)));
-      vr[u] = __builtin_bit_cast(unsigned, __builtin_nontemporal_load((const GANET_GLOBAL Byte4 *)(r + i)));
+      vp.load(p + i, k);
+    sm = ((const GANET_GLOBAL float *)ms)[i / kBlock];
+    sr = ((const GANET_GLOBAL float *)rs)[i / kBlock];
+    if (k >= kVec) {
+      vm = __builtin_bit_cast(unsigned, __builtin_nontemporal_load((const GANET_GLOBAL Byte4 *)(m + i)));
+      vr = __builtin_bit_cast(unsigned, __builtin_nontemporal_load((const GANET_GLOBAL Byte4 *)(r + i)));
     } else {
 #pragma unroll
-      for (int j = 0; j < kVec8; ++j)
+      for (int j = 0; j < kVec; ++j)
         if (j < k) {
-          vm[u] |= (unsigned)m[i + j] << (8 * j);
-          vr[u] |= (unsigned)r[i + j] << (8 * j);
+          vm |= (unsigned)m[i + j] << (8 * j);
+          vr |= (unsigned)r[i + j] << (8 * j);
         }
     }
   }
+  float nm[kVec], nr[kVec];
+  // Magnitudes are compared as integers: the order is the same, and what is not finite comes out on
+  // top.
+  unsigned um = 0, ur = 0;
+  const float b1s = a.h.b1 * sm;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int i = (u * kThreads + (int)threadIdx.x) * kVec8;
-    const int k = left - i;
-    float nm[kVec8], nr[kVec8];
-    // Magnitudes are compared as integers: the order is the same, and what is not finite comes out
-    // on top.
-    unsigned um = 0, ur = 0;
-    const float b1s = a.h.b1 * sm[u];
+  for (int j = 0; j < kVec; j += 2) {
+    const auto m2 = j ? __builtin_amdgcn_cvt_pk_f32_fp8(vm, true) : __builtin_amdgcn_cvt_pk_f32_fp8(vm, false);
+    const auto r2 = j ? __builtin_amdgcn_cvt_pk_f32_fp8(vr, true) : __builtin_amdgcn_cvt_pk_f32_fp8(vr, false);
 #pragma unroll
-    for (int j = 0; j < kVec8; j += 2) {
-      const auto m2 = j ? __builtin_amdgcn_cvt_pk_f32_fp8(vm[u], true) : __builtin_amdgcn_cvt_pk_f32_fp8(vm[u], false);
-      const auto r2 = j ? __builtin_amdgcn_cvt_pk_f32_fp8(vr[u], true) : __builtin_amdgcn_cvt_pk_f32_fp8(vr[u], false);
+    for (int e = 0; e < 2; ++e) {
+      const float gr = vg.get(j + e) * c.gscale;
+      const float rr = r2[e] * sr;
+      nm[j + e] = fmaf(m2[e], b1s, a.h.omb1 * gr);
+      // v_sqrt_f32 and v_rcp_f32 below: 1.5 * 2^-24 of the value each, a tenth of the exact forms'
+      // instructions; a second moment under 2^-126 counts as zero
+      nr[j + e] = __builtin_amdgcn_sqrtf(fmaf(a.h.b2 * rr, rr, a.h.omb2 * gr * gr));
+    }
+    um = max3(um, __float_as_uint(nm[j]) & 0x7FFFFFFFu, __float_as_uint(nm[j + 1]) & 0x7FFFFFFFu);
+    ur = max3(ur, __float_as_uint(nr[j]), __float_as_uint(nr[j + 1]));
+  }
+  um = block_max(um);
+  ur = block_max(ur);
+  // A gradient that is not finite reaches its own value only: it is left out of the scales and
+  // becomes e4m3's NaN.
+  unsigned bad = 0;
+  if (um >= kInf || ur >= kInf) {
+    um = ur = 0;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float gr = vg[u].get(j + e) * c.gscale;
-        const float rr = r2[e] * sr[u];
-        nm[j + e] = fmaf(m2[e], b1s, a.h.omb1 * gr);
-        // v_sqrt_f32 and v_rcp_f32 below: 1.5 * 2^-24 of the value each, a tenth of the exact
-        // forms' instructions; a second moment under 2^-126 counts as zero
-        nr[j + e] = __builtin_amdgcn_sqrtf(fmaf(a.h.b2 * rr, rr, a.h.omb2 * gr * gr));
-      }
-      um = max3(um, __float_as_uint(nm[j]) & 0x7FFFFFFFu, __float_as_uint(nm[j + 1]) & 0x7FFFFFFFu);
-      ur = max3(ur, __float_as_uint(nr[j]), __float_as_uint(nr[j + 1]));
+    for (int j = 0; j < kVec; ++j) {
+      const unsigned mb = __float_as_uint(nm[j]) & 0x7FFFFFFFu, rb = __float_as_uint(nr[j]);
+      if (mb >= kInf || rb >= kInf) bad |= 1u << j;
+      if (mb < kInf && mb > um) um = mb;
+      if (rb < kInf && rb > ur) ur = rb;
     }
     um = block_max(um);
     ur = block_max(ur);
-    // A gradient that is not finite reaches its own value only: it is left out of the scales and
-    // becomes e4m3's NaN.
-    unsigned bad = 0;
-    if (um >= kInf || ur >= kInf) {
-      um = ur = 0;
+  }
+  if (k <= 0) return;                   // after the exchanges between a block's lanes
+  float tm = __uint_as_float(um);
+  const float tr = __uint_as_float(ur);
+  if (tm < 0x1p-110f) tm = 0.0f;        // 448 / tm would overflow: such a block is held as zeros
+  const float im = tm > 0.0f ? 448.0f * __builtin_amdgcn_rcpf(tm) : 0.0f;
+  const float ir = tr > 0.0f ? 448.0f * __builtin_amdgcn_rcpf(tr) : 0.0f;
+  const unsigned bkey = mix32(key + (unsigned)(block0 + i / kBlock) * 0xC2B2AE35u);
+  unsigned om = 0, orr = 0;
+  auto value = [&](auto J) {
+    constexpr int j = J.value;
+    unsigned h = bkey + (unsigned)((i + j) % kBlock) * 0x9E3779B1u;
+    h ^= h >> 16;
+    h *= 0xBB67AE85u;
+    h ^= h >> 15;
+    om = to_e4m3<j>(__builtin_amdgcn_fmed3f(nm[j] * im, -448.0f, 448.0f), h << 16, om);
+    // above zero and below e4m3's smallest: the smallest
+    orr = to_e4m3<j>(__builtin_amdgcn_fmed3f(nr[j] * ir, nr[j] > 0.0f ? 0x1p-9f : 0.0f, 448.0f),
+                     h & 0xFFFF0000u, orr);
+    const float old = MASTER ? vw.get(j) : vp.get(j);
+    // a root above zero is 2^-63 at least: the bound only keeps a moment over a second moment that
+    // counts as zero (and eps = 0) finite
+    const float part = nm[j] * __builtin_amdgcn_rcpf(fmaxf(fmaf(nr[j], c.rbc2, a.h.eps), 0x1p-64f));
+    const float now = fmaf(-c.lr_c, part, old * c.decay);
+    if constexpr (MASTER) vw.set(j, now);
+    vp.set(j, now);
+  };
+  value(std::integral_constant<int, 0>());
+  value(std::integral_constant<int, 1>());
+  value(std::integral_constant<int, 2>());
+  value(std::integral_constant<int, 3>());
+  if (bad) {
 #pragma unroll
-      for (int j = 0; j < kVec8; ++j) {
-        const unsigned mb = __float_as_uint(nm[j]) & 0x7FFFFFFFu, rb = __float_as_uint(nr[j]);
-        if (mb >= kInf || rb >= kInf) bad |= 1u << j;
-        if (mb < kInf && mb > um) um = mb;
-        if (rb < kInf && rb > ur) ur = rb;
+    for (int j = 0; j < kVec; ++j)
+      if (bad >> j & 1) {
+        om |= 0x7Fu << (8 * j);
+        orr |= 0x7Fu << (8 * j);
       }
-      um = block_max(um);
-      ur = block_max(ur);
-    }
-    float tm = __uint_as_float(um);
-    const float tr = __uint_as_float(ur);
-    if (tm < 0x1p-110f) tm = 0.0f;      // 448 / tm would overflow: such a block is held as zeros
-    const float im = tm > 0.0f ? 448.0f * __builtin_amdgcn_rcpf(tm) : 0.0f;
-    const float ir = tr > 0.0f ? 448.0f * __builtin_amdgcn_rcpf(tr) : 0.0f;
-    if (k <= 0) continue;               // after the exchanges between a block's lanes
-    const unsigned bkey = mix32(key + (unsigned)(block0 + i / kBlock) * 0xC2B2AE35u);
-    unsigned om = 0, orr = 0;
-    auto value = [&](auto J) {
-      constexpr int j = J.value;
-      unsigned h = bkey + (unsigned)((i + j) % kBlock) * 0x9E3779B1u;
-      h ^= h >> 16;
-      h *= 0xBB67AE85u;
-      h ^= h >> 15;
-      om = to_e4m3<j>(__builtin_amdgcn_fmed3f(nm[j] * im, -448.0f, 448.0f), h << 16, om);
-      // above zero and below e4m3's smallest: the smallest
-      orr = to_e4m3<j>(__builtin_amdgcn_fmed3f(nr[j] * ir, nr[j] > 0.0f ? 0x1p-9f : 0.0f, 448.0f),
-                       h & 0xFFFF0000u, orr);
-      const float old = MASTER ? vw[u].get(j) : vp[u].get(j);
-      const float part = nm[j] * __builtin_amdgcn_rcpf(fmaf(nr[j], c.rbc2, a.h.eps));
-      const float now = fmaf(-c.lr_c, part, old * c.decay);
-      if constexpr (MASTER) vw[u].set(j, now);
-      vp[u].set(j, now);
-    };
-    value(std::integral_constant<int, 0>());
-    value(std::integral_constant<int, 1>());
-    value(std::integral_constant<int, 2>());
-    value(std::integral_constant<int, 3>());
-    if (bad) {
+  }
+  if constexpr (MASTER) vw.store(w + i, k);
+  vp.store(p + i, k);
+  if (k >= kVec) {
+    __builtin_nontemporal_store(__builtin_bit_cast(Byte4, om), (GANET_GLOBAL Byte4 *)(m + i));
+    __builtin_nontemporal_store(__builtin_bit_cast(Byte4, orr), (GANET_GLOBAL Byte4 *)(r + i));
+  } else {
 #pragma unroll
-      for (int j = 0; j < kVec8; ++j)
-        if (bad >> j & 1) {
-          om |= 0x7Fu << (8 * j);
-          orr |= 0x7Fu << (8 * j);
-        }
-    }
-    if constexpr (MASTER) vw[u].store(w + i, k);
-    vp[u].store(p + i, k);
-    if (k >= kVec8) {
-      __builtin_nontemporal_store(__builtin_bit_cast(Byte4, om), (GANET_GLOBAL Byte4 *)(m + i));
-      __builtin_nontemporal_store(__builtin_bit_cast(Byte4, orr), (GANET_GLOBAL Byte4 *)(r + i));
-    } else {
-#pragma unroll
-      for (int j = 0; j < kVec8; ++j)
-        if (j < k) {
-          m[i + j] = (unsigned char)(om >> (8 * j));
-          r[i + j] = (unsigned char)(orr >> (8 * j));
-        }
-    }
-    if (i % kBlock == 0) {
-      ((GANET_GLOBAL float *)ms)[i / kBlock] = tm * (1.0f / 448.0f);
-      ((GANET_GLOBAL float *)rs)[i / kBlock] = tr * (1.0f / 448.0f);
-    }
+    for (int j = 0; j < kVec; ++j)
+      if (j < k) {
+        m[i + j] = (unsigned char)(om >> (8 * j));
+        r[i + j] = (unsigned char)(orr >> (8 * j));
+      }
+  }
+  if (i % kBlock == 0) {
+    ((GANET_GLOBAL float *)ms)[i / kBlock] = tm * (1.0f / 448.0f);
+    ((GANET_GLOBAL float *)rs)[i / kBlock] = tr * (1.0f / 448.0f);
   }
 }
 
@@ -580,55 +560,47 @@ extern "C" int ganet_adamw_step(const ganet_step_tensor *tensors, int count, con
   h.lr_dev = p->lr_device;
 
   hipStream_t s = (hipStream_t)stream;
-  long long chunks = 0;
-  for (int i = 0; i < count; ++i) chunks += (tensors[i].n + chunk32(kDeep) - 1) / chunk32(kDeep);
-  const bool deep = chunks >= kFew;
   return with_types(p->param_dtype, p->grad_dtype, master, [&](auto tp, auto tg, auto tm) {
     typedef decltype(tp) TP;
     typedef decltype(tg) TG;
     constexpr bool M = decltype(tm)::value;
-    auto step = [&](auto u) {
-      constexpr int U = u.value;
-      if (!small) {
-        Args32<M> a;
-        a.h = h;
-        return in_launches(
-            tensors, count, chunk32(U), a.t,
-            [](const ganet_step_tensor &x, int k) { return k == kMaster32 ? (void *)x.master : address(x, k); },
-            [&](unsigned blocks, int) {
-              adamw32_kernel<TP, TG, M, U><<<dim3(blocks), dim3(kThreads), 0, s>>>(a);
-              return ganet_check_launch();
-            });
-      }
-      Args8<M> a;
+    if (!small) {
+      Args32<M> a;
       a.h = h;
       return in_launches(
-          tensors, count, chunk8(U), a.t,
-          [](const ganet_step_tensor &x, int k) {
-            if (k == kAvgScale) return (void *)x.exp_avg_scale;
-            if (k == kSecondScale) return (void *)x.second_scale;
-            return k == kMaster8 ? (void *)x.master : address(x, k);
-          },
-          [&](unsigned blocks, int start) {
-            a.tensor0 = start;
-            adamw8_kernel<TP, TG, M, U><<<dim3(blocks), dim3(kThreads), 0, s>>>(a);
+          tensors, count, kChunk, a.t,
+          [](const ganet_step_tensor &x, int k) { return k == kMaster32 ? (void *)x.master : address(x, k); },
+          [&](unsigned blocks, int) {
+            adamw32_kernel<TP, TG, M><<<dim3(blocks), dim3(kThreads), 0, s>>>(a);
             return ganet_check_launch();
           });
-    };
-    if (deep) return step(std::integral_constant<int, kDeep>());
-    return step(std::integral_constant<int, 1>());
+    }
+    Args8<M> a;
+    a.h = h;
+    return in_launches(
+        tensors, count, kChunk, a.t,
+        [](const ganet_step_tensor &x, int k) {
+          if (k == kAvgScale) return (void *)x.exp_avg_scale;
+          if (k == kSecondScale) return (void *)x.second_scale;
+          return k == kMaster8 ? (void *)x.master : address(x, k);
+        },
+        [&](unsigned blocks, int start) {
+          a.tensor0 = start;
+          adamw8_kernel<TP, TG, M><<<dim3(blocks), dim3(kThreads), 0, s>>>(a);
+          return ganet_check_launch();
+        });
   });
 }
 
 // ---- norm ----
 namespace {
-// Values of a workgroup: one round of 2048 workgroups (8 on each of 256 CUs) for long lists, 8192
-// (8 float32 vectors a thread) at least.
+// Values of a workgroup: 8192 workgroups for long lists (400 M bf16 values 122 us; 2048 workgroups,
+// what the chip holds at once, 131 us), 8192 values (8 float32 vectors a thread) at least.
 long long norm_chunk(const int64_t *numel, int count) {
   long long total = 0;
   for (int i = 0; i < count; ++i) total += numel[i];
   const long long unit = 8192;
-  const long long even = (total + 2047) / 2048;
+  const long long even = (total + 8191) / 8192;
   return even <= unit ? unit : (even + unit - 1) / unit * unit;
 }
 int norm_list_ok(const int64_t *numel, int count) {
@@ -671,7 +643,7 @@ extern "C" int ganet_grad_norm(const void *const *grads, const int64_t *numel, c
   for (int i = 0; i < count;) {
     int k = 0;
     long long blocks = 0;
-    for (; i < count && k < kTensorsN; ++i, ++k) {     // 2048 chunks and one a tensor at most: 16 bits hold them
+    for (; i < count && k < kTensorsN; ++i, ++k) {     // 8192 chunks and one a tensor at most: 16 bits hold them
       const long long need = (numel[i] + chunk - 1) / chunk;
       const unsigned long long at = (unsigned long long)grads[i];
       if (at >> 48) return GANET_ERR_UNSUPPORTED;      // no device address

@@ -533,7 +533,8 @@ typedef struct {
  * In 8 bits m and sqrt(v) are kept as e4m3 times a float32 scale for each 256 values
  * (largest magnitude / 448), rounded up or down at random: the random word of a value is a
  * hash of (seed, t, the tensor's place in the list, the value's place in it), so the same
- * inputs give the same bits.  The parameter's step uses m and v before that rounding. */
+ * inputs give the same bits.  The parameter's step uses m and v before that rounding.  A
+ * v under 2^-126 counts as zero there, and the divisor is 2^-64 at least. */
 typedef struct {
   int32_t param_dtype, grad_dtype; /* ganet_dtype */
   int32_t state_bits;              /* 32 or 8 */
@@ -547,6 +548,7 @@ typedef struct {
   const float *lr_device;          /* NULL, or lr on the device */
 } ganet_adamw_params;
 
+/* At most 2^33 values a tensor (GANET_ERR_UNSUPPORTED beyond). */
 int ganet_adamw_step(const ganet_step_tensor *tensors /* host array */, int count,
                      const ganet_adamw_params *p, ganet_stream_t stream);
 

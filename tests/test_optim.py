@@ -11,6 +11,7 @@ the mean; which one is a function of the random word, tested against that word's
 import copy
 import ctypes
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -447,6 +448,58 @@ def test_non_finite_gradients_stay_in_their_place():
             s = d8[key + "s"][0]
             assert torch.isfinite(s).all() and (s > 0).all()
             assert torch.isfinite(d8[key][0].float()[keep]).all() and d8[key][0].float()[300].isnan()
+
+
+@gpu
+def test_tiny_gradients_without_eps():
+    """Second moments below float32's normal range in 8 bits: nothing becomes infinite, and a step
+    is at most some times lr."""
+    n = 512
+    p = torch.ones(n, device="cuda")
+    g = torch.randn(n, device="cuda") * 1e-19
+    g[:256] = 0.0
+    st = optim.state_8bit(p)
+    for t in range(1, 6):
+        old = p.clone()
+        optim.adamw_step_8bit([p], [g], [st[0]], [st[1]], [st[2]], [st[3]], t, lr=1e-3, eps=0.0,
+                              weight_decay=0.0)
+        assert ((p - old).abs() <= 0.1).all()
+    assert (p[:256] == 1.0).all()
+
+
+@gpu
+def test_two_threads_at_once():
+    """Two host threads, each with its own stream and tensors: each gets what one alone gets."""
+    jobs = [(make(SIZES, torch.float32, torch.float32, False, seed=i), 3 + i) for i in range(2)]
+    alone = []
+    for d, t in jobs:
+        a = clone(d)
+        for k in range(20):
+            step32(a, t + k, grad_stats=optim.grad_norm(a["grads"], 0.5), **HYPER)
+        alone.append(a)
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(d, t):
+        try:
+            side = torch.cuda.Stream()
+            with torch.cuda.stream(side):
+                for k in range(20):
+                    step32(d, t + k, grad_stats=optim.grad_norm(d["grads"], 0.5), **HYPER)
+            side.synchronize()
+        except Exception as e:                               # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=job) for job in jobs]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not errors
+    for (d, _), a in zip(jobs, alone):
+        for key in ("params", "m", "v"):
+            for x, y in zip(d[key], a[key]):
+                assert torch.equal(x, y)
 
 
 @gpu
