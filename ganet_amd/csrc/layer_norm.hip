@@ -630,11 +630,9 @@ __global__ __launch_bounds__(64 * WAVES, 4) void ln_planes_bwd(Args a, int tiles
         vg[k].load(g + k * a.inner);
       }
     }
-    Vec<float, N> shift, rstd;                       // xh = x rstd - mean rstd
-    shift.load(a.mean + img * a.inner + pos);
+    Vec<float, N> mean, rstd;
+    mean.load(a.mean + img * a.inner + pos);
     rstd.load(a.rstd + img * a.inner + pos);
-#pragma unroll
-    for (int j = 0; j < N; ++j) shift.v[j] *= -rstd.v[j];
     float m[2 * N];                                  // sums of a, of a xh
 #pragma unroll
     for (int j = 0; j < 2 * N; ++j) m[j] = 0.0f;
@@ -644,7 +642,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void ln_planes_bwd(Args a, int tiles
         const float w = c0 + k < a.C ? weights[c0 + k] : 0.0f;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-          const float xh = fmaf(vx[k].get(j), rstd.v[j], shift.v[j]), dy = vg[k].get(j);
+          const float xh = (vx[k].get(j) - mean.v[j]) * rstd.v[j], dy = vg[k].get(j);
           const float wa = dy * w;
           m[j] += wa;
           m[N + j] = fmaf(wa, xh, m[N + j]);
@@ -674,7 +672,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void ln_planes_bwd(Args a, int tiles
         Vec<T, N> o;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-          const float xh = fmaf(vx[k].get(j), rstd.v[j], shift.v[j]);
+          const float xh = (vx[k].get(j) - mean.v[j]) * rstd.v[j];
           o.set(j, rstd.v[j] * (vg[k].get(j) * w - m[j] - xh * m[N + j]));
         }
         o.store_kept(dx + k * a.inner);
@@ -833,9 +831,9 @@ long long tiles_of(const ganet_layer_norm_params *p, int tile) { return (p->inne
 enum { kAny = 0 };
 template <bool BACKWARD, typename T, typename F>
 int with_plane_shape(const ganet_layer_norm_params *p, F &&f) {
-#define GANET_PLANE(VB, NC, WAVES)                                                                      \
-  if (p->C <= 4 * (WAVES) * (NC) && p->inner >= (VB) / (int)sizeof(T))                                                                          \
-    return f(std::integral_constant<int, VB>(), std::integral_constant<int, NC>(),                      \
+#define GANET_PLANE(VB, NC, WAVES)                                                  \
+  if (p->C <= 4 * (WAVES) * (NC) && p->inner >= (VB) / (int)sizeof(T))              \
+    return f(std::integral_constant<int, VB>(), std::integral_constant<int, NC>(),  \
              std::integral_constant<int, WAVES>())
   if constexpr (!BACKWARD) {
     GANET_PLANE(16, 16, 1);

@@ -232,6 +232,7 @@ def test_other_strides_and_orders():
 def test_large_mean_and_constant_rows():
     x, w, b, g = make((40, 320), -1, torch.float32, torch.float32, offset=1000.0)
     both(x, w, b, g, -1)
+    both(*make((3, 40, 9, 7), 1, torch.float32, torch.float32, offset=1000.0), 1)
     x = torch.full((7, 96), 3.25, device="cuda")                    # no variance: y is the bias
     y, mean, rstd = norm.layer_norm_forward(x, w[:96], b[:96])
     assert torch.equal(y, b[:96].expand(7, 96)) and (mean == 3.25).all()
@@ -428,3 +429,50 @@ def test_more_rows_than_a_launch_takes():
     b = torch.full((1,), 0.75, dtype=torch.bfloat16, device="cuda")
     y = norm.layer_norm(x, None, b)
     assert float(y.min()) == float(y.max()) == 0.75
+
+
+@gpu
+@pytest.mark.parametrize("layout", ["rows", "nchw", "nhwc"])
+def test_captured_training_step(layout):
+    """Forward, backward and the optimizer's step in one captured graph, replayed with new inputs,
+    against the same steps taken eagerly."""
+    from ganet_amd import optim
+    dim, shape = (-1, (130, 48)) if layout == "rows" else (1, (2, 48, 5, 13))
+    x, _, _, g = make(shape, dim, torch.float32, torch.float32)
+    if layout == "nhwc":
+        x, g = (t.contiguous(memory_format=torch.channels_last) for t in (x, g))
+
+    def build():
+        m = norm.LayerNorm(48, channel_dim=dim).cuda()
+        return m, optim.AdamW(m.parameters(), lr=1e-2, capturable=True, max_grad_norm=1.0)
+
+    def step(m, o):
+        for p in m.parameters():
+            p.grad = None
+        m(x).backward(g)
+        o.step()
+
+    (m, o), (twin, e) = build(), build()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):                    # states and first launches, outside the graph
+        step(m, o)
+    torch.cuda.current_stream().wait_stream(side)
+    step(twin, e)
+    torch.cuda.synchronize()
+    for p in m.parameters():
+        p.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        m(x).backward(g)
+        o.step()
+    for turn in range(4):
+        fresh = make(shape, dim, torch.float32, torch.float32, seed=turn + 1)
+        x.copy_(fresh[0])
+        g.copy_(fresh[3])
+        torch.cuda.synchronize()
+        graph.replay()
+        step(twin, e)
+        torch.cuda.synchronize()
+        for p, q in zip(m.parameters(), twin.parameters()):
+            assert torch.equal(p, q), turn
