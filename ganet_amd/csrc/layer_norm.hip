@@ -201,7 +201,7 @@ __device__ __forceinline__ float row_sum(float v, float *part, int slot) {
     constexpr int W = LANES / 64;
     v = group_sum<64>(v);
     if ((threadIdx.x & 63) == 0) part[slot * W + (threadIdx.x >> 6)] = v;
-    __syncthreads();
+    ganet_vec::lds_barrier();
     v = 0.0f;
 #pragma unroll
     for (int i = 0; i < W; ++i) v += part[slot * W + i];
@@ -299,7 +299,7 @@ __global__ __launch_bounds__(kBwdThreads) void ln_rows_bwd(Args a) {
   float w_reg[LDS_W ? 1 : NV][N], dw[NV][N], db[NV][N];
   if constexpr (LDS_W) {
     for (int c = threadIdx.x; c < COLS; c += kBwdThreads) w_lds[c] = c < a.C ? load_weight(a.w, a.wdtype, c, 1.0f) : 0.0f;
-    __syncthreads();
+    ganet_vec::lds_barrier();
   }
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
@@ -383,7 +383,7 @@ __global__ __launch_bounds__(kBwdThreads) void ln_rows_bwd(Args a) {
         p[threadIdx.x >> 6] = s1;
         p[kBwdThreads / 64 + (threadIdx.x >> 6)] = s2;
       }
-      __syncthreads();
+      ganet_vec::lds_barrier();
       m1 = m2 = 0.0f;
 #pragma unroll
       for (int i = 0; i < W; ++i) {
@@ -427,7 +427,7 @@ __global__ __launch_bounds__(kBwdThreads) void ln_rows_bwd(Args a) {
     }
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-      __syncthreads();
+      ganet_vec::lds_barrier();
       if (LANES >= 64 || ((int)threadIdx.x & 63) < LANES) {
 #pragma unroll
         for (int v = 0; v < NV; ++v)
@@ -435,7 +435,7 @@ __global__ __launch_bounds__(kBwdThreads) void ln_rows_bwd(Args a) {
           for (int k = 0; k < N; ++k)
             sums[mine * COLS + (v * LANES + l) * N + k] = which ? db[v][k] : dw[v][k];
       }
-      __syncthreads();
+      ganet_vec::lds_barrier();
       for (int c = threadIdx.x; c < a.C; c += kBwdThreads) {
         float s = 0.0f;
 #pragma unroll
@@ -482,7 +482,7 @@ __device__ __forceinline__ void slots_sum(float (&s)[M], float (*part)[64][M / 4
     s[i] += s[i + Q];                   // rows: values i, i + Q, i + 2 Q, i + 3 Q
     part[wave][lane][i] = s[i];
   }
-  __syncthreads();
+  ganet_vec::lds_barrier();
 #pragma unroll
   for (int i = 0; i < Q; ++i) s[i] = part[0][lane][i];
 #pragma unroll
@@ -505,14 +505,13 @@ __device__ __forceinline__ void slots_sum(float (&s)[M], float (*part)[64][M / 4
 // own: it gets an eighth of the tiles, neighbours one after another, so that the cache lines that two
 // tiles share (planes start at any address) meet in one L2.
 struct Share {
-  long long end, step, at;
-  __device__ __forceinline__ explicit Share(long long tiles) {
-    const long long per = (tiles + 7) / 8, from = (blockIdx.x & 7) * per;
+  unsigned end, step, at;                            // fewer than 2^31 tiles (with_plane_shape)
+  __device__ __forceinline__ explicit Share(unsigned tiles) {
+    const unsigned per = (tiles + 7) / 8, from = (blockIdx.x & 7) * per;
     at = from + (blockIdx.x >> 3);
     end = from + per < tiles ? from + per : tiles;
     step = (gridDim.x + 7 - (blockIdx.x & 7)) >> 3;
   }
-  __device__ __forceinline__ long long first() const { return at; }
 };
 
 // Where a lane's N positions begin.  A vector that would pass the plane's end is moved back to end
@@ -533,11 +532,12 @@ __global__ __launch_bounds__(64 * WAVES) void ln_planes_fwd(Args a, int tiles, i
   __shared__ __align__(16) float part[2][WAVES][64][N / 4];
   __shared__ float weights[2][P::SLOTS * NC];
   int own;
-  const Share share(a.outer * tiles);
-  const long long i = share.first();
-  if (i >= share.end) return;
-  const long long img = i / tiles;
-  const long long pos = plane_position<N>((i % tiles) * P::TILE + (threadIdx.x & 15) * N, a.inner, own);
+  const Share share((unsigned)a.outer * (unsigned)tiles);
+  if (share.at >= share.end) return;
+  const unsigned image = share.at / (unsigned)tiles;
+  const long long img = image;
+  const long long pos = plane_position<N>(
+      (long long)(share.at - image * (unsigned)tiles) * P::TILE + (threadIdx.x & 15) * N, a.inner, own);
   const int c0 = (int)(threadIdx.x >> 4) * nc;       // nc <= NC channels of a slot
   const T *x = (const T *)a.x + img * a.xs + (long long)c0 * a.inner + pos;
   Vec<T, N> v[NC];
@@ -599,7 +599,8 @@ __global__ __launch_bounds__(64 * WAVES) void ln_planes_fwd(Args a, int tiles, i
   }
 }
 
-// Backward: 16 wavefronts a CU (128 registers), however they are grouped.
+// Backward: 16 wavefronts a CU (128 registers), however they are grouped.  Loading the next tile into
+// registers meanwhile was measured and gains nothing (bf16 32x256x40x100 47.4 and 47.6 us).
 template <typename T, int VB, int NC, int WAVES, bool SUMS>
 __global__ __launch_bounds__(64 * WAVES, 4) void ln_planes_bwd(Args a, int tiles, int nc) {
   typedef Plane<T, VB, NC, WAVES> P;
@@ -608,16 +609,18 @@ __global__ __launch_bounds__(64 * WAVES, 4) void ln_planes_bwd(Args a, int tiles
   __shared__ float weights[P::SLOTS * NC];
   const int c0 = (int)(threadIdx.x >> 4) * nc;
   for (int c = threadIdx.x; c < a.C; c += P::THREADS) weights[c] = load_weight(a.w, a.wdtype, c, 1.0f);
-  __syncthreads();
+  ganet_vec::lds_barrier();
   float dw[NC], db[NC];
 #pragma unroll
   for (int k = 0; k < NC; ++k) dw[k] = db[k] = 0.0f;
   int turn = 0;
-  const Share share(a.outer * tiles);
-  for (long long i = share.first(); i < share.end; i += share.step, turn ^= 1) {
+  const Share share((unsigned)a.outer * (unsigned)tiles);
+  for (unsigned i = share.at; i < share.end; i += share.step, turn ^= 1) {
     int own;
-    const long long img = i / tiles;
-    const long long pos = plane_position<N>((i % tiles) * P::TILE + (threadIdx.x & 15) * N, a.inner, own);
+    const unsigned image = i / (unsigned)tiles;
+    const long long img = image;
+    const long long pos = plane_position<N>(
+        (long long)(i - image * (unsigned)tiles) * P::TILE + (threadIdx.x & 15) * N, a.inner, own);
     const long long c_at = (long long)c0 * a.inner + pos;
     const T *x = (const T *)a.x + img * a.xs + c_at, *g = (const T *)a.g + img * a.gs + c_at;
     Vec<T, N> vx[NC], vg[NC];
@@ -832,7 +835,8 @@ enum { kAny = 0 };
 template <bool BACKWARD, typename T, typename F>
 int with_plane_shape(const ganet_layer_norm_params *p, F &&f) {
 #define GANET_PLANE(VB, NC, WAVES)                                                  \
-  if (p->C <= 4 * (WAVES) * (NC) && p->inner >= (VB) / (int)sizeof(T))              \
+  if (p->C <= 4 * (WAVES) * (NC) && p->inner >= (VB) / (int)sizeof(T) &&            \
+      p->outer * tiles_of(p, 16 * (VB) / (int)sizeof(T)) < kMostThreads / (64 * (WAVES)) - 8) \
     return f(std::integral_constant<int, VB>(), std::integral_constant<int, NC>(),  \
              std::integral_constant<int, WAVES>())
   if constexpr (!BACKWARD) {
@@ -913,19 +917,12 @@ int launch_forward(const ganet_layer_norm_params *p, const Args &a, hipStream_t 
       return (int)GANET_OK;
     });
   return with_plane_shape<false, T>(p, [&](auto vb, auto nc, auto waves) {
-    auto any = [&] {
+    if constexpr (vb.value == kAny) {
       const long long work = p->outer * tiles_of(p, kTile);
       ln_planes_any_fwd<T><<<dim3((unsigned)(work < 8192 ? work : 8192)), dim3(kThreads), 0, s>>>(a);
-    };
-    if constexpr (vb.value == kAny) {
-      any();
     } else {
       typedef Plane<T, vb.value, nc.value, waves.value> P;
       const long long tiles = tiles_of(p, P::TILE);
-      if (p->outer * tiles > kMostThreads / P::THREADS - 8) {    // more than a launch takes
-        any();
-        return ganet_check_launch();
-      }
       ln_planes_fwd<T, vb.value, nc.value, waves.value>
           <<<dim3((unsigned)((p->outer * tiles + 7) / 8 * 8)), dim3(P::THREADS), 0, s>>>(a, (int)tiles,
                                                                           (p->C + P::SLOTS - 1) / P::SLOTS);

@@ -129,6 +129,15 @@ __device__ __forceinline__ void swap_halves(float &a, float &b) {
   a = __uint_as_float(r[0]);
   b = __uint_as_float(r[1]);
 }
+// A barrier for what passes through LDS.  __syncthreads also waits for every load and store to
+// global memory under way; here none of them carries anything to another wavefront, and those for
+// the next tile or row are meant to stay under way.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // The sum over each group of W neighbouring lanes, in all of them.
 template <int W>
 __device__ __forceinline__ float group_sum(float v) {
