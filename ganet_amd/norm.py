@@ -236,6 +236,7 @@ class LayerNormFunction(Function):
     @staticmethod
     def forward(ctx, input, weight, bias, eps, channel_dim):
         ctx.channel_dim = channel_dim
+        ctx.bias_dtype = bias.dtype if bias is not None else None
         out, mean, rstd = _forward(input, weight, bias, eps, channel_dim,
                                    any(ctx.needs_input_grad))
         if mean is not None:
@@ -247,6 +248,10 @@ class LayerNormFunction(Function):
     def backward(ctx, grad_output):
         input, weight, mean, rstd = ctx.saved_tensors
         want = ctx.needs_input_grad
+        if weight is None and want[2] and ctx.bias_dtype != input.dtype:
+            # the sums of a bias alone are rounded to the weight's dtype: one of the bias's, of ones
+            weight = torch.ones(input.shape[ctx.channel_dim], dtype=ctx.bias_dtype,
+                                device=input.device)
         return layer_norm_backward(input, weight, grad_output, mean, rstd, ctx.channel_dim,
                                    *want[:3]) + (None, None)
 

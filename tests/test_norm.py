@@ -332,6 +332,17 @@ def test_autograd_and_module():
 
 
 @gpu
+def test_a_bias_alone_keeps_its_precision():
+    """257 gradients of one and one of 2^-7 a channel: float32 holds their sum, bfloat16 does not."""
+    x = torch.randn(258, 33, device="cuda").bfloat16()
+    b = torch.zeros(33, device="cuda", requires_grad=True)
+    g = torch.ones(258, 33, device="cuda").bfloat16()
+    g[0] = 2.0 ** -7
+    norm.layer_norm(x, None, b).backward(g)
+    assert b.grad.dtype == torch.float32 and bool((b.grad == 257 + 2.0 ** -7).all())
+
+
+@gpu
 def test_refusals():
     x = torch.zeros(4, 8, device="cuda")
     with pytest.raises(TypeError):
