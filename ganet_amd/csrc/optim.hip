@@ -485,7 +485,6 @@ int in_launches(const ganet_step_tensor *ts, int count, long long chunk, Table<P
     long long blocks = 0;
     for (; i < count && k < MOST; ++i, ++k) {
       const long long n = ts[i].n, need = (n + chunk - 1) / chunk;
-      if (need > kMostBlocks) return GANET_ERR_UNSUPPORTED;
       if (blocks + need > kMostBlocks) break;
       tab.first[k] = (int)blocks;
       tab.tail[k] = (unsigned short)(n - (need - 1) * chunk);      // not read where need == 0
@@ -533,6 +532,7 @@ extern "C" int ganet_adamw_step(const ganet_step_tensor *tensors, int count, con
     if ((t.master != nullptr) != master) return GANET_ERR_BAD_SHAPE;
     if (!t.param || !t.grad || !t.exp_avg || !t.second) return GANET_ERR_NULL;
     if (small && (!t.exp_avg_scale || !t.second_scale)) return GANET_ERR_NULL;
+    if (t.n > kMostBlocks * kChunk) return GANET_ERR_UNSUPPORTED;    // before any tensor is stepped
   }
   if (master && p->param_dtype == GANET_F32) return GANET_ERR_BAD_SHAPE;
 
@@ -633,6 +633,7 @@ extern "C" int ganet_grad_norm(const void *const *grads, const int64_t *numel, c
   for (int i = 0; i < count; ++i) {
     if (!dtype_ok(dtypes[i])) return GANET_ERR_BAD_SHAPE;
     if (numel[i] > 0 && !grads[i]) return GANET_ERR_NULL;
+    if ((unsigned long long)grads[i] >> 48) return GANET_ERR_UNSUPPORTED;      // no device address
   }
   if (workspace_bytes < ganet_grad_norm_workspace_bytes(numel, count)) return GANET_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
@@ -646,7 +647,6 @@ extern "C" int ganet_grad_norm(const void *const *grads, const int64_t *numel, c
     for (; i < count && k < kTensorsN; ++i, ++k) {     // 8192 chunks and one a tensor at most: 16 bits hold them
       const long long need = (numel[i] + chunk - 1) / chunk;
       const unsigned long long at = (unsigned long long)grads[i];
-      if (at >> 48) return GANET_ERR_UNSUPPORTED;      // no device address
       a.low[k] = (unsigned)at;
       a.high_first[k] = (unsigned)(at >> 32) << 16 | (unsigned)blocks;
       a.tail_type[k] = (unsigned)dtypes[i] << 30 | (need ? (unsigned)(numel[i] - (need - 1) * chunk) : 0);

@@ -257,6 +257,21 @@ def test_c_abi_refusals_without_gpu():
     assert L.ganet_grad_norm_workspace_bytes((ctypes.c_int64 * 1)(-5), 1) == 0
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_too_large_a_tensor_is_refused_before_any_step(bits):
+    """At the end of a list that takes two launches: nothing is launched (that would be an error of
+    another kind without a GPU)."""
+    n = 200
+    ts = (_lib.StepTensor * n)(*[
+        _lib.StepTensor(param=256, grad=256, exp_avg=256, second=256, exp_avg_scale=256,
+                        second_scale=256, master=None, n=16) for _ in range(n)])
+    ts[n - 1].n = (1 << 33) + 1
+    p = _lib.AdamwParams(param_dtype=0, grad_dtype=0, state_bits=bits, step=1, lr=1e-3, beta1=0.9,
+                         beta2=0.999, eps=1e-8, weight_decay=0.0)
+    rc = _lib.lib().ganet_adamw_step(ts, n, ctypes.byref(p), None)
+    assert rc == _lib.GANET_ERR_UNSUPPORTED
+
+
 def test_dense_and_order():
     t = torch.zeros(4, 3, 5, 7)
     cl = t.contiguous(memory_format=torch.channels_last)
