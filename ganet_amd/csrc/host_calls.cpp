@@ -127,6 +127,21 @@ PyObject *grads(PyObject *, PyObject *list) {
   }
 }
 
+// written(list): the tensors' values have changed, so that autograd refuses a backward pass that saved
+// the old ones, as it does after torch's own in-place operations.
+PyObject *written(PyObject *, PyObject *list) {
+  try {
+    for (Py_ssize_t i = 0, n = length(list); i < n; ++i) {
+      const at::Tensor *t = item(list, i);
+      if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();   // those have no versions
+    }
+    Py_RETURN_NONE;
+  } catch (const std::exception &e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
 // ---- layer norm -----------------------------------------------------------------------------
 // The calls of ganet_amd/norm.py where tensors lie as the kernels take them: in Python the outputs,
 // the parameters and the checks of a small call cost more than its kernel.
@@ -287,6 +302,7 @@ PyMethodDef methods[] = {
     {"step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(step)), METH_FASTCALL,
      "The table of an AdamW step over plain lists of tensors, or None."},
     {"grads", grads, METH_O, "Addresses, sizes and types of a plain list of gradients, or None."},
+    {"written", written, METH_O, "Marks a list of tensors as changed in place."},
     {"layer_norm_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(layer_norm_forward)),
      METH_FASTCALL, "Layer norm's forward on tensors in the kernels' order, or None."},
     {"layer_norm_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(layer_norm_backward)),

@@ -173,6 +173,9 @@ def _step(params, grads, avgs, seconds, avg_scales, second_scales, bits, step, l
     rc = _lib.call(index, _lib.lib().ganet_adamw_step, rows, n, ctypes.byref(h))
     if rc:
         _lib.check(rc, "ganet_adamw_step")
+    for ts in (params, masters):
+        if ts is not None:
+            _lib.host().written(list(ts))
 
 
 def _scalar(t, dtype, index, what):

@@ -692,6 +692,28 @@ def test_another_stream():
 
 
 @gpu
+@pytest.mark.parametrize("order", [torch.contiguous_format, torch.channels_last])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_is_a_change_in_place(bits, order):
+    """A backward pass that saved the weights of before the step is refused, as after torch's."""
+    p = torch.ones(2, 3, 40, 50, device="cuda").contiguous(memory_format=order).bfloat16()
+    p.requires_grad_()
+    opt = optim.AdamW([p], state_bits=bits, master_weights=True)
+    for _ in range(2):                       # a fresh state, a kept one
+        loss = (p.float() * p.float()).sum() + (p * p).sum()
+        p.grad = torch.ones_like(p)
+        before = p._version, opt.state[p]["master"]._version if p in opt.state else 0
+        opt.step()
+        assert p._version > before[0] and opt.state[p]["master"]._version > before[1]
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
+    with torch.inference_mode():             # tensors without versions
+        q = [torch.ones(9, device="cuda") for _ in range(4)]
+        optim.adamw_step(q[:1], q[1:2], q[2:3], q[3:], 1)
+        assert float(q[0][0]) < 1
+
+
+@gpu
 @pytest.mark.parametrize("bits", [32, 8])
 def test_offsets_past_32_bits(bits):
     n, last = (1 << 31) + 1001, 777
