@@ -827,10 +827,9 @@ int with_row_shape(int C, F &&f) {
 long long tiles_of(const ganet_layer_norm_params *p, int tile) { return (p->inner + tile - 1) / tile; }
 
 // Planes.  Forward: 16 channels a slot, as many wavefronts as C takes (bf16 128x64x40x100: one
-// wavefront 22 us, four with four channels a slot 31 us; 8x1024x40x100: 28 us with this and with half
-// the wavefronts).  Backward, which keeps two maps and the channels' sums: eight channels a slot, and
-// four where 16-bit values make eight positions a lane (32x256x40x100: 45 us, with eight 50 us;
-// float32 with its four positions the other way round, 75 and 72 us).
+// wavefront 22 us, four with four channels a slot 31 us; float32 44 and 47 us).  Backward, which keeps two maps and the channels' sums: eight channels a slot, and
+// four where 16-bit values make eight positions a lane (64x128x40x100: 43 us, with eight 47 us;
+// 32x256x40x100: 47 and 48 us; float32 with its four positions the other way round, 75 and 72 us).
 enum { kAny = 0 };
 template <bool BACKWARD, typename T, typename F>
 int with_plane_shape(const ganet_layer_norm_params *p, F &&f) {
