@@ -21,6 +21,12 @@ static int32_t pick(int kind) {
   }
 }
 
+static int64_t pick64(int kind) {
+  static const int64_t far[] = {1ll << 31, (1ll << 33) + 1, 1ll << 40, (1ll << 40) + 1, 1ll << 46, 1ll << 60,
+                                INT64_MAX, INT64_MIN, -1};
+  return kind < 3 ? pick(kind) : (rng() % 2 ? far[rng() % 9] : (int64_t)rng());
+}
+
 int main() {
   unsigned long long acc = 0;
   for (int it = 0; it < 400000; ++it) {
@@ -59,6 +65,22 @@ int main() {
     d.max_groups = pick((int)(rng() % 4));
     d.flags = (int32_t)(rng() % 32);
     acc += ganet_decode_workspace_bytes(&d);
+
+    ganet_layer_norm_params n;
+    std::memset(&n, 0, sizeof n);
+    n.outer = pick64((int)(rng() % 4));
+    n.inner = rng() % 3 ? pick64((int)(rng() % 4)) : 1;
+    n.C = pick((int)(rng() % 3));
+    n.x_stride = rng() % 2 ? n.C * (n.inner & 0xFFFFFFFF) : pick64((int)(rng() % 4));
+    n.y_stride = rng() % 2 ? n.x_stride : pick64((int)(rng() % 4));
+    n.g_stride = rng() % 2 ? n.x_stride : pick64((int)(rng() % 4));
+    n.dtype = (int32_t)(rng() % 3);
+    n.weight_dtype = (int32_t)(rng() % 4);
+    acc += ganet_layer_norm_backward_workspace_bytes(&n);
+
+    int64_t numel[5];
+    for (int64_t &k : numel) k = wild == 3 ? pick64((int)(rng() % 4)) : (int64_t)(rng() % (1ull << (rng() % 41)));
+    acc += ganet_grad_norm_workspace_bytes(numel, (int)(rng() % 6));
   }
   std::printf("plan fuzz: 400000 parameter sets, checksum %llu\n", acc);
   return 0;
