@@ -155,6 +155,9 @@ __global__ __launch_bounds__(kThreads) void adamw32_kernel(Args32<MASTER> a) {
 // that keeps the mean: with beta2 = 0.999 an average moves by a thousandth a step, far less than
 // half of e4m3's spacing (2^-4), and rounding to nearest would stop it for good.  An r above zero
 // never becomes zero (m over a zero r would be a step of m / eps).
+// The new moments, their scales and what is rounded are formed by single float32 operations in a fixed
+// order (no contraction; root and reciprocal rounded to nearest): a state is the same bits wherever
+// the formula is computed so, and two trainings do not drift apart by roundings that fell otherwise.
 constexpr int kBlock = GANET_STATE_BLOCK;
 enum { kAvgScale = 4, kSecondScale, kMaster8 };
 template <bool MASTER>
@@ -183,6 +186,19 @@ __device__ __forceinline__ unsigned mix32(unsigned x) {
 template <int SEL>
 __device__ __forceinline__ unsigned to_e4m3(float v, unsigned random, unsigned to) {
   return (unsigned)__builtin_amdgcn_cvt_sr_fp8_f32(v, (int)(random | 0x8000u), (int)to, SEL);
+}
+
+// Root and reciprocal rounded to nearest, by one Newton step on the instructions' estimates (both
+// equal sqrtf and 1 / x for every float32 from 1 to 4; the general forms, which also serve the ends
+// of the range, cost a step 3 %).  A root of less than 2^-126 is zero here, of infinity NaN.
+__device__ __forceinline__ float root(float x) {
+  const float y = __builtin_amdgcn_rsqf(x), s = x * y;
+  const float r = fmaf(fmaf(-s, s, x), 0.5f * y, s);
+  return x < 0x1p-126f ? 0.0f : r;
+}
+__device__ __forceinline__ float reciprocal(float x) {        // 2^-110 .. 2^126
+  const float y = __builtin_amdgcn_rcpf(x);
+  return fmaf(fmaf(-x, y, 1.0f), y, y);
 }
 
 __device__ __forceinline__ unsigned max3(unsigned a, unsigned b, unsigned c) {
@@ -245,23 +261,22 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8<MASTER> a) {
         }
     }
   }
-  float nm[kVec], nr[kVec];
+  float nm[kVec], nr[kVec], sq[kVec];
   // Magnitudes are compared as integers: the order is the same, and what is not finite comes out on
   // top.
   unsigned um = 0, ur = 0;
-  const float b1s = a.h.b1 * sm;
 #pragma unroll
   for (int j = 0; j < kVec; j += 2) {
+#pragma clang fp contract(off)
     const auto m2 = j ? __builtin_amdgcn_cvt_pk_f32_fp8(vm, true) : __builtin_amdgcn_cvt_pk_f32_fp8(vm, false);
     const auto r2 = j ? __builtin_amdgcn_cvt_pk_f32_fp8(vr, true) : __builtin_amdgcn_cvt_pk_f32_fp8(vr, false);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const float gr = vg.get(j + e) * c.gscale;
       const float rr = r2[e] * sr;
-      nm[j + e] = fmaf(m2[e], b1s, a.h.omb1 * gr);
-      // v_sqrt_f32 and v_rcp_f32 below: 1.5 * 2^-24 of the value each, a tenth of the exact forms'
-      // instructions; a second moment under 2^-126 counts as zero
-      nr[j + e] = __builtin_amdgcn_sqrtf(fmaf(a.h.b2 * rr, rr, a.h.omb2 * gr * gr));
+      nm[j + e] = m2[e] * sm * a.h.b1 + a.h.omb1 * gr;
+      sq[j + e] = rr * rr * a.h.b2 + gr * gr * a.h.omb2;
+      nr[j + e] = root(sq[j + e]);
     }
     um = max3(um, __float_as_uint(nm[j]) & 0x7FFFFFFFu, __float_as_uint(nm[j + 1]) & 0x7FFFFFFFu);
     ur = max3(ur, __float_as_uint(nr[j]), __float_as_uint(nr[j + 1]));
@@ -275,6 +290,7 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8<MASTER> a) {
     um = ur = 0;
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
+      if (sq[j] == INFINITY) nr[j] = INFINITY;         // a step of zero
       const unsigned mb = __float_as_uint(nm[j]) & 0x7FFFFFFFu, rb = __float_as_uint(nr[j]);
       if (mb >= kInf || rb >= kInf) bad |= 1u << j;
       if (mb < kInf && mb > um) um = mb;
@@ -287,8 +303,8 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8<MASTER> a) {
   float tm = __uint_as_float(um);
   const float tr = __uint_as_float(ur);
   if (tm < 0x1p-110f) tm = 0.0f;        // 448 / tm would overflow: such a block is held as zeros
-  const float im = tm > 0.0f ? 448.0f * __builtin_amdgcn_rcpf(tm) : 0.0f;
-  const float ir = tr > 0.0f ? 448.0f * __builtin_amdgcn_rcpf(tr) : 0.0f;
+  const float im = tm > 0.0f ? 448.0f * reciprocal(tm) : 0.0f;
+  const float ir = tr > 0.0f ? 448.0f * reciprocal(tr) : 0.0f;
   const unsigned bkey = mix32(key + (unsigned)(block0 + i / kBlock) * 0xC2B2AE35u);
   unsigned om = 0, orr = 0;
   auto value = [&](auto J) {

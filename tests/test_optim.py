@@ -465,6 +465,63 @@ def test_non_finite_gradients_stay_in_their_place():
             assert torch.isfinite(d8[key][0].float()[keep]).all() and d8[key][0].float()[300].isnan()
 
 
+def states_in_float32(m, r, ms, rs, g, factor, seed, step, tensor, hyper):
+    """Codes and scales after a step, every operation rounded to float32 by itself (numpy)."""
+    f = np.float32
+    b1, b2 = hyper["betas"]
+    n = g.size
+    at = np.arange(n) // BLOCK
+    g = g * f(factor)
+    m = m * ms[at] * f(b1) + g * f(1 - b1)
+    r = r * rs[at]
+    r = np.sqrt(r * r * f(b2) + g * g * f(1 - b2))
+    h = words(seed, step, tensor, n)
+    out = []
+    for x, bits in ((m, h & np.uint32(0xFFFF)), (r, h >> np.uint32(16))):
+        top = np.maximum.reduceat(np.abs(x), np.arange(0, n, BLOCK))
+        y = np.minimum(np.abs(x) * (f(448) * (f(1) / top))[at], f(448)).astype(np.float64)
+        lower, grid = around(y)
+        code = np.minimum(np.floor(y / grid + (bits + 0.5) / 65536) * grid, 448.0)
+        if x is r:
+            code = np.where((x > 0) & (code == 0), 2.0 ** -9, code)
+        out += [(code * np.sign(x)).astype(f), top * (f(1) / f(448))]
+    return out
+
+
+@gpu
+def test_states_bit_for_bit():
+    """Codes and scales are those of the formula in float32, a step after the other."""
+    n, seed, factor = 300 * BLOCK + 77, 41, 0.3
+    d = make8([5, n], torch.float32, torch.float32, False)
+    stats = torch.tensor([1.0, factor, 0.0, 0.0], device="cuda")
+
+    def host():
+        return [d[k][1].float().cpu().numpy() for k in ("m", "r", "ms", "rs")]
+
+    for t in range(7, 11):
+        want = states_in_float32(*host(), d["grads"][1].cpu().numpy(), factor, seed, t, 1, HYPER)
+        step8(d, t, seed, grad_stats=stats, **HYPER)
+        got = host()
+        for g, w in zip(got, (want[0], want[2], want[1], want[3])):
+            assert np.array_equal(g, w), t
+        d["grads"][1].mul_(-0.7)
+
+
+@gpu
+def test_squares_past_the_largest_float():
+    """A finite gradient whose square is not: its weight does not move, its neighbours do not notice."""
+    p = torch.ones(512, device="cuda")
+    g = torch.full((512,), 1e-3, device="cuda")
+    g[100] = 1e20
+    st = optim.state_8bit(p)
+    optim.adamw_step_8bit([p], [g], [st[0]], [st[1]], [st[2]], [st[3]], 1, lr=1e-2, weight_decay=0.0)
+    assert float(p[100]) == 1.0
+    rest = torch.arange(512, device="cuda") != 100
+    # m / (1 - b1) over sqrt(v / (1 - b2)) + eps is 1 - 1e-5; a few roundings of 2^-24
+    assert ((1 - p[rest]) - 1e-2 * (1 - 1e-5)).abs().max() <= 16 * U
+    assert torch.isfinite(st[0].float()[rest]).all() and torch.isfinite(st[2]).all()
+
+
 @gpu
 def test_tiny_gradients_without_eps():
     """Second moments below float32's normal range in 8 bits: nothing becomes infinite, and a step
