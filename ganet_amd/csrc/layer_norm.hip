@@ -7,7 +7,8 @@
 // The variance is formed from (x - mean), a second pass over the values: sums of squares would lose
 // it where the mean is large.  Everything between the loads and the one rounding of each output is
 // float32.  dw and db: every workgroup keeps sums of its own and leaves them in the workspace, a
-// second launch adds them in a fixed order (no atomics: the same inputs give the same bits).
+// second launch adds them in a fixed order; few positions are added in the first (no atomics: the same
+// inputs give the same bits).
 #include <math.h>
 
 #include "vec_device.h"
@@ -26,6 +27,9 @@ struct Args {
   void *y;                          // y, or grad_x (may be null in the backward)
   float *mean, *rstd;               // written (forward, may be null) or read
   float *partial;                   // [workgroups][2][C] or null
+  void *dw, *db;                    // grad_weight and grad_bias, where the launch writes them itself
+  unsigned main;                    // workgroups before those that do ...
+  int strip;                        // ... and the vectors of columns that each of those takes (rows)
   long long outer, inner, xs, ys, gs;
   int C, wdtype;
   float eps, inv_c, c;              // 1 / C and C
@@ -73,6 +77,21 @@ __device__ __forceinline__ void load_weights(const void *w, int dtype, int c, in
   else
     load_some<f16_t, N>((const f16_t *)w + c, C - c, out);
 }
+
+__device__ __forceinline__ void store_weight(void *w, int dtype, int c, float v) {
+  if (!w) return;
+  if (dtype == GANET_F32)
+    store1((float *)w + c, v);
+  else if (dtype == GANET_BF16)
+    store1((bf16_t *)w + c, v);
+  else
+    store1((f16_t *)w + c, v);
+}
+
+// Where a backward leaves its sums over positions: nowhere; each workgroup's in the workspace, for a
+// second launch; or, for few values, by workgroups of their own in the same launch, which read x and
+// grad_y again (from the caches) and need no sums over channels.
+enum Sums { kNoSums, kPartial, kApart };
 
 // Adds a value over the lanes that are LANES apart (the row groups of a wavefront).
 template <int LANES>
@@ -283,8 +302,65 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_rows_fwd(Args a)
 // before it works on this one.  Few, large workgroups: each leaves [2][C] floats to be added.
 constexpr int kBwdThreads = 1024;
 
-template <typename T, int LANES, int NV, bool SUMS>
+// kApart: the sums of STRIP vectors of columns.  Groups of STRIP lanes take the rows, four at once.
+template <typename T, int STRIP>
+__device__ __forceinline__ void strip_sums(const Args &a, int strip) {
+  constexpr int N = kN<T>, GROUPS = kBwdThreads / STRIP, U = 4;
+  __shared__ float part[2][kBwdThreads / 64][STRIP * N];
+  const int l = threadIdx.x & (STRIP - 1), c = (strip * STRIP + l) * N;
+  float s[2][N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) s[0][k] = s[1][k] = 0.0f;
+  for (int row = (int)threadIdx.x / STRIP; row < (int)a.outer; row += GROUPS * U) {
+    Vec<T, N> x[U], g[U];
+    float mu[U], rs[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = row + u * GROUPS;
+      const bool in = r < (int)a.outer;
+      mu[u] = in ? a.mean[r] : 0.0f;
+      rs[u] = in ? a.rstd[r] : 0.0f;
+      if (in && c < a.C) {
+        x[u].load_kept((const T *)a.x + r * a.xs + c, a.C - c);
+        g[u].load_kept((const T *)a.g + r * a.gs + c, a.C - c);
+      } else {
+        x[u].zero();
+        g[u].zero();
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const float dy = g[u].get(k);
+        s[0][k] += dy * ((x[u].get(k) - mu[u]) * rs[u]);
+        s[1][k] += dy;
+      }
+  }
+#pragma unroll
+  for (int which = 0; which < 2; ++which)
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const float v = across_groups<STRIP>(s[which][k]);
+      if ((threadIdx.x & 63) < STRIP) part[which][threadIdx.x >> 6][l * N + k] = v;
+    }
+  ganet_vec::lds_barrier();
+  const int at = threadIdx.x % (STRIP * N), which = threadIdx.x / (STRIP * N);
+  if (which > 1 || strip * STRIP * N + at >= a.C) return;
+  float v = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kBwdThreads / 64; ++i) v += part[which][i][at];
+  store_weight(which ? a.db : a.dw, a.wdtype, strip * STRIP * N + at, v);
+}
+
+template <typename T, int LANES, int NV, Sums HOW>
 __global__ __launch_bounds__(kBwdThreads) void ln_rows_bwd(Args a) {
+  if constexpr (HOW == kApart)
+    if (blockIdx.x >= a.main) {
+      const int strip = (int)(blockIdx.x - a.main);
+      return a.strip == 4 ? strip_sums<T, 4>(a, strip) : strip_sums<T, 8>(a, strip);
+    }
+  constexpr bool SUMS = HOW == kPartial;
   constexpr int N = kN<T>;
   constexpr int ROWS = kBwdThreads / LANES;
   constexpr int W = LANES > 64 ? LANES / 64 : 1;
@@ -331,7 +407,7 @@ __global__ __launch_bounds__(kBwdThreads) void ln_rows_bwd(Args a) {
     }
   };
   constexpr bool AHEAD = !LDS_W;                     // 16 columns fill the 128 registers by themselves
-  const long long step = (long long)gridDim.x * ROWS;
+  const long long step = (long long)a.main * ROWS;
   const long long first = (long long)blockIdx.x * ROWS;
   if (AHEAD) fetch(first + group);
   int turn = 0;
@@ -506,11 +582,11 @@ __device__ __forceinline__ void slots_sum(float (&s)[M], float (*part)[64][M / 4
 // tiles share (planes start at any address) meet in one L2.
 struct Share {
   unsigned end, step, at;                            // fewer than 2^31 tiles (with_plane_shape)
-  __device__ __forceinline__ explicit Share(unsigned tiles) {
+  __device__ __forceinline__ Share(unsigned tiles, unsigned workgroups) {
     const unsigned per = (tiles + 7) / 8, from = (blockIdx.x & 7) * per;
     at = from + (blockIdx.x >> 3);
     end = from + per < tiles ? from + per : tiles;
-    step = (gridDim.x + 7 - (blockIdx.x & 7)) >> 3;
+    step = (workgroups + 7 - (blockIdx.x & 7)) >> 3;
   }
 };
 
@@ -532,7 +608,7 @@ __global__ __launch_bounds__(64 * WAVES) void ln_planes_fwd(Args a, int tiles, i
   __shared__ __align__(16) float part[2][WAVES][64][N / 4];
   __shared__ float weights[2][P::SLOTS * NC];
   int own;
-  const Share share((unsigned)a.outer * (unsigned)tiles);
+  const Share share((unsigned)a.outer * (unsigned)tiles, gridDim.x);
   if (share.at >= share.end) return;
   const unsigned image = share.at / (unsigned)tiles;
   const long long img = image;
@@ -601,9 +677,56 @@ __global__ __launch_bounds__(64 * WAVES) void ln_planes_fwd(Args a, int tiles, i
 
 // Backward: 16 wavefronts a CU (128 registers), however they are grouped.  Loading the next tile into
 // registers meanwhile was measured and gains nothing (bf16 32x256x40x100 47.4 and 47.6 us).
-template <typename T, int VB, int NC, int WAVES, bool SUMS>
+// kApart: the sums of one channel, a vector of each image's plane after the other.
+template <typename T, int N, int THREADS>
+__device__ __forceinline__ void channel_sums(const Args &a, int c) {
+  __shared__ float part[2][THREADS / 64];
+  constexpr int U = 2;
+  const int vecs = (int)((a.inner + N - 1) / N), all = (int)a.outer * vecs;
+  float dw = 0.0f, db = 0.0f;
+  for (int i = threadIdx.x; i < all; i += THREADS * U) {
+    Vec<T, N> x[U], g[U];
+    Vec<float, N> mean[U], rstd[U];
+    int own[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = i + u * THREADS, image = (at < all ? at : i) / vecs;
+      const long long pos = plane_position<N>((long long)((at < all ? at : i) - image * vecs) * N, a.inner, own[u]);
+      if (at >= all) own[u] = N;
+      x[u].load_kept((const T *)a.x + image * a.xs + c * a.inner + pos);
+      g[u].load_kept((const T *)a.g + image * a.gs + c * a.inner + pos);
+      mean[u].load_kept(a.mean + image * a.inner + pos);
+      rstd[u].load_kept(a.rstd + image * a.inner + pos);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float dy = j >= own[u] ? g[u].get(j) : 0.0f;
+        dw += j >= own[u] ? dy * ((x[u].get(j) - mean[u].v[j]) * rstd[u].v[j]) : 0.0f;
+        db += dy;
+      }
+  }
+  dw = group_sum<64>(dw);
+  db = group_sum<64>(db);
+  if ((threadIdx.x & 63) == 0) {
+    part[0][threadIdx.x >> 6] = dw;
+    part[1][threadIdx.x >> 6] = db;
+  }
+  ganet_vec::lds_barrier();
+  if (threadIdx.x > 1) return;
+  float v = 0.0f;
+#pragma unroll
+  for (int i = 0; i < THREADS / 64; ++i) v += part[threadIdx.x][i];
+  store_weight(threadIdx.x ? a.db : a.dw, a.wdtype, c, v);
+}
+
+template <typename T, int VB, int NC, int WAVES, Sums HOW>
 __global__ __launch_bounds__(64 * WAVES, 4) void ln_planes_bwd(Args a, int tiles, int nc) {
   typedef Plane<T, VB, NC, WAVES> P;
+  if constexpr (HOW == kApart)
+    if (blockIdx.x >= a.main) return channel_sums<T, P::N, P::THREADS>(a, (int)(blockIdx.x - a.main));
+  constexpr bool SUMS = HOW == kPartial;
   constexpr int N = P::N;
   __shared__ __align__(16) float part[2][WAVES][64][N / 2];
   __shared__ float weights[P::SLOTS * NC];
@@ -614,7 +737,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void ln_planes_bwd(Args a, int tiles
 #pragma unroll
   for (int k = 0; k < NC; ++k) dw[k] = db[k] = 0.0f;
   int turn = 0;
-  const Share share((unsigned)a.outer * (unsigned)tiles);
+  const Share share((unsigned)a.outer * (unsigned)tiles, a.main);
   for (unsigned i = share.at; i < share.end; i += share.step, turn ^= 1) {
     int own;
     const unsigned image = i / (unsigned)tiles;
@@ -729,12 +852,7 @@ __global__ __launch_bounds__(kFinish) void ln_finish(const float *partial, int n
   s = 0.0f;
 #pragma unroll
   for (int i = 0; i < kFinish / 64; ++i) s += part[i][col];
-  if (dtype == GANET_F32)
-    store1((float *)out + c, s);
-  else if (dtype == GANET_BF16)
-    store1((bf16_t *)out + c, s);
-  else
-    store1((f16_t *)out + c, s);
+  store_weight(out, dtype, c, s);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -860,6 +978,14 @@ int with_plane_shape(const ganet_layer_norm_params *p, F &&f) {
   return f(std::integral_constant<int, kAny>(), std::integral_constant<int, 1>(), std::integral_constant<int, 1>());
 }
 
+// Up to where the sums over positions go to workgroups of the same launch.  One launch less is 3 us
+// less for a call that the host bounds (250 rows of 256: 9.5 and 7.2 us), and wide rows leave no
+// partial sums as large as themselves (250 x 16384 bf16 35 and 13 us); what it costs is one workgroup's
+// way through all positions of its columns (1024 rows of 4096 bf16 17 and 11 us, 2048 rows 20 and 29;
+// 16000 positions of 256 channels 11.4 and 9.5 us, 32000 14.5 and 19.7) and reading the values twice
+// (4 x 40 x 100 positions of 512 channels float32 32 and 34 us, of 256 20.2 and 19.1).
+constexpr long long kApartRows = 1024, kApartPositions = 1 << 14, kApartValues = 1 << 22;
+
 // Workgroups of the backward, each with sums of its own: what is on the chip at once.
 int backward_blocks(const ganet_layer_norm_params *p) {
   int blocks = 0;
@@ -885,6 +1011,21 @@ int backward_blocks(const ganet_layer_norm_params *p) {
     });
   });
   return blocks;
+}
+
+// Whether the sums go apart, into workgroups of the same launch.
+bool sums_apart(const ganet_layer_norm_params *p) {
+  const long long positions = p->outer * p->inner;
+  if (p->inner == 1) return positions <= kApartRows;
+  if (positions > kApartPositions || positions * p->C > kApartValues) return false;
+  bool apart = false;
+  with_type(p->dtype, [&](auto t) {
+    return with_plane_shape<true, decltype(t)>(p, [&](auto vb, auto, auto) {
+      apart = vb.value != kAny;
+      return GANET_OK;
+    });
+  });
+  return apart;
 }
 
 template <typename T>
@@ -930,24 +1071,30 @@ int launch_forward(const ganet_layer_norm_params *p, const Args &a, hipStream_t 
   });
 }
 
-template <typename T, bool SUMS>
-int launch_backward(const ganet_layer_norm_params *p, const Args &a, int blocks, hipStream_t s) {
+template <typename T, Sums HOW>
+int launch_backward(const ganet_layer_norm_params *p, Args a, int blocks, hipStream_t s) {
+  a.main = (unsigned)blocks;
   if (p->inner == 1)
     return with_row_shape<true, T>(p->C, [&](auto lanes, auto nv) {
       constexpr int L = lanes.value, NV = nv.value;
       constexpr int groups = L < 64 ? kBwdThreads / 64 : kBwdThreads / L;
-      constexpr size_t room = SUMS ? (size_t)groups * L * NV * kN<T> * sizeof(float) : 0;
-      ln_rows_bwd<T, L, NV, SUMS><<<dim3(blocks), dim3(kBwdThreads), room, s>>>(a);
+      constexpr size_t room = HOW == kPartial ? (size_t)groups * L * NV * kN<T> * sizeof(float) : 0;
+      // 64 or 128 bytes of a row: the narrow ones where the others are too few for the chip (777 rows of
+      // 1001 f16 7.7 and 8.9 us; 777 of 4096 12.1 and 9.6)
+      const int vecs = (p->C + kN<T> - 1) / kN<T>;
+      a.strip = vecs > 31 * 8 ? 8 : 4;
+      const int more = HOW == kApart ? (vecs + a.strip - 1) / a.strip : 0;
+      ln_rows_bwd<T, L, NV, HOW><<<dim3(blocks + more), dim3(kBwdThreads), room, s>>>(a);
       return ganet_check_launch();
     });
   return with_plane_shape<true, T>(p, [&](auto vb, auto nc, auto waves) {
     if constexpr (vb.value == kAny) {
       ln_planes_any_bwd<T>
-          <<<dim3(blocks), dim3(kThreads), SUMS ? (size_t)2 * p->C * sizeof(float) : 0, s>>>(a);
+          <<<dim3(blocks), dim3(kThreads), HOW == kPartial ? (size_t)2 * p->C * sizeof(float) : 0, s>>>(a);
     } else {
       typedef Plane<T, vb.value, nc.value, waves.value> P;
-      ln_planes_bwd<T, vb.value, nc.value, waves.value, SUMS>
-          <<<dim3(blocks), dim3(P::THREADS), 0, s>>>(a, (int)tiles_of(p, P::TILE), (p->C + P::SLOTS - 1) / P::SLOTS);
+      ln_planes_bwd<T, vb.value, nc.value, waves.value, HOW><<<dim3(blocks + (HOW == kApart ? p->C : 0)), dim3(P::THREADS), 0, s>>>(
+          a, (int)tiles_of(p, P::TILE), (p->C + P::SLOTS - 1) / P::SLOTS);
     }
     return ganet_check_launch();
   });
@@ -974,7 +1121,8 @@ extern "C" int ganet_layer_norm_forward(const void *x, const void *weight, const
 
 extern "C" size_t ganet_layer_norm_backward_workspace_bytes(const ganet_layer_norm_params *p) {
   if (params_ok(p, true) != GANET_OK) return 0;
-  return ganet_align_up((size_t)(backward_blocks(p) + 1) * 2 * p->C * sizeof(float), 256);
+  const size_t blocks = sums_apart(p) ? 0 : (size_t)backward_blocks(p);
+  return ganet_align_up((blocks + 1) * 2 * p->C * sizeof(float), 256);
 }
 
 extern "C" int ganet_layer_norm_backward(const void *x, const void *weight, const void *grad_y, const float *mean,
@@ -1000,11 +1148,17 @@ extern "C" int ganet_layer_norm_backward(const void *x, const void *weight, cons
     a.rstd = (float *)rstd;
     a.partial = sums ? (float *)workspace : nullptr;
     blocks = backward_blocks(p);
+    const bool apart = sums && sums_apart(p);
+    if (apart) {
+      a.dw = grad_weight;
+      a.db = grad_bias;
+    }
     const int rc = with_type(p->dtype, [&](auto t) {
       typedef decltype(t) T;
-      return sums ? launch_backward<T, true>(p, a, blocks, s) : launch_backward<T, false>(p, a, blocks, s);
+      if (apart) return launch_backward<T, kApart>(p, a, grad_x ? blocks : 0, s);
+      return sums ? launch_backward<T, kPartial>(p, a, blocks, s) : launch_backward<T, kNoSums>(p, a, blocks, s);
     });
-    if (rc != GANET_OK) return rc;
+    if (rc != GANET_OK || apart) return rc;
   }
   if (!sums) return GANET_OK;
   ln_finish<<<dim3((p->C + kFinishCols - 1) / kFinishCols, 2), dim3(kFinish), 0, s>>>((const float *)workspace, blocks, p->C, grad_weight,

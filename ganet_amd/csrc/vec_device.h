@@ -64,9 +64,10 @@ struct Vec {
     __builtin_nontemporal_store((Mem)v, (GANET_GLOBAL Mem *)(p));
   }
   // ... or is read by what follows, or shares its lines with a neighbour
+  __device__ __forceinline__ void load_kept(const T *p) { v = *(const GANET_GLOBAL Mem *)(p); }
   __device__ __forceinline__ void load_kept(const T *p, long long k) {
     if (k >= N)
-      v = *(const GANET_GLOBAL Mem *)(p);
+      load_kept(p);
     else
       load(p, k);
   }

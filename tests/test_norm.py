@@ -201,6 +201,24 @@ def test_maps(shape, channels_last, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("c", [1, 7, 64, 100, 257, 511, 1001, 2048, 2049, 4096, 5000, 8192, 16384])
+def test_more_rows(c):
+    """Every width with enough rows for sums in the workspace."""
+    for n in (1024, 1025):
+        both(*make((n, c), -1, torch.float32, torch.float32), -1)
+        both(*make((n, c), -1, torch.bfloat16, torch.float32), -1)
+
+
+@gpu
+@pytest.mark.parametrize("c", [1, 16, 33, 64, 129, 256, 257, 512, 600, 1024])
+def test_more_positions(c):
+    for shape in ((2, c, 97, 101), (8, c, 32, 64), (3, c, 9, 13)):      # past, at and below the limit
+        if c * shape[0] * shape[2] * shape[3] < 6e6:
+            both(*make(shape, 1, torch.float32, torch.float32), 1)
+            both(*make(shape, 1, torch.float16, torch.float32), 1)
+
+
+@gpu
 @pytest.mark.parametrize("layout", ["rows", "nchw"])
 def test_many_positions(layout):
     """More rows and tiles than the backward has workgroups."""
