@@ -101,26 +101,39 @@ PyObject *step(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   }
 }
 
+// Addresses, sizes and types of a list of gradients that are all contiguous and on one GPU.
+struct Grads {
+  std::vector<const void *> address;
+  std::vector<std::int64_t> size;
+  std::vector<std::int32_t> type;
+  int gpu = -1;
+};
+bool read(PyObject *list, Grads &g) {
+  const Py_ssize_t n = length(list);
+  if (n < 1) return false;
+  g.address.resize(n);
+  g.size.resize(n);
+  g.type.resize(n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const at::Tensor *t = item(list, i);
+    if (!t || !t->is_cuda() || t->layout() != at::kStrided || !t->is_contiguous()) return false;
+    g.type[i] = code(t->scalar_type());
+    if (i == 0) g.gpu = static_cast<int>(t->get_device());
+    if (g.type[i] == kOther || g.type[i] == kE4M3 || t->get_device() != g.gpu) return false;
+    g.address[i] = t->data_ptr();
+    g.size[i] = t->numel();
+  }
+  return true;
+}
+
 // grads(list) -> (gpu, addresses, sizes, types) or None
 PyObject *grads(PyObject *, PyObject *list) {
   try {
-    const Py_ssize_t n = length(list);
-    if (n < 1) Py_RETURN_NONE;
-    std::vector<std::uint64_t> address(n);
-    std::vector<std::int64_t> size(n);
-    std::vector<std::int32_t> type(n);
-    int gpu = -1;
-    for (Py_ssize_t i = 0; i < n; ++i) {
-      const at::Tensor *t = item(list, i);
-      if (!t || !t->is_cuda() || t->layout() != at::kStrided || !t->is_contiguous()) Py_RETURN_NONE;
-      type[i] = code(t->scalar_type());
-      if (i == 0) gpu = static_cast<int>(t->get_device());
-      if (type[i] == kOther || type[i] == kE4M3 || t->get_device() != gpu) Py_RETURN_NONE;
-      address[i] = reinterpret_cast<std::uint64_t>(t->data_ptr());
-      size[i] = t->numel();
-    }
-    return Py_BuildValue("iNNN", gpu, bytes(address.data(), n * 8), bytes(size.data(), n * 8),
-                         bytes(type.data(), n * 4));
+    Grads g;
+    if (!read(list, g)) Py_RETURN_NONE;
+    const size_t n = g.size.size();
+    return Py_BuildValue("iNNN", g.gpu, bytes(g.address.data(), n * 8), bytes(g.size.data(), n * 8),
+                         bytes(g.type.data(), n * 4));
   } catch (const std::exception &) {
     PyErr_Clear();
     Py_RETURN_NONE;
@@ -209,6 +222,37 @@ void *data(const at::Tensor *t) { return t ? t->data_ptr() : nullptr; }
 PyObject *wrapped(const at::Tensor &t) {
   if (t.defined()) return THPVariable_Wrap(t);
   Py_RETURN_NONE;
+}
+
+// grad_norm(workspace query, entry point, gradients, max_norm, inv_scale, gpu, stream) -> the float32 [4]
+// tensor, the entry point's status where it is not 0, or None
+PyObject *grad_norm(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  if (nargs != 7) {
+    PyErr_SetString(PyExc_TypeError, "grad_norm() takes 7 arguments");
+    return nullptr;
+  }
+  auto query = reinterpret_cast<decltype(&ganet_grad_norm_workspace_bytes)>(address(args[0]));
+  auto entry = reinterpret_cast<decltype(&ganet_grad_norm)>(address(args[1]));
+  const double max_norm = PyFloat_AsDouble(args[3]), inv_scale = PyFloat_AsDouble(args[4]);
+  const long gpu = PyLong_AsLong(args[5]);
+  void *stream = address(args[6]);
+  if (PyErr_Occurred()) return nullptr;
+  try {
+    Grads g;
+    if (!query || !entry || !read(args[2], g) || g.gpu != gpu || g.size.size() > 1 << 20) Py_RETURN_NONE;
+    const int n = static_cast<int>(g.size.size());
+    const auto plain = item(args[2], 0)->options().requires_grad(false);
+    const size_t bytes = query(g.size.data(), n);
+    const at::Tensor out = at::empty({4}, plain.dtype(at::kFloat));
+    const at::Tensor ws = at::empty({static_cast<std::int64_t>(std::max<size_t>(bytes, 256))}, plain.dtype(at::kByte));
+    const int rc = entry(g.address.data(), g.size.data(), g.type.data(), n, max_norm, inv_scale, out.data_ptr<float>(),
+                         ws.data_ptr(), bytes, stream);
+    if (rc) return PyLong_FromLong(rc);
+    return wrapped(out);
+  } catch (const std::exception &e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
 }
 
 // layer_norm_forward(entry point, x, weight, bias, eps, channel_dim, stats, stream) ->
@@ -302,6 +346,8 @@ PyMethodDef methods[] = {
     {"step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(step)), METH_FASTCALL,
      "The table of an AdamW step over plain lists of tensors, or None."},
     {"grads", grads, METH_O, "Addresses, sizes and types of a plain list of gradients, or None."},
+    {"grad_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(grad_norm)), METH_FASTCALL,
+     "The norm of a plain list of gradients, or None."},
     {"written", written, METH_O, "Marks a list of tensors as changed in place."},
     {"layer_norm_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(layer_norm_forward)),
      METH_FASTCALL, "Layer norm's forward on tensors in the kernels' order, or None."},

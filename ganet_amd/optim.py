@@ -228,14 +228,24 @@ def grad_norm(grads, max_norm=None, inv_scale=1.0, out=None):
     adamw_step_8bit take the tensor as grad_stats.  Gradients of several dtypes may be mixed."""
     grads = list(grads)
     n = len(grads)
+    max_norm = math.inf if max_norm is None else float(max_norm)
+    if not max_norm >= 0 or not math.isfinite(inv_scale):
+        raise ValueError("grad_norm: max_norm %r, inv_scale %r" % (max_norm, inv_scale))
+    if out is None and n and torch.is_tensor(grads[0]):
+        index = grads[0].get_device()
+        if index >= 0 and torch.cuda.current_device() == index:
+            stats = _lib.host().grad_norm(_lib.address("ganet_grad_norm_workspace_bytes"),
+                                          _lib.address("ganet_grad_norm"), grads, max_norm,
+                                          inv_scale, index, _lib.raw_stream(index))
+            if torch.is_tensor(stats):
+                return stats
+            if stats is not None:
+                _lib.check(stats, "ganet_grad_norm")
     found = _lib.host().grads(grads)
     if found is not None:
         index, ptrs, numel, dtypes = found
     else:
         index, ptrs, numel, dtypes, grads = _read_grads(grads, out)
-    max_norm = math.inf if max_norm is None else float(max_norm)
-    if not max_norm >= 0 or not math.isfinite(inv_scale):
-        raise ValueError("grad_norm: max_norm %r, inv_scale %r" % (max_norm, inv_scale))
     L = _lib.lib()
     if out is None:
         out = torch.empty(4, dtype=torch.float32, device=grads[0].device)
