@@ -18,6 +18,8 @@
 
 namespace {
 
+static_assert(sizeof(ganet_step_tensor) == 64, "eight words a tensor");
+
 enum { kFloat32 = 0, kBFloat16 = 1, kFloat16 = 2, kE4M3 = 3, kOther = -1 };
 
 int code(at::ScalarType t) {
@@ -44,8 +46,68 @@ PyObject *bytes(const void *p, size_t n) {
   return PyBytes_FromStringAndSize(static_cast<const char *>(p), static_cast<Py_ssize_t>(n));
 }
 
+// The table of an AdamW step over the lists params, grads, avgs, seconds, avg_scales, second_scales and
+// masters (the last three may be None).
+struct Step {
+  int gpu, param, grad, state;
+  std::vector<std::uint64_t> rows;                   // of ganet_step_tensor
+};
+bool read(PyObject *const *lists, std::int64_t block, Step &s) {
+  const Py_ssize_t n = length(lists[0]);
+  if (n < 1) return false;
+  s.rows.assign(static_cast<size_t>(n) * 8, 0);
+  std::vector<std::uint64_t> written;
+  int types[7] = {kOther, kOther, kOther, kOther, kOther, kOther, kOther};
+  s.gpu = -1;
+  for (int k = 0; k < 7; ++k) {
+    if (lists[k] == Py_None) {
+      if (k < 4) return false;
+      continue;
+    }
+    if (length(lists[k]) != n) return false;
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      const at::Tensor *t = item(lists[k], i), *p = item(lists[0], i);
+      if (!t || !p || !t->is_cuda() || t->layout() != at::kStrided || !t->is_contiguous()) return false;
+      const int type = code(t->scalar_type()), at = static_cast<int>(t->get_device());
+      if (i == 0) types[k] = type;
+      if (i == 0 && k == 0) s.gpu = at;
+      if (type == kOther || type != types[k] || at != s.gpu) return false;
+      const std::int64_t values = p->numel();
+      if (k == 4 || k == 5) {
+        if (t->numel() != (values + block - 1) / block) return false;
+      } else if (!t->sizes().equals(p->sizes())) {
+        return false;
+      }
+      const auto address = reinterpret_cast<std::uint64_t>(t->data_ptr());
+      s.rows[i * 8 + k] = address;
+      if (k == 0) s.rows[i * 8 + 7] = static_cast<std::uint64_t>(values);
+      if (k != 1 && values) written.push_back(address);
+    }
+  }
+  std::sort(written.begin(), written.end());
+  if (std::adjacent_find(written.begin(), written.end()) != written.end()) return false;
+  s.param = types[0];
+  s.grad = types[1];
+  s.state = types[2];
+  if (types[2] != types[3] || (types[2] != kFloat32 && types[2] != kE4M3) || types[0] == kE4M3 || types[1] == kE4M3)
+    return false;
+  if (lists[6] != Py_None && (types[6] != kFloat32 || types[0] == kFloat32)) return false;
+  for (int k = 4; k < 6; ++k)
+    if ((lists[k] == Py_None) != (types[2] != kE4M3) || (lists[k] != Py_None && types[k] != kFloat32)) return false;
+  return true;
+}
+
+// The tensors' values have changed: autograd refuses a backward pass that saved the old ones, as it does
+// after torch's own in-place operations.
+void mark(PyObject *list) {
+  for (Py_ssize_t i = 0, n = length(list); i < n; ++i) {
+    const at::Tensor *t = item(list, i);
+    if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();   // those have no versions
+  }
+}
+
 // step(params, grads, avgs, seconds, avg_scales, second_scales, masters, block) ->
-// (gpu, parameter type, gradient type, state type, rows of ganet_step_tensor) or None
+// (gpu, parameter type, gradient type, state bits, rows of ganet_step_tensor) or None
 PyObject *step(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   if (nargs != 8) {
     PyErr_SetString(PyExc_TypeError, "step() takes 8 arguments");
@@ -57,47 +119,73 @@ PyObject *step(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     return nullptr;
   }
   try {
-    const Py_ssize_t n = length(args[0]);
-    if (n < 1) Py_RETURN_NONE;
-    std::vector<std::uint64_t> rows(static_cast<size_t>(n) * 8, 0);
-    std::vector<std::uint64_t> written;
-    int types[7] = {kOther, kOther, kOther, kOther, kOther, kOther, kOther};
-    int gpu = -1;
-    for (int k = 0; k < 7; ++k) {
-      if (args[k] == Py_None) {
-        if (k < 4) Py_RETURN_NONE;
-        continue;
-      }
-      if (length(args[k]) != n) Py_RETURN_NONE;
-      for (Py_ssize_t i = 0; i < n; ++i) {
-        const at::Tensor *t = item(args[k], i), *p = item(args[0], i);
-        if (!t || !p || !t->is_cuda() || t->layout() != at::kStrided || !t->is_contiguous()) Py_RETURN_NONE;
-        const int type = code(t->scalar_type()), at = static_cast<int>(t->get_device());
-        if (i == 0) types[k] = type;
-        if (i == 0 && k == 0) gpu = at;
-        if (type == kOther || type != types[k] || at != gpu) Py_RETURN_NONE;
-        const std::int64_t values = p->numel();
-        if (k == 4 || k == 5) {
-          if (t->numel() != (values + block - 1) / block) Py_RETURN_NONE;
-        } else if (!t->sizes().equals(p->sizes())) {
-          Py_RETURN_NONE;
-        }
-        const auto address = reinterpret_cast<std::uint64_t>(t->data_ptr());
-        rows[i * 8 + k] = address;
-        if (k == 0) rows[i * 8 + 7] = static_cast<std::uint64_t>(values);
-        if (k != 1 && values) written.push_back(address);
-      }
-    }
-    std::sort(written.begin(), written.end());
-    if (std::adjacent_find(written.begin(), written.end()) != written.end()) Py_RETURN_NONE;
-    if (types[2] != types[3] || (args[6] != Py_None && types[6] != kFloat32)) Py_RETURN_NONE;
-    for (int k = 4; k < 6; ++k)
-      if ((args[k] == Py_None) != (types[2] != kE4M3) || (args[k] != Py_None && types[k] != kFloat32))
-        Py_RETURN_NONE;
-    return Py_BuildValue("iiiiN", gpu, types[0], types[1], types[2], bytes(rows.data(), rows.size() * 8));
+    Step s;
+    if (!read(args, block, s)) Py_RETURN_NONE;
+    return Py_BuildValue("iiiiN", s.gpu, s.param, s.grad, s.state == kE4M3 ? 8 : 32, bytes(s.rows.data(), s.rows.size() * 8));
   } catch (const std::exception &) {   // a tensor without storage: Python's own reading names it
     PyErr_Clear();
     Py_RETURN_NONE;
+  }
+}
+
+void *address(PyObject *o) { return PyLong_AsVoidPtr(o); }
+
+// adamw(entry point, the seven lists, block, state bits, step, lr, beta1, beta2, eps, weight_decay,
+// grad_stats, skip_nonfinite, seed, gpu, stream) -> the entry point's status, or None where nothing was done
+PyObject *adamw(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  if (nargs != 21) {
+    PyErr_SetString(PyExc_TypeError, "adamw() takes 21 arguments");
+    return nullptr;
+  }
+  auto entry = reinterpret_cast<decltype(&ganet_adamw_step)>(address(args[0]));
+  const long block = PyLong_AsLong(args[8]), bits = PyLong_AsLong(args[9]), gpu = PyLong_AsLong(args[19]);
+  ganet_adamw_params p = {};
+  p.step = PyLong_AsLongLong(args[10]);
+  p.lr = PyFloat_AsDouble(args[11]);
+  p.beta1 = PyFloat_AsDouble(args[12]);
+  p.beta2 = PyFloat_AsDouble(args[13]);
+  p.eps = PyFloat_AsDouble(args[14]);
+  p.weight_decay = PyFloat_AsDouble(args[15]);
+  p.skip_nonfinite = PyObject_IsTrue(args[17]);
+  p.seed = static_cast<std::uint32_t>(PyLong_AsUnsignedLongMask(args[18]));
+  void *stream = address(args[20]);
+  if (PyErr_Occurred()) return nullptr;
+  try {
+    Step s;
+    if (!entry || block < 1 || !read(args + 1, block, s) || s.gpu != gpu || bits != (s.state == kE4M3 ? 8 : 32) ||
+        s.rows.size() / 8 > INT32_MAX)
+      Py_RETURN_NONE;
+    if (args[16] != Py_None) {
+      const at::Tensor *t = THPVariable_Check(args[16]) ? &THPVariable_Unpack(args[16]) : nullptr;
+      if (!t || !t->is_cuda() || t->get_device() != s.gpu || t->scalar_type() != at::kFloat || t->numel() != 4 ||
+          !t->is_contiguous())
+        Py_RETURN_NONE;
+      p.grad_stats = t->data_ptr<float>();
+    }
+    p.param_dtype = s.param;
+    p.grad_dtype = s.grad;
+    p.state_bits = static_cast<std::int32_t>(bits);
+    const int rc = entry(reinterpret_cast<const ganet_step_tensor *>(s.rows.data()), static_cast<int>(s.rows.size() / 8),
+                         &p, stream);
+    if (rc == 0) {
+      mark(args[1]);
+      if (args[7] != Py_None) mark(args[7]);
+    }
+    return PyLong_FromLong(rc);
+  } catch (const std::exception &e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
+// written(list)
+PyObject *written(PyObject *, PyObject *list) {
+  try {
+    mark(list);
+    Py_RETURN_NONE;
+  } catch (const std::exception &e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
   }
 }
 
@@ -137,21 +225,6 @@ PyObject *grads(PyObject *, PyObject *list) {
   } catch (const std::exception &) {
     PyErr_Clear();
     Py_RETURN_NONE;
-  }
-}
-
-// written(list): the tensors' values have changed, so that autograd refuses a backward pass that saved
-// the old ones, as it does after torch's own in-place operations.
-PyObject *written(PyObject *, PyObject *list) {
-  try {
-    for (Py_ssize_t i = 0, n = length(list); i < n; ++i) {
-      const at::Tensor *t = item(list, i);
-      if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();   // those have no versions
-    }
-    Py_RETURN_NONE;
-  } catch (const std::exception &e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
   }
 }
 
@@ -217,7 +290,6 @@ ganet_layer_norm_params parameters(const Where &w, int type, int weight_type, fl
   p.eps = eps;
   return p;
 }
-void *address(PyObject *o) { return PyLong_AsVoidPtr(o); }
 void *data(const at::Tensor *t) { return t ? t->data_ptr() : nullptr; }
 PyObject *wrapped(const at::Tensor &t) {
   if (t.defined()) return THPVariable_Wrap(t);
@@ -345,6 +417,8 @@ PyObject *layer_norm_backward(PyObject *, PyObject *const *args, Py_ssize_t narg
 PyMethodDef methods[] = {
     {"step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(step)), METH_FASTCALL,
      "The table of an AdamW step over plain lists of tensors, or None."},
+    {"adamw", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw)), METH_FASTCALL,
+     "An AdamW step over plain lists of tensors, or None."},
     {"grads", grads, METH_O, "Addresses, sizes and types of a plain list of gradients, or None."},
     {"grad_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(grad_norm)), METH_FASTCALL,
      "The norm of a plain list of gradients, or None."},

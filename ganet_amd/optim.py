@@ -145,9 +145,19 @@ def _step(params, grads, avgs, seconds, avg_scales, second_scales, bits, step, l
           weight_decay, masters, grad_stats, skip_nonfinite, seed):
     n = len(params)
     lists = (params, grads, avgs, seconds, avg_scales, second_scales, masters)
+    if n and type(step) is int and not torch.is_tensor(lr) and torch.is_tensor(params[0]):
+        index = params[0].get_device()
+        if index >= 0 and torch.cuda.current_device() == index:
+            rc = _lib.host().adamw(_lib.address("ganet_adamw_step"), *lists, BLOCK, bits, step, lr,
+                                   betas[0], betas[1], eps, weight_decay, grad_stats,
+                                   skip_nonfinite, int(seed), index, _lib.raw_stream(index))
+            if rc is not None:
+                if rc:
+                    _lib.check(rc, "ganet_adamw_step")
+                return
+    # a step or lr on the device, another order of memory, another GPU, or something wrong
     found = _lib.host().step(*lists, BLOCK)
-    if (found is not None and max(found[1:3]) < 3 and found[3] == (0 if bits == 32 else 3)
-            and not (masters is not None and found[1] == 0)):
+    if found is not None and found[3] == bits:
         index, ptype, gtype, _, rows = found
     elif n or any(lists[1:]):
         if not n:
