@@ -361,50 +361,55 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        every = [(group, p) for group in self.param_groups for p in group["params"]
-                 if p.grad is not None]
+        every = [(group, p, p.grad) for group in self.param_groups for p in group["params"]]
+        every = [one for one in every if one[2] is not None]
         if not every:
             return loss
-        if any(p.grad.is_sparse for _, p in every):
+        grads = [g for _, _, g in every]
+        if any(g.is_sparse for g in grads):
             raise RuntimeError("AdamW: sparse gradients")
         if every[0][1].is_cuda and torch.cuda.is_current_stream_capturing():
             # the number of the step would be part of the graph, a new state its memory
             if not self.capturable:
                 raise RuntimeError("AdamW: a captured step needs capturable=True")
-            if any("step" not in self.state.get(p, ()) for _, p in every):
+            if any("step" not in self.state.get(p, ()) for _, p, _ in every):
                 raise RuntimeError("AdamW: make one step before the capture")
         if grad_stats is None and self.max_grad_norm is not None:
-            grad_stats = grad_norm([p.grad for _, p in every], self.max_grad_norm)
+            grad_stats = grad_norm(grads, self.max_grad_norm)
         self.grad_stats = grad_stats
-        fresh, counters, lists = {}, {}, {}
-        for group, p in every:
-            if p not in self.state or "step" not in self.state[p]:
+        # one call for the parameters that share a group, a GPU, their types and their step
+        fresh, counters, calls, state = {}, {}, {}, self.state
+        for group, p, g in every:
+            st = state.get(p)
+            if st is None or "step" not in st:
                 self._init_state(p, fresh)
-            st = self.state[p]
+                st = state[p]
             if self.capturable:
-                counters[id(st["step"])] = st["step"]
                 at = id(st["step"])
+                counters[at] = st["step"]
             else:
-                st["step"] += 1
-                at = st["step"]
-            key = (id(group), p.device, p.dtype, p.grad.dtype, "avg_scale" in st, "master" in st,
+                at = st["step"] = st["step"] + 1
+            key = (id(group), p.get_device(), p.dtype, g.dtype, "avg_scale" in st, "master" in st,
                    at)
-            lists.setdefault(key, (group, []))[1].append(p)
+            call = calls.get(key)
+            if call is None:
+                call = calls[key] = (group, [], [], [])
+            call[1].append(p)
+            call[2].append(g)
+            call[3].append(st)
         for t in counters.values():
             t.add_(1)
-        for key, (group, ps) in lists.items():
-            st = [self.state[p] for p in ps]
+        for key, (group, ps, gs, st) in calls.items():
             common = dict(lr=group["lr"], betas=group["betas"], eps=group["eps"],
                           weight_decay=group["weight_decay"], grad_stats=grad_stats,
                           masters=[s["master"] for s in st] if key[5] else None,
                           skip_nonfinite=self.skip_nonfinite)
-            grads = [p.grad for p in ps]
             if key[4]:
-                adamw_step_8bit(ps, grads, [s["exp_avg"] for s in st], [s["exp_rms"] for s in st],
+                adamw_step_8bit(ps, gs, [s["exp_avg"] for s in st], [s["exp_rms"] for s in st],
                                 [s["avg_scale"] for s in st], [s["rms_scale"] for s in st],
                                 st[0]["step"], seed=self.seed, **common)
             else:
-                adamw_step(ps, grads, [s["exp_avg"] for s in st], [s["exp_avg_sq"] for s in st],
+                adamw_step(ps, gs, [s["exp_avg"] for s in st], [s["exp_avg_sq"] for s in st],
                            st[0]["step"], **common)
         return loss
 
