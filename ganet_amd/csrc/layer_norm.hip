@@ -28,8 +28,7 @@ struct Args {
   float *mean, *rstd;               // written (forward, may be null) or read
   float *partial;                   // [workgroups][2][C] or null
   void *dw, *db;                    // grad_weight and grad_bias, where the launch writes them itself
-  unsigned main;                    // workgroups before those that do ...
-  int strip;                        // ... and the vectors of columns that each of those takes (rows)
+  unsigned main;                    // workgroups before those that do
   long long outer, inner, xs, ys, gs;
   int C, wdtype;
   float eps, inv_c, c;              // 1 / C and C
@@ -302,16 +301,19 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_rows_fwd(Args a)
 // before it works on this one.  Few, large workgroups: each leaves [2][C] floats to be added.
 constexpr int kBwdThreads = 1024;
 
-// kApart: the sums of STRIP vectors of columns.  Groups of STRIP lanes take the rows, four at once.
-template <typename T, int STRIP>
+// kApart: the sums of eight vectors of columns (128 bytes of a row; 64 are slower for wide rows, 512 x
+// 5000 float32 17.8 and 14.3 us, and faster for few, 512 x 255 bf16 8.4 and 9.4).  128 groups of eight
+// lanes take the rows, four at once.
+constexpr int kStrip = 8;
+template <typename T>
 __device__ __forceinline__ void strip_sums(const Args &a, int strip) {
-  constexpr int N = kN<T>, GROUPS = kBwdThreads / STRIP, U = 4;
-  __shared__ float part[2][kBwdThreads / 64][STRIP * N];
-  const int l = threadIdx.x & (STRIP - 1), c = (strip * STRIP + l) * N;
+  constexpr int N = kN<T>, GROUPS = kBwdThreads / kStrip, U = 4;
+  __shared__ float part[2][kBwdThreads / 64][kStrip * N];
+  const int l = threadIdx.x & (kStrip - 1), c = (strip * kStrip + l) * N;
   float s[2][N];
 #pragma unroll
   for (int k = 0; k < N; ++k) s[0][k] = s[1][k] = 0.0f;
-  for (int row = (int)threadIdx.x / STRIP; row < (int)a.outer; row += GROUPS * U) {
+  for (int row = (int)threadIdx.x / kStrip; row < (int)a.outer; row += GROUPS * U) {
     Vec<T, N> x[U], g[U];
     float mu[U], rs[U];
 #pragma unroll
@@ -341,24 +343,26 @@ __device__ __forceinline__ void strip_sums(const Args &a, int strip) {
   for (int which = 0; which < 2; ++which)
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      const float v = across_groups<STRIP>(s[which][k]);
-      if ((threadIdx.x & 63) < STRIP) part[which][threadIdx.x >> 6][l * N + k] = v;
+      const float v = across_groups<kStrip>(s[which][k]);
+      if ((threadIdx.x & 63) < kStrip) part[which][threadIdx.x >> 6][l * N + k] = v;
     }
   ganet_vec::lds_barrier();
-  const int at = threadIdx.x % (STRIP * N), which = threadIdx.x / (STRIP * N);
-  if (which > 1 || strip * STRIP * N + at >= a.C) return;
+  const int at = threadIdx.x % (kStrip * N), which = threadIdx.x / (kStrip * N);
+  if (which > 1 || strip * kStrip * N + at >= a.C) return;
   float v = 0.0f;
 #pragma unroll
   for (int i = 0; i < kBwdThreads / 64; ++i) v += part[which][i][at];
-  store_weight(which ? a.db : a.dw, a.wdtype, strip * STRIP * N + at, v);
+  store_weight(which ? a.db : a.dw, a.wdtype, strip * kStrip * N + at, v);
 }
 
 template <typename T, int LANES, int NV, Sums HOW>
 __global__ __launch_bounds__(kBwdThreads) void ln_rows_bwd(Args a) {
   if constexpr (HOW == kApart)
     if (blockIdx.x >= a.main) {
-      const int strip = (int)(blockIdx.x - a.main);
-      return a.strip == 4 ? strip_sums<T, 4>(a, strip) : strip_sums<T, 8>(a, strip);
+      // neighbouring strips on one XCD: rows of odd length share cache lines
+      const int i = (int)(blockIdx.x - a.main), strip = (i & 7) * ((int)(gridDim.x - a.main) >> 3) + (i >> 3);
+      if (strip * kStrip * kN<T> < a.C) strip_sums<T>(a, strip);
+      return;
     }
   constexpr bool SUMS = HOW == kPartial;
   constexpr int N = kN<T>;
@@ -980,11 +984,11 @@ int with_plane_shape(const ganet_layer_norm_params *p, F &&f) {
 
 // Up to where the sums over positions go to workgroups of the same launch.  One launch less is 3 us
 // less for a call that the host bounds (250 rows of 256: 9.5 and 7.2 us), and wide rows leave no
-// partial sums as large as themselves (250 x 16384 bf16 35 and 13 us); what it costs is one workgroup's
-// way through all positions of its columns (1024 rows of 4096 bf16 17 and 11 us, 2048 rows 20 and 29;
-// 16000 positions of 256 channels 11.4 and 9.5 us, 32000 14.5 and 19.7) and reading the values twice
-// (4 x 40 x 100 positions of 512 channels float32 32 and 34 us, of 256 20.2 and 19.1).
-constexpr long long kApartRows = 1024, kApartPositions = 1 << 14, kApartValues = 1 << 22;
+// partial sums as large as themselves (256 x 16384 bf16 35.7 us and 18.7).  What it costs is one
+// workgroup's way through all positions of its columns and reading the values twice.  The GPU's time
+// over three sets of tensors in turn: 512 rows of 1024 float32 4.7 us (with partial sums 6.7), 1024 rows
+// 13.8 (8.4); 4 x 256 x 40 x 100 bf16 11.7 (13.6), 8 x 256 x 40 x 100 19.7 (14.5).
+constexpr long long kApartRows = 512, kApartPositions = 1 << 14, kApartValues = 1 << 22;
 
 // Workgroups of the backward, each with sums of its own: what is on the chip at once.
 int backward_blocks(const ganet_layer_norm_params *p) {
@@ -1079,11 +1083,8 @@ int launch_backward(const ganet_layer_norm_params *p, Args a, int blocks, hipStr
       constexpr int L = lanes.value, NV = nv.value;
       constexpr int groups = L < 64 ? kBwdThreads / 64 : kBwdThreads / L;
       constexpr size_t room = HOW == kPartial ? (size_t)groups * L * NV * kN<T> * sizeof(float) : 0;
-      // 64 or 128 bytes of a row: the narrow ones where the others are too few for the chip (777 rows of
-      // 1001 f16 7.7 and 8.9 us; 777 of 4096 12.1 and 9.6)
-      const int vecs = (p->C + kN<T> - 1) / kN<T>;
-      a.strip = vecs > 31 * 8 ? 8 : 4;
-      const int more = HOW == kApart ? (vecs + a.strip - 1) / a.strip : 0;
+      constexpr int columns = 8 * kStrip * kN<T>;              // of eight strips
+      const int more = HOW == kApart ? (p->C + columns - 1) / columns * 8 : 0;
       ln_rows_bwd<T, L, NV, HOW><<<dim3(blocks + more), dim3(kBwdThreads), room, s>>>(a);
       return ganet_check_launch();
     });
