@@ -502,7 +502,8 @@ int ganet_layer_norm_forward(const void *x, const void *weight, const void *bias
  *   grad_x = rstd * (a - mean_C(a) - xh * mean_C(a * xh)),
  *   grad_weight = sum over positions of grad_y * xh, grad_bias = sum of grad_y.
  * The sums over positions are formed in a fixed order: partial sums of each workgroup go
- * to the workspace, a second launch adds them.  The same inputs give the same bits.
+ * to the workspace, a second launch adds them (few positions: one launch, which leaves the
+ * workspace alone).  The same inputs give the same bits.
  * Outputs must not overlap inputs. */
 size_t ganet_layer_norm_backward_workspace_bytes(const ganet_layer_norm_params *p);
 int ganet_layer_norm_backward(const void *x, const void *weight, const void *grad_y,
