@@ -283,18 +283,26 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8<MASTER> a) {
   }
   um = block_max(um);
   ur = block_max(ur);
-  // A gradient that is not finite reaches its own value only: it is left out of the scales and
-  // becomes e4m3's NaN.
-  unsigned bad = 0;
+  // What is not finite reaches its own value only: it is left out of the scales.  After a gradient that
+  // is not, both codes are e4m3's NaN.  A finite gradient whose square is not leaves a second moment
+  // of infinity, as in float32: r's code is NaN over an m that is none, and the value stands still (m over
+  // infinity) in this step and in all that follow.
+  unsigned bad = 0, held = 0;           // a bit a value: both codes NaN; r's
   if (um >= kInf || ur >= kInf) {
     um = ur = 0;
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
-      if (sq[j] == INFINITY) nr[j] = INFINITY;         // a step of zero
+      const unsigned cm = vm >> (8 * j) & 0x7F, cr = vr >> (8 * j) & 0x7F;
+      if (sq[j] == INFINITY || (cr == 0x7F && cm != 0x7F)) nr[j] = INFINITY;
       const unsigned mb = __float_as_uint(nm[j]) & 0x7FFFFFFFu, rb = __float_as_uint(nr[j]);
-      if (mb >= kInf || rb >= kInf) bad |= 1u << j;
-      if (mb < kInf && mb > um) um = mb;
-      if (rb < kInf && rb > ur) ur = rb;
+      if (mb >= kInf || rb > kInf)
+        bad |= 1u << j;
+      else if (rb == kInf)
+        held |= 1u << j;
+      else {
+        if (mb > um) um = mb;
+        if (rb > ur) ur = rb;
+      }
     }
     um = block_max(um);
     ur = block_max(ur);
@@ -329,13 +337,12 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8<MASTER> a) {
   value(std::integral_constant<int, 1>());
   value(std::integral_constant<int, 2>());
   value(std::integral_constant<int, 3>());
-  if (bad) {
+  if (bad | held) {
 #pragma unroll
-    for (int j = 0; j < kVec; ++j)
-      if (bad >> j & 1) {
-        om |= 0x7Fu << (8 * j);
-        orr |= 0x7Fu << (8 * j);
-      }
+    for (int j = 0; j < kVec; ++j) {
+      if (bad >> j & 1) om |= 0x7Fu << (8 * j);
+      if ((bad | held) >> j & 1) orr |= 0x7Fu << (8 * j);
+    }
   }
   if constexpr (MASTER) vw.store(w + i, k);
   vp.store(p + i, k);
