@@ -300,7 +300,9 @@ class AdamW(torch.optim.Optimizer):
     skip_nonfinite: with max_grad_norm (or grad_stats given to step) a step whose gradients' norm
     is not finite changes no weight and no moment; the step number goes on.
     capturable: step numbers live on the device, so that a step captured into a HIP graph counts
-    on when replayed; make one step before the capture.  lr may be a float32 tensor on the device.
+    on when replayed; make one step before the capture, with gradients for the same parameters.  lr
+    may be a float32 tensor on the device.  Bias corrections are formed in float32 there, so such a
+    step and one that the host counts may differ in a weight's last bit.
     `grad_stats` holds the last step's grad_norm tensor."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
@@ -322,6 +324,7 @@ class AdamW(torch.optim.Optimizer):
         self.max_grad_norm, self.skip_nonfinite = max_grad_norm, skip_nonfinite
         self.seed, self.min_8bit_size, self.capturable = seed, min_8bit_size, capturable
         self.grad_stats = None
+        self._captured = {}               # step numbers on the device that a graph counts, by id
 
     def __getstate__(self):
         """Copies and pickles keep the options too (torch's own state has the groups only)."""
@@ -329,7 +332,7 @@ class AdamW(torch.optim.Optimizer):
         for name in ("state_bits", "master_weights", "max_grad_norm", "skip_nonfinite", "seed",
                      "min_8bit_size", "capturable"):
             kept[name] = getattr(self, name)
-        kept["grad_stats"] = None
+        kept["grad_stats"], kept["_captured"] = None, {}
         return kept
 
     def _init_state(self, p, fresh):
@@ -355,6 +358,33 @@ class AdamW(torch.optim.Optimizer):
         if self.master_weights and p.dtype != torch.float32:
             st["master"] = p.detach().float()
 
+    def _split_counters(self, stepped, capturing):
+        """Parameters share their step number on the device with all that have been stepped as often;
+        those that are stepped while others of theirs have no gradient get one of their own."""
+        now, users = {}, {}
+        for _, p, _ in stepped:
+            st = self.state.get(p, ())
+            if "step" in st:
+                now.setdefault(id(st["step"]), []).append(st)
+        if sum(map(len, now.values())) < len(self.state):
+            for st in self.state.values():
+                if "step" in st:
+                    at = id(st["step"])
+                    users[at] = users.get(at, 0) + 1
+        parted = [sts for at, sts in now.items() if len(sts) < users.get(at, 0)]
+        if parted and capturing:             # the copy of the number would be part of the graph
+            raise RuntimeError("AdamW: a parameter without a gradient shares its step number with some "
+                               "of a captured step: make one step with the same gradients before")
+        if any(id(sts[0]["step"]) in self._captured for sts in parted):
+            raise RuntimeError("AdamW: a captured step counts these parameters with one number: all of "
+                               "them need gradients (load_state_dict(state_dict()) forgets the graph)")
+        for sts in parted:
+            number = sts[0]["step"].clone()
+            for st in sts:
+                st["step"] = number
+        if capturing:
+            self._captured.update((id(sts[0]["step"]), sts[0]["step"]) for sts in now.values())
+
     @torch.no_grad()
     def step(self, closure=None, grad_stats=None):
         loss = None
@@ -368,12 +398,15 @@ class AdamW(torch.optim.Optimizer):
         grads = [g for _, _, g in every]
         if any(g.is_sparse for g in grads):
             raise RuntimeError("AdamW: sparse gradients")
-        if every[0][1].is_cuda and torch.cuda.is_current_stream_capturing():
+        capturing = every[0][1].is_cuda and torch.cuda.is_current_stream_capturing()
+        if capturing:
             # the number of the step would be part of the graph, a new state its memory
             if not self.capturable:
                 raise RuntimeError("AdamW: a captured step needs capturable=True")
             if any("step" not in self.state.get(p, ()) for _, p, _ in every):
                 raise RuntimeError("AdamW: make one step before the capture")
+        if self.capturable:
+            self._split_counters(every, capturing)
         if grad_stats is None and self.max_grad_norm is not None:
             grad_stats = grad_norm(grads, self.max_grad_norm)
         self.grad_stats = grad_stats

@@ -49,3 +49,92 @@ def test_a_square_past_the_largest_float_stops_its_weight_only(dtype, master):
             assert torch.equal(a, b), t
         if t >= 1:                                                 # from the second step on
             assert torch.equal(one[0][at], runs[0][0][0][at]) and torch.isfinite(one[0]).all()
+
+
+def numbers(opt, ps):
+    return [int(opt.state[p]["step"]) if p in opt.state else 0 for p in ps]
+
+
+def sparse_steps(opt, ps, present, t_of, gen, bits=32):
+    """One step in which only the parameters `present` have gradients, checked with a number of its
+    own for each of them."""
+    for i, p in enumerate(ps):
+        p.grad = torch.randn(p.shape, generator=gen, device="cuda") if i in present else None
+    some = [ps[i] for i in present]
+    had = [p in opt.state for p in some]
+    before = [dict(params=[p.detach().clone()], grads=[p.grad], masters=None,
+                   m=[opt.state[p]["exp_avg"].clone() if h else torch.zeros_like(p)],
+                   v=[opt.state[p]["exp_avg_sq"].clone() if h else torch.zeros_like(p)])
+              for p, h in zip(some, had)] if bits == 32 else None
+    opt.step()
+    for i in present:
+        t_of[i] += 1
+    if before is not None:
+        for i, p, b in zip(present, some, before):
+            s = opt.state[p]
+            check32(b, dict(params=[p.detach()], m=[s["exp_avg"]], v=[s["exp_avg_sq"]]), t_of[i], HYPER)
+    assert numbers(opt, ps) == t_of
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_parameter_without_a_gradient_is_not_counted(capturable, bits):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(4)
+    ps = [torch.nn.Parameter(torch.randn(n, generator=gen, device="cuda")) for n in (300, 70, 513)]
+    opt = optim.AdamW(ps, capturable=capturable, state_bits=bits, min_8bit_size=1, **HYPER)
+    t_of = [0, 0, 0]
+    for present in ((0, 1), (0, 2), (0, 1, 2), (0, 2), (2,), (0, 1, 2), (1,)):      # the third comes later
+        sparse_steps(opt, ps, present, t_of, gen, bits)
+    twin = optim.AdamW(ps, capturable=capturable, state_bits=bits, min_8bit_size=1, **HYPER)
+    twin.load_state_dict(opt.state_dict())
+    assert numbers(twin, ps) == t_of == [5, 4, 5]
+    for present in ((0, 1, 2), (0,), (1, 2)):
+        sparse_steps(twin, ps, present, t_of, gen, bits)
+
+
+@gpu
+def test_captured_steps_and_missing_gradients():
+    """What a captured step shares a number with has to have a gradient too, before and after."""
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(5)
+
+    def fresh():
+        ps = [torch.nn.Parameter(torch.randn(n, generator=gen, device="cuda")) for n in (300, 70)]
+        for p in ps:
+            p.grad = torch.randn(p.shape, generator=gen, device="cuda")
+        opt = optim.AdamW(ps, capturable=True, **HYPER)
+        opt.step()
+        torch.cuda.synchronize()
+        return ps, opt
+
+    ps, opt = fresh()
+    keep, ps[1].grad = ps[1].grad, None
+    with pytest.raises(RuntimeError, match="gradient"):      # would count ps[1] on every replay
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            opt.step()
+    opt.step()                                               # the same outside: has numbers of its own
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+    assert numbers(opt, ps) == [5, 1]
+    ps[1].grad = keep
+    opt.step()
+    assert numbers(opt, ps) == [6, 2]
+
+    ps, opt = fresh()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    graph.replay()
+    torch.cuda.synchronize()
+    ps[1].grad = None
+    with pytest.raises(RuntimeError, match="captured"):      # the graph counts both with one number
+        opt.step()
+    assert numbers(opt, ps) == [2, 2]
