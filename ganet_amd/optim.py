@@ -27,6 +27,7 @@ from . import _lib
 from .dcn import _DTYPES
 
 BLOCK = _lib.GANET_STATE_BLOCK
+_PLACE = 0x85EBCA6B           # a place further in the list adds this to the seed of the random words
 
 
 _ptrs, _sizes, _gpus = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
@@ -216,7 +217,9 @@ def adamw_step_8bit(params, grads, exp_avgs, exp_rms, avg_scales, rms_scales, st
     are float8_e4m3fn of the parameter's shape, in units of avg_scales / rms_scales, one float32
     for each 256 values in memory order (state_8bit makes them).  States are rounded up or down at
     random, by a hash of (seed, step, the parameter's place in the list, the value's place in it):
-    the same inputs give the same bits.  Parameters move by the moments before that rounding."""
+    the same inputs give the same bits.  Several calls of one step need seeds of their own, or their
+    i-th parameters are rounded alike (AdamW counts the places on over its calls).  Parameters move
+    by the moments before that rounding."""
     _step(params, grads, exp_avgs, exp_rms, avg_scales, rms_scales, 8, step, lr, betas, eps,
           weight_decay, masters, grad_stats, skip_nonfinite, seed)
 
@@ -292,7 +295,8 @@ def _read_grads(grads, out):
 
 
 class AdamW(torch.optim.Optimizer):
-    """AdamW over the parameters of a model, a few launches a step.
+    """AdamW over the parameters of a model, a few launches a step (parameters of equal settings and
+    types share one, whatever groups they are in).
 
     state_bits=8: moments in 8 bits (parameters of fewer than min_8bit_size values keep 32).
     master_weights: 16-bit parameters get float32 masters, made from them at their first step.
@@ -391,8 +395,14 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        every = [(group, p, p.grad) for group in self.param_groups for p in group["params"]]
-        every = [one for one in every if one[2] is not None]
+        # groups of equal settings are one
+        every, alike = [], {}
+        for group in self.param_groups:
+            lr = group["lr"]
+            values = (("lr", id(lr)) if torch.is_tensor(lr) else lr, tuple(group["betas"]),
+                      group["eps"], group["weight_decay"])
+            first = alike.setdefault(values, group)
+            every += [(first, p, p.grad) for p in group["params"] if p.grad is not None]
         if not every:
             return loss
         grads = [g for _, _, g in every]
@@ -432,6 +442,7 @@ class AdamW(torch.optim.Optimizer):
             call[3].append(st)
         for t in counters.values():
             t.add_(1)
+        place = 0                             # 8-bit tensors of the calls before
         for key, (group, ps, gs, st) in calls.items():
             common = dict(lr=group["lr"], betas=group["betas"], eps=group["eps"],
                           weight_decay=group["weight_decay"], grad_stats=grad_stats,
@@ -440,7 +451,8 @@ class AdamW(torch.optim.Optimizer):
             if key[4]:
                 adamw_step_8bit(ps, gs, [s["exp_avg"] for s in st], [s["exp_rms"] for s in st],
                                 [s["avg_scale"] for s in st], [s["rms_scale"] for s in st],
-                                st[0]["step"], seed=self.seed, **common)
+                                st[0]["step"], seed=self.seed + place * _PLACE, **common)
+                place += len(ps)
             else:
                 adamw_step(ps, gs, [s["exp_avg"] for s in st], [s["exp_avg_sq"] for s in st],
                            st[0]["step"], **common)

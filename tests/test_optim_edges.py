@@ -138,3 +138,62 @@ def test_captured_steps_and_missing_gradients():
     with pytest.raises(RuntimeError, match="captured"):      # the graph counts both with one number
         opt.step()
     assert numbers(opt, ps) == [2, 2]
+
+
+def codes(opt, p):
+    return [opt.state[p][k].view(torch.uint8) for k in ("exp_avg", "exp_rms")]
+
+
+@gpu
+@pytest.mark.parametrize("capturable", [False, True])
+def test_groups_round_with_words_of_their_own(capturable):
+    """Equal weights with equal gradients in two groups: equal moments, unlike roundings; the words
+    are those of one list of all tensors."""
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(6)
+    value, grad = (torch.randn(5000, generator=gen, device="cuda") for _ in range(2))
+    ps = [torch.nn.Parameter(value.clone()) for _ in range(4)]
+    opt = optim.AdamW([dict(params=ps[:2], weight_decay=0.0), dict(params=ps[2:], weight_decay=0.1)],
+                      state_bits=8, seed=21, capturable=capturable)
+    st = [optim.state_8bit(p.detach()) for p in ps]
+    raw = [value.clone() for _ in ps]
+    for t in (1, 2):
+        for p in ps:
+            p.grad = grad.clone()
+        opt.step()
+        # the moments do not depend on the weights: one raw call over all four
+        optim.adamw_step_8bit(raw, [grad] * 4, *([s[k] for s in st] for k in range(4)), t, seed=21)
+        for p, s in zip(ps, st):
+            for a, b in zip(codes(opt, p), s[:2]):
+                assert torch.equal(a, b.view(torch.uint8))
+    for i in range(4):
+        for j in range(i):
+            for a, b in zip(codes(opt, ps[i]), codes(opt, ps[j])):
+                assert not torch.equal(a, b), (i, j)
+
+
+@gpu
+def test_groups_alike_are_stepped_in_one_call(monkeypatch):
+    """One group a parameter, as a config with settings by name makes them."""
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(7)
+    values = [torch.randn(500 + i, generator=gen, device="cuda") for i in range(6)]
+    grads = [torch.randn(500 + i, generator=gen, device="cuda") for i in range(6)]
+    done = []
+    for split in (True, False):
+        ps = [torch.nn.Parameter(v.clone()) for v in values]
+        opt = optim.AdamW([dict(params=[p], betas=[0.9, 0.99]) for p in ps] if split else ps, lr=1e-2,
+                          betas=(0.9, 0.99), state_bits=8, min_8bit_size=503, seed=3)
+        calls = []
+        for name in ("adamw_step", "adamw_step_8bit"):
+            monkeypatch.setattr(optim, name, lambda *a, _f=getattr(optim, name), **kw: (
+                calls.append(len(a[0])), _f(*a, **kw))[1])
+        for _ in range(2):
+            for p, g in zip(ps, grads):
+                p.grad = g.clone()
+            opt.step()
+        monkeypatch.undo()
+        assert sorted(calls) == [3, 3, 3, 3]
+        done.append([p.detach() for p in ps] + [c for p in ps[3:] for c in codes(opt, p)])
+    for a, b in zip(*done):
+        assert torch.equal(a, b)
