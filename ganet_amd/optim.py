@@ -465,7 +465,8 @@ class AdamW(torch.optim.Optimizer):
         ps = [p for group in self.param_groups for p in group["params"]]
         counters = {}
         for i, p in zip(ids, ps):
-            for name, value in state_dict["state"].get(i, {}).items():
+            saved = state_dict["state"].get(i, {})
+            for name, value in saved.items():
                 if name == "step":
                     value = int(value)
                     if self.capturable:        # one counter for the parameters that share a number
@@ -474,18 +475,53 @@ class AdamW(torch.optim.Optimizer):
                             counters[key] = torch.full((), value, dtype=torch.int64,
                                                        device=p.device)
                         value = counters[key]
-                elif name in ("avg_scale", "rms_scale"):
-                    value = value.detach().to(p.device, copy=True)
+                elif name in _SCALES.values():
+                    continue                   # comes with its codes
+                elif torch.is_tensor(value) and value.dtype == torch.float8_e4m3fn:
+                    scale = _SCALES[name]
+                    value, self.state[p][scale] = _codes_like(p, value.detach(), saved[scale].detach(),
+                                                              name == "exp_rms")
                 elif torch.is_tensor(value):
-                    kept = torch.empty_like(p, dtype=value.dtype)
-                    value = kept.copy_(value.detach()) if value.dtype != torch.float8_e4m3fn else \
-                        _copy_codes(kept, value)
+                    value = _values_like(p, value)
                 self.state[p][name] = value
 
 
-def _copy_codes(to, codes):
-    to.view(torch.uint8).copy_(codes.detach().view(torch.uint8))
-    return to
+_SCALES = dict(exp_avg="avg_scale", exp_rms="rms_scale")      # of the states in 8 bits
+
+
+def _values_like(p, value):
+    """A copy of a state's values in the parameter's memory order."""
+    return torch.empty_like(p, dtype=value.dtype).copy_(value.detach())
+
+
+def _codes_like(p, codes, scale, root):
+    """Copies of a state's codes and scales in the parameter's memory order.  A scale belongs to 256
+    values in memory order: where the state was saved from another one its values are divided into
+    other blocks, each rounded to nearest in its new scale; a root above zero stays above zero."""
+    codes = codes.to(p.device, copy=True)
+    scale = scale.to(p.device, copy=True)
+    if _same_order(p, codes):
+        return codes, scale
+    if not _dense(codes) or not _dense(p):
+        raise ValueError("AdamW: a saved state of shape %s and strides %s for a parameter of shape %s and "
+                         "strides %s" % (tuple(codes.shape), codes.stride(), tuple(p.shape), p.stride()))
+    n = p.numel()
+
+    def flat(t):
+        return t.as_strided((n,), (1,))
+
+    saved = torch.empty_strided(codes.shape, codes.stride(), dtype=torch.float32, device=p.device)
+    flat(saved).copy_(flat(codes.view(torch.uint8)).view(torch.float8_e4m3fn).float()
+                      * scale.repeat_interleave(BLOCK)[:n])
+    x = torch.nn.functional.pad(flat(_values_like(p, saved)), (0, -n % BLOCK)).reshape(-1, BLOCK)
+    top = torch.where(x.isnan(), torch.zeros_like(x), x.abs()).amax(1)
+    top = torch.where(top < 2.0 ** -110, torch.zeros_like(top), top)      # as the step holds such blocks
+    y = (x * torch.where(top > 0, 448 / top, torch.zeros_like(top))[:, None]).clamp(-448, 448)
+    if root:
+        y = torch.where((x > 0) & (y < 2.0 ** -9), torch.full_like(y, 2.0 ** -9), y)
+    kept = torch.empty_like(p, dtype=torch.uint8)
+    flat(kept).copy_(y.reshape(-1)[:n].to(torch.float8_e4m3fn).view(torch.uint8))
+    return kept.view(torch.float8_e4m3fn), top / 448
 
 
 def register_with_mmcv(force=False):

@@ -197,3 +197,51 @@ def test_groups_alike_are_stepped_in_one_call(monkeypatch):
         done.append([p.detach() for p in ps] + [c for p in ps[3:] for c in codes(opt, p)])
     for a, b in zip(*done):
         assert torch.equal(a, b)
+
+
+@gpu
+def test_states_of_another_memory_order():
+    """Scales belong to 256 values in memory order: states saved from a channels_last weight and loaded
+    into a contiguous one are divided into other blocks.  A value keeps its sign and is off by half
+    of e4m3's spacing in its new scale, 2^-4 of itself or 2^-10 of the scale; a root above zero
+    stays above zero (2^-9 of the scale at least)."""
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(8)
+    shape = (16, 40, 3, 3)
+    w = torch.randn(shape, generator=gen, device="cuda")
+    size = torch.exp(torch.randn(shape, generator=gen, device="cuda") * 2)
+    p = torch.nn.Parameter(w.contiguous(memory_format=torch.channels_last))
+    q = torch.nn.Parameter(w.clone())
+    a, b, same = (optim.AdamW([x], state_bits=8, seed=2) for x in (p, q, torch.nn.Parameter(p.detach())))
+    for _ in range(3):
+        p.grad = (torch.randn(shape, generator=gen, device="cuda") * size).contiguous(
+            memory_format=torch.channels_last)
+        a.step()
+
+    def values(opt, p, key, scale):
+        """The state in the weight's shape, and the scale of each of its values."""
+        s = opt.state[p]
+        spread = s[scale].repeat_interleave(BLOCK)[:p.numel()]
+        per = torch.empty_like(p, requires_grad=False)
+        per.as_strided((p.numel(),), (1,)).copy_(spread)
+        assert s[key].stride() == p.stride()
+        return s[key].float() * per, per
+
+    b.load_state_dict(a.state_dict())
+    for key, scale in (("exp_avg", "avg_scale"), ("exp_rms", "rms_scale")):
+        old, _ = values(a, p, key, scale)
+        new, per = values(b, q, key, scale)
+        least = 2.0 ** -9 if key == "exp_rms" else 2.0 ** -10
+        tol = torch.maximum(old.abs() * 2.0 ** -4, per * least) * (1 + 8 * U)
+        assert ((new - old).abs() <= tol).all()
+        assert ((new > 0) == (old > 0)).all() or key == "exp_avg"
+        assert (new * old >= 0).all()
+    q.grad = p.grad.contiguous()
+    b.step()
+    assert torch.isfinite(q).all()
+    # in the same order nothing changes
+    same.load_state_dict(a.state_dict())
+    r = same.param_groups[0]["params"][0]
+    for k in ("exp_avg", "exp_rms", "avg_scale", "rms_scale"):
+        one, two = a.state[p][k], same.state[r][k]
+        assert torch.equal(one.view(torch.uint8), two.view(torch.uint8)) and one.stride() == two.stride()
