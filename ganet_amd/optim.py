@@ -459,7 +459,9 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """States keep the types they were saved in (torch would cast them to the parameter's)."""
+        """States keep the types they were saved in (torch would cast them to the parameter's); 16-bit
+        moments, as torch's AdamW keeps for 16-bit parameters, become float32, and with
+        master_weights a state without a master gets one from the parameter."""
         super(AdamW, self).load_state_dict(state_dict)
         ids = [i for group in state_dict["param_groups"] for i in group["params"]]
         ps = [p for group in self.param_groups for p in group["params"]]
@@ -482,8 +484,10 @@ class AdamW(torch.optim.Optimizer):
                     value, self.state[p][scale] = _codes_like(p, value.detach(), saved[scale].detach(),
                                                               name == "exp_rms")
                 elif torch.is_tensor(value):
-                    value = _values_like(p, value)
+                    value = _values_like(p, value.float() if name in ("exp_avg", "exp_avg_sq") else value)
                 self.state[p][name] = value
+            if saved and self.master_weights and p.dtype != torch.float32 and "master" not in saved:
+                self.state[p]["master"] = p.detach().float()
 
 
 _SCALES = dict(exp_avg="avg_scale", exp_rms="rms_scale")      # of the states in 8 bits

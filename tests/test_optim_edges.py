@@ -245,3 +245,37 @@ def test_states_of_another_memory_order():
     for k in ("exp_avg", "exp_rms", "avg_scale", "rms_scale"):
         one, two = a.state[p][k], same.state[r][k]
         assert torch.equal(one.view(torch.uint8), two.view(torch.uint8)) and one.stride() == two.stride()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("master", [False, True])
+def test_states_of_torch_are_taken_over(dtype, master):
+    """torch.optim.AdamW keeps 16-bit moments for 16-bit weights, and no masters."""
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(9)
+    ps = [torch.nn.Parameter(torch.randn(n, generator=gen, device="cuda").to(dtype)) for n in (77, 400)]
+    theirs = torch.optim.AdamW(ps, lr=HYPER["lr"], weight_decay=HYPER["weight_decay"])
+
+    def gradients():
+        for p in ps:
+            p.grad = torch.randn(p.shape, generator=gen, device="cuda").to(dtype)
+
+    for _ in range(3):
+        gradients()
+        theirs.step()
+    ours = optim.AdamW(ps, master_weights=master, **HYPER)
+    ours.load_state_dict(theirs.state_dict())
+    masters = master and dtype != torch.float32
+    before = dict(params=[p.detach().clone() for p in ps], grads=None,
+                  m=[theirs.state[p]["exp_avg"].float() for p in ps],
+                  v=[theirs.state[p]["exp_avg_sq"].float() for p in ps],
+                  masters=[p.detach().float() for p in ps] if masters else None)
+    gradients()
+    before["grads"] = [p.grad for p in ps]
+    ours.step()
+    st = [ours.state[p] for p in ps]
+    assert all(("master" in s) == masters for s in st)
+    check32(before, dict(params=[p.detach() for p in ps], m=[s["exp_avg"] for s in st],
+                         v=[s["exp_avg_sq"] for s in st],
+                         masters=[s["master"] for s in st] if masters else None), 4, HYPER)
