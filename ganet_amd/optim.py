@@ -294,6 +294,15 @@ def _read_grads(grads, out):
             dtypes.tobytes(), grads)
 
 
+def _check_settings(lr, betas, eps, weight_decay):
+    if not torch.is_tensor(lr) and not 0 <= lr < math.inf:
+        raise ValueError("AdamW: lr %r" % (lr,))
+    if not all(0 <= b < 1 for b in betas):
+        raise ValueError("AdamW: betas %r" % (betas,))
+    if not 0 <= eps < math.inf or not 0 <= weight_decay < math.inf:
+        raise ValueError("AdamW: eps %r, weight_decay %r" % (eps, weight_decay))
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW over the parameters of a model, a few launches a step (parameters of equal settings and
     types share one, whatever groups they are in).
@@ -312,12 +321,7 @@ class AdamW(torch.optim.Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
                  state_bits=32, master_weights=False, max_grad_norm=None, skip_nonfinite=True,
                  seed=0, min_8bit_size=4096, capturable=False):
-        if not torch.is_tensor(lr) and not (0 <= lr < math.inf):
-            raise ValueError("AdamW: lr %r" % (lr,))
-        if not all(0 <= b < 1 for b in betas):
-            raise ValueError("AdamW: betas %r" % (betas,))
-        if not 0 <= eps < math.inf or not 0 <= weight_decay < math.inf:
-            raise ValueError("AdamW: eps %r, weight_decay %r" % (eps, weight_decay))
+        _check_settings(lr, betas, eps, weight_decay)
         if state_bits not in (32, 8):
             raise ValueError("AdamW: states of %r bits" % (state_bits,))
         if max_grad_norm is not None and not max_grad_norm >= 0:
@@ -347,7 +351,7 @@ class AdamW(torch.optim.Optimizer):
             raise TypeError("AdamW: unsupported dtype %s" % p.dtype)
         if not _dense(p):
             raise ValueError("AdamW: a parameter of strides %s is not dense" % (p.stride(),))
-        st = self.state[p]
+        st = {}
         if self.capturable:
             if p.device not in fresh:
                 fresh[p.device] = torch.zeros((), dtype=torch.int64, device=p.device)
@@ -361,6 +365,7 @@ class AdamW(torch.optim.Optimizer):
             st["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
         if self.master_weights and p.dtype != torch.float32:
             st["master"] = p.detach().float()
+        self.state[p] = st                    # whole or not at all
 
     def _split_counters(self, stepped, capturing):
         """Parameters share their step number on the device with all that have been stepped as often;
@@ -401,6 +406,8 @@ class AdamW(torch.optim.Optimizer):
             lr = group["lr"]
             values = (("lr", id(lr)) if torch.is_tensor(lr) else lr, tuple(group["betas"]),
                       group["eps"], group["weight_decay"])
+            if values not in alike:
+                _check_settings(lr, *values[1:])
             first = alike.setdefault(values, group)
             every += [(first, p, p.grad) for p in group["params"] if p.grad is not None]
         if not every:
@@ -427,11 +434,10 @@ class AdamW(torch.optim.Optimizer):
             if st is None or "step" not in st:
                 self._init_state(p, fresh)
                 st = state[p]
+            at = st["step"]
             if self.capturable:
-                at = id(st["step"])
+                at = id(at)
                 counters[at] = st["step"]
-            else:
-                at = st["step"] = st["step"] + 1
             key = (id(group), p.get_device(), p.dtype, g.dtype, "avg_scale" in st, "master" in st,
                    at)
             call = calls.get(key)
@@ -448,14 +454,18 @@ class AdamW(torch.optim.Optimizer):
                           weight_decay=group["weight_decay"], grad_stats=grad_stats,
                           masters=[s["master"] for s in st] if key[5] else None,
                           skip_nonfinite=self.skip_nonfinite)
+            number = st[0]["step"] if self.capturable else key[6] + 1
             if key[4]:
                 adamw_step_8bit(ps, gs, [s["exp_avg"] for s in st], [s["exp_rms"] for s in st],
                                 [s["avg_scale"] for s in st], [s["rms_scale"] for s in st],
-                                st[0]["step"], seed=self.seed + place * _PLACE, **common)
+                                number, seed=self.seed + place * _PLACE, **common)
                 place += len(ps)
             else:
                 adamw_step(ps, gs, [s["exp_avg"] for s in st], [s["exp_avg_sq"] for s in st],
-                           st[0]["step"], **common)
+                           number, **common)
+            if not self.capturable:               # a call that is refused has stepped nothing
+                for s in st:
+                    s["step"] = number
         return loss
 
     def load_state_dict(self, state_dict):

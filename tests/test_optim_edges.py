@@ -279,3 +279,36 @@ def test_states_of_torch_are_taken_over(dtype, master):
     check32(before, dict(params=[p.detach() for p in ps], m=[s["exp_avg"] for s in st],
                          v=[s["exp_avg_sq"] for s in st],
                          masters=[s["master"] for s in st] if masters else None), 4, HYPER)
+
+
+@gpu
+def test_a_refused_step_counts_nothing():
+    """A parameter that was not stepped keeps its number and gets no half-made state."""
+    def parameter(*shape):
+        return torch.nn.Parameter(torch.ones(*shape, device="cuda"))
+
+    good, gaps, late = parameter(60), torch.nn.Parameter(torch.ones(8, 6, device="cuda")[:, ::2]), parameter(9)
+    opt = optim.AdamW([good, gaps], **HYPER)
+    for p in (good, gaps):
+        p.grad = torch.ones_like(p)
+    with pytest.raises(ValueError):
+        opt.step()
+    assert torch.equal(good, torch.ones_like(good)) and numbers(opt, [good]) == [0]
+    gaps.grad = None
+    opt.step()
+    assert numbers(opt, [good]) == [1] and gaps not in opt.state
+    check = torch.ones(60, device="cuda")
+    optim.adamw_step([check], [good.grad], [torch.zeros_like(check)], [torch.zeros_like(check)], 1, **HYPER)
+    assert torch.equal(check, good)
+
+    for capturable in (False, True):
+        good, late = parameter(60), parameter(9)
+        opt = optim.AdamW([dict(params=[good]), dict(params=[late], lr=1e-4)], capturable=capturable)
+        for p in (good, late):
+            p.grad = torch.ones_like(p)
+        opt.param_groups[1]["lr"] = -1.0
+        with pytest.raises((ValueError, _lib.GanetError)):
+            opt.step()
+        assert torch.equal(late, torch.ones_like(late))
+        # whatever was stepped has been counted, and what was not has not
+        assert numbers(opt, [good, late]) == [int(not torch.equal(good, torch.ones_like(good))), 0]
