@@ -4,7 +4,7 @@
 // A step checks every tensor of every list (GPU, type, shape, order, address): in Python that is
 // some 40 ns an attribute, 100 us for the seven lists of a 62-tensor model, as long as the step
 // itself.  Here it is a few.  The functions only accept the plain case - one GPU, one type a list,
-// everything contiguous and of its parameter's shape, nothing twice - and return None for anything
+// everything contiguous and of its parameter's shape, no memory twice - and return None for anything
 // else; Python then looks again, copies what can be copied and names what is wrong.
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
@@ -12,6 +12,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <utility>
 #include <vector>
 
 #include "ganet_hip.h"
@@ -56,7 +57,7 @@ bool read(PyObject *const *lists, std::int64_t block, Step &s) {
   const Py_ssize_t n = length(lists[0]);
   if (n < 1) return false;
   s.rows.assign(static_cast<size_t>(n) * 8, 0);
-  std::vector<std::uint64_t> written;
+  std::vector<std::pair<std::uint64_t, std::uint64_t>> written;        // addresses and bytes
   int types[7] = {kOther, kOther, kOther, kOther, kOther, kOther, kOther};
   s.gpu = -1;
   for (int k = 0; k < 7; ++k) {
@@ -81,11 +82,12 @@ bool read(PyObject *const *lists, std::int64_t block, Step &s) {
       const auto address = reinterpret_cast<std::uint64_t>(t->data_ptr());
       s.rows[i * 8 + k] = address;
       if (k == 0) s.rows[i * 8 + 7] = static_cast<std::uint64_t>(values);
-      if (k != 1 && values) written.push_back(address);
+      if (k != 1 && values) written.emplace_back(address, t->nbytes());
     }
   }
   std::sort(written.begin(), written.end());
-  if (std::adjacent_find(written.begin(), written.end()) != written.end()) return false;
+  for (size_t i = 1; i < written.size(); ++i)
+    if (written[i].first < written[i - 1].first + written[i - 1].second) return false;
   s.param = types[0];
   s.grad = types[1];
   s.state = types[2];

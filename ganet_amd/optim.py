@@ -55,6 +55,17 @@ def _same_order(a, b):
     return all(x == y for x, y, n in zip(a.stride(), b.stride(), a.shape) if n != 1)
 
 
+def _overlap(spans):
+    """Whether two of the (address, bytes) share a byte."""
+    end = 0
+    for begin, size in sorted(spans):
+        if size:
+            if begin < end:
+                return True
+            end = begin + size
+    return False
+
+
 def _one(tensors, what, index, dtype=None):
     """Checks that a list's tensors share one GPU and dtype; returns the dtype."""
     gpus = set(map(_gpus, tensors))
@@ -110,14 +121,14 @@ def _table(params, grads, avgs, seconds, avg_scales, second_scales, masters, bit
     none = [0] * n
     columns = [list(map(_ptrs, params)), None, list(map(_ptrs, avgs)), list(map(_ptrs, seconds)),
                none, none, none, sizes]
-    written = columns[0] + columns[2] + columns[3]
+    written = list(chain(params, avgs, seconds))
     if masters is not None:
         if pdtype == torch.float32:
             raise TypeError("adamw: masters of float32 parameters")
         _one(masters, "masters", index, torch.float32)
         _like_params(params, shapes, plain, masters, "a master")
         columns[6] = list(map(_ptrs, masters))
-        written += columns[6]
+        written += masters
     if bits == 8:
         blocks = [-(-k // BLOCK) for k in sizes]
         for at, ts in ((4, avg_scales), (5, second_scales)):
@@ -126,7 +137,7 @@ def _table(params, grads, avgs, seconds, avg_scales, second_scales, masters, bit
                 raise ValueError("adamw: a dense scale for each %d values of a parameter is wanted"
                                  % BLOCK)
             columns[at] = list(map(_ptrs, ts))
-        written += columns[4] + columns[5]
+        written += chain(avg_scales, second_scales)
     # gradients in their parameters' order
     if list(map(_shapes, grads)) != shapes:
         raise ValueError("adamw: a gradient's shape is not its parameter's")
@@ -134,10 +145,8 @@ def _table(params, grads, avgs, seconds, avg_scales, second_scales, masters, bit
         grads = [g if _same_order(p, g) else torch.empty_like(p, dtype=gdtype).copy_(g)
                  for p, g in zip(params, grads)]
     columns[1] = list(map(_ptrs, grads))
-    if 0 in sizes:                              # these have no address
-        written = [address for address in written if address]
-    if len(set(written)) != len(written):
-        raise ValueError("adamw: a tensor is in the lists twice")
+    if _overlap([(t.data_ptr(), t.nbytes) for t in written]):
+        raise ValueError("adamw: tensors in the lists share memory, or one is there twice")
     rows = array("Q", chain.from_iterable(zip(*columns))).tobytes()
     return index, _DTYPES[pdtype], _DTYPES[gdtype], rows, grads
 

@@ -512,7 +512,8 @@ int ganet_layer_norm_backward(const void *x, const void *weight, const void *gra
                               const ganet_layer_norm_params *p, void *workspace,
                               size_t workspace_bytes, ganet_stream_t stream);
 
-/* One tensor of an AdamW step: dense, `n` values, all device memory, all in the same order. */
+/* One tensor of an AdamW step: dense, `n` values, all device memory, all in the same order.  What is
+ * written overlaps nothing else of the list (`grad` may be the `param` of its row, in one type). */
 typedef struct {
   void *param;             /* param_dtype */
   const void *grad;        /* grad_dtype */

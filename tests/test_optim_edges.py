@@ -312,3 +312,38 @@ def test_a_refused_step_counts_nothing():
         assert torch.equal(late, torch.ones_like(late))
         # whatever was stepped has been counted, and what was not has not
         assert numbers(opt, [good, late]) == [int(not torch.equal(good, torch.ones_like(good))), 0]
+
+
+def test_overlaps():
+    inside = optim._overlap
+    assert not inside([]) and not inside([(100, 4)]) and not inside([(100, 4), (104, 4), (0, 100)])
+    assert inside([(100, 4), (100, 4)]) and inside([(100, 8), (104, 4)]) and inside([(104, 4), (96, 9)])
+    assert inside([(0, 1000), (10, 4), (500, 4)])
+    assert not inside([(100, 0), (100, 4)]) and not inside([(0, 0), (0, 0)])      # nothing in them
+
+
+@gpu
+def test_tensors_that_share_memory_are_refused():
+    """Views of one buffer that share some values: which step they would get is a matter of luck."""
+    flat = torch.zeros(4096, device="cuda")
+
+    def call(a, b, ma=None, mb=None):
+        zeros = [torch.zeros_like(a) for _ in range(6)]
+        optim.adamw_step([a, b], zeros[:2], [zeros[2] if ma is None else ma, zeros[3] if mb is None else mb],
+                         zeros[4:], 1)
+
+    call(flat[:100], flat[100:200])                                  # neighbours
+    with pytest.raises(ValueError, match="memory"):
+        call(flat[:100], flat[99:199])
+    with pytest.raises(ValueError, match="memory"):
+        call(flat[:100], flat[100:200], flat[150:250])
+    with pytest.raises(ValueError, match="memory"):
+        call(flat[:100].view(10, 10).t(), flat[50:150].view(10, 10).t())
+    call(flat[:100].view(10, 10).t(), flat[100:200].view(10, 10).t())
+    p = [flat[:512], flat[600:1112]]
+    st = [optim.state_8bit(t) for t in p]
+    scales = torch.zeros(3, device="cuda")
+    with pytest.raises(ValueError, match="memory"):
+        optim.adamw_step_8bit(p, [torch.zeros(512, device="cuda")] * 2, *([s[k] for s in st] for k in (0, 1)),
+                              [scales[:2], scales[1:]], [s[3] for s in st], 1)
+    assert not flat.any()
