@@ -8,10 +8,12 @@
 // else; Python then looks again, copies what can be copied and names what is wrong.
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
 #include <cstdint>
+#include <exception>
 #include <utility>
 #include <vector>
 
@@ -41,6 +43,12 @@ const at::Tensor *item(PyObject *list, Py_ssize_t i) {
 Py_ssize_t length(PyObject *list) {
   if (PyList_Check(list)) return PyList_GET_SIZE(list);
   return PyTuple_Check(list) ? PyTuple_GET_SIZE(list) : -1;
+}
+
+// The exception under way as Python's (torch.OutOfMemoryError stays one).
+PyObject *raised() {
+  torch::translate_exception_to_python(std::current_exception());
+  return nullptr;
 }
 
 PyObject *bytes(const void *p, size_t n) {
@@ -124,7 +132,7 @@ PyObject *step(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     Step s;
     if (!read(args, block, s)) Py_RETURN_NONE;
     return Py_BuildValue("iiiiN", s.gpu, s.param, s.grad, s.state == kE4M3 ? 8 : 32, bytes(s.rows.data(), s.rows.size() * 8));
-  } catch (const std::exception &) {   // a tensor without storage: Python's own reading names it
+  } catch (...) {   // a tensor without storage: Python's own reading names it
     PyErr_Clear();
     Py_RETURN_NONE;
   }
@@ -174,9 +182,8 @@ PyObject *adamw(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
       if (args[7] != Py_None) mark(args[7]);
     }
     return PyLong_FromLong(rc);
-  } catch (const std::exception &e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
+  } catch (...) {
+    return raised();
   }
 }
 
@@ -185,9 +192,8 @@ PyObject *written(PyObject *, PyObject *list) {
   try {
     mark(list);
     Py_RETURN_NONE;
-  } catch (const std::exception &e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
+  } catch (...) {
+    return raised();
   }
 }
 
@@ -224,7 +230,7 @@ PyObject *grads(PyObject *, PyObject *list) {
     const size_t n = g.size.size();
     return Py_BuildValue("iNNN", g.gpu, bytes(g.address.data(), n * 8), bytes(g.size.data(), n * 8),
                          bytes(g.type.data(), n * 4));
-  } catch (const std::exception &) {
+  } catch (...) {
     PyErr_Clear();
     Py_RETURN_NONE;
   }
@@ -323,9 +329,8 @@ PyObject *grad_norm(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
                          ws.data_ptr(), bytes, stream);
     if (rc) return PyLong_FromLong(rc);
     return wrapped(out);
-  } catch (const std::exception &e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
+  } catch (...) {
+    return raised();
   }
 }
 
@@ -362,9 +367,8 @@ PyObject *layer_norm_forward(PyObject *, PyObject *const *args, Py_ssize_t nargs
                          stats ? mean.data_ptr<float>() : nullptr, stats ? rstd.data_ptr<float>() : nullptr, &p, stream);
     if (rc) return PyLong_FromLong(rc);
     return Py_BuildValue("NNN", wrapped(y), wrapped(mean), wrapped(rstd));
-  } catch (const std::exception &e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
+  } catch (...) {
+    return raised();
   }
 }
 
@@ -410,9 +414,8 @@ PyObject *layer_norm_backward(PyObject *, PyObject *const *args, Py_ssize_t narg
                          out(gb), &p, out(ws), bytes, stream);
     if (rc) return PyLong_FromLong(rc);
     return Py_BuildValue("NNN", wrapped(gx), wrapped(gw), wrapped(gb));
-  } catch (const std::exception &e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
+  } catch (...) {
+    return raised();
   }
 }
 

@@ -347,3 +347,24 @@ def test_tensors_that_share_memory_are_refused():
         optim.adamw_step_8bit(p, [torch.zeros(512, device="cuda")] * 2, *([s[k] for s in st] for k in (0, 1)),
                               [scales[:2], scales[1:]], [s[3] for s in st], 1)
     assert not flat.any()
+
+
+@gpu
+def test_out_of_memory_keeps_its_type():
+    """Programs catch torch.OutOfMemoryError to try again with less."""
+    from ganet_amd import norm
+    g = torch.zeros(1 << 20, device="cuda")
+    x = torch.zeros(1 << 22, 64, device="cuda", dtype=torch.bfloat16)
+    y, mean, rstd = norm.layer_norm_forward(x[:64])
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(0).total_memory
+    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (1 << 25)) / total)
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            norm.layer_norm_forward(x)
+        with pytest.raises(torch.OutOfMemoryError):
+            norm.layer_norm(x)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert float(optim.grad_norm([g])[0]) == 0.0 and torch.equal(norm.layer_norm(x)[0], x[0])
