@@ -19,7 +19,7 @@ import ctypes
 
 import torch
 import torch.nn as nn
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -237,10 +237,8 @@ class LayerNormFunction(Function):
     def forward(ctx, input, weight, bias, eps, channel_dim):
         ctx.channel_dim = channel_dim
         ctx.bias_dtype = bias.dtype if bias is not None else None
-        out, mean, rstd = _forward(input, weight, bias, eps, channel_dim,
-                                   any(ctx.needs_input_grad))
-        if mean is not None:
-            ctx.save_for_backward(input, weight, mean, rstd)
+        out, mean, rstd = _forward(input, weight, bias, eps, channel_dim, True)
+        ctx.save_for_backward(input, weight, mean, rstd)
         return out
 
     @staticmethod
@@ -257,8 +255,13 @@ class LayerNormFunction(Function):
 
 
 def layer_norm(input, weight=None, bias=None, eps=1e-5, channel_dim=-1):
-    """Layer norm over `channel_dim` with gradients; see layer_norm_forward."""
-    return LayerNormFunction.apply(input, weight, bias, eps, channel_dim)
+    """Layer norm over `channel_dim` with gradients; see layer_norm_forward.  Where no backward can
+    follow (evaluation) mean and rstd are not written."""
+    if ((torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                         for t in (input, weight, bias)))
+            or forward_ad._current_level >= 0):           # has no forward derivative: autograd says so
+        return LayerNormFunction.apply(input, weight, bias, eps, channel_dim)
+    return _forward(input, weight, bias, eps, channel_dim, False)[0]
 
 
 class LayerNorm(nn.Module):
