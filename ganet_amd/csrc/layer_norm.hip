@@ -100,9 +100,25 @@ __device__ __forceinline__ float across_groups(float v) {
   return v;
 }
 
+// v[0] + ... + v[N - 1] in pairs, N a power of two
+template <int N>
+__device__ __forceinline__ float tree_sum(const float (&v)[N]) {
+  if constexpr (N == 1) {
+    return v[0];
+  } else {
+    float h[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) h[i] = v[i] + v[i + N / 2];
+    return tree_sum(h);
+  }
+}
+
 // ---------------------------------------------------------------------------------------------
 // Planes of any C: 64 positions a workgroup, the values read again for each pass
 // ---------------------------------------------------------------------------------------------
+// More than 1024 channels, or planes of fewer positions than a vector.  Bound by latency: one value a load and
+// three passes (4x2048x40x100: float32 forward 219 us, backward 641, bf16 234 and 465; the backward's two sums over a
+// wavefront for each channel and tile are the most of it).
 constexpr int kThreads = 256;
 
 // Planes: lane l of every wavefront owns position 64 * tile + l, the wavefronts share the channels.
@@ -119,32 +135,54 @@ __device__ __forceinline__ float positions_sum(float v, float (*part)[kTile]) {
   return v;
 }
 
+// A wavefront's channels, kAtOnce of them at once: f(i, c, in) for the i-th of each turn; past the last
+// `in` is false and c some channel, so that loads need no branch.  Sums are kept for each i by themselves:
+// a lane's sum is ceil(C / 64) terms in order and then a tree (all of its C / 4 in order, 16384 equal terms
+// lost 2^-14 of a mean).
+constexpr int kAtOnce = 16;
+constexpr int kWaves = kThreads / 64;
+template <typename F>
+__device__ __forceinline__ void channels_of_wave(int C, F &&f) {
+  for (int c0 = (int)threadIdx.x >> 6; c0 < C; c0 += kAtOnce * kWaves)
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int c = c0 + i * kWaves;
+      f(i, c < C ? c : c0, c < C);
+    }
+}
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void ln_planes_any_fwd(Args a) {
-  __shared__ float part[kThreads / 64][kTile];
+  __shared__ float part[kWaves][kTile];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long long tiles = (a.inner + kTile - 1) / kTile;
   for (long long i = blockIdx.x; i < a.outer * tiles; i += gridDim.x) {
-    const long long b = i / tiles, pos = (i % tiles) * kTile + lane;
-    const bool in = pos < a.inner;
+    const long long b = i / tiles, at = (i % tiles) * kTile + lane;
+    const bool valid = at < a.inner;
+    const long long pos = valid ? at : a.inner - 1;
     const T *x = (const T *)a.x + b * a.xs + pos;
     T *y = (T *)a.y + b * a.ys + pos;
-    float s = 0.0f;
-    for (int c = wave; c < a.C; c += kThreads / 64)
-      if (in) s += load1(x + c * a.inner);
-    const float mean = positions_sum(s, part) / a.c;
-    s = 0.0f;
-    for (int c = wave; c < a.C; c += kThreads / 64)
-      if (in) {
-        const float d = load1(x + c * a.inner) - mean;
-        s += d * d;
-      }
-    const float rstd = 1.0f / sqrtf(positions_sum(s, part) * a.inv_c + a.eps);
-    for (int c = wave; c < a.C; c += kThreads / 64)
-      if (in)
+    float s[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) s[k] = 0.0f;
+    channels_of_wave(a.C, [&](int k, int c, bool in) {
+      const float v = load1(x + c * a.inner);
+      s[k] += in ? v : 0.0f;
+    });
+    const float mean = positions_sum(tree_sum(s), part) / a.c;
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) s[k] = 0.0f;
+    channels_of_wave(a.C, [&](int k, int c, bool in) {
+      const float d = load1(x + c * a.inner) - mean;
+      s[k] += in ? d * d : 0.0f;
+    });
+    const float rstd = 1.0f / sqrtf(positions_sum(tree_sum(s), part) * a.inv_c + a.eps);
+    if (valid)
+#pragma unroll 4
+      for (int c = wave; c < a.C; c += kWaves)
         store1(y + c * a.inner, (load1(x + c * a.inner) - mean) * rstd * load_weight(a.w, a.wdtype, c, 1.0f) +
                                     load_weight(a.b, a.wdtype, c, 0.0f));
-    if (in && wave == 0 && a.mean) {
+    if (valid && wave == 0 && a.mean) {
       a.mean[b * a.inner + pos] = mean;
       a.rstd[b * a.inner + pos] = rstd;
     }
@@ -153,41 +191,43 @@ __global__ __launch_bounds__(kThreads) void ln_planes_any_fwd(Args a) {
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void ln_planes_any_bwd(Args a) {
-  __shared__ float part[kThreads / 64][kTile];
-  extern __shared__ float sums[];               // [2][C]: a wavefront's own channels
+  __shared__ float part[kWaves][kTile];
+  extern __shared__ float sums[];               // [2][C]: a wavefront's own channels; 128 KiB at most
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (a.partial)
     for (int c = threadIdx.x; c < 2 * a.C; c += kThreads) sums[c] = 0.0f;
   __syncthreads();
   const long long tiles = (a.inner + kTile - 1) / kTile;
   for (long long i = blockIdx.x; i < a.outer * tiles; i += gridDim.x) {
-    const long long b = i / tiles, pos = (i % tiles) * kTile + lane;
-    const bool in = pos < a.inner;
+    const long long b = i / tiles, at = (i % tiles) * kTile + lane;
+    const bool valid = at < a.inner;
+    const long long pos = valid ? at : a.inner - 1;
     const T *x = (const T *)a.x + b * a.xs + pos;
     const T *g = (const T *)a.g + b * a.gs + pos;
     T *dx = (T *)a.y + b * a.ys + pos;
-    const float mean = in ? a.mean[b * a.inner + pos] : 0.0f;
-    const float rstd = in ? a.rstd[b * a.inner + pos] : 0.0f;
-    float s1 = 0.0f, s2 = 0.0f;
-    for (int c = wave; c < a.C; c += kThreads / 64) {
-      const float xh = in ? (load1(x + c * a.inner) - mean) * rstd : 0.0f;
-      const float dy = in ? load1(g + c * a.inner) : 0.0f;
+    const float mean = a.mean[b * a.inner + pos], rstd = a.rstd[b * a.inner + pos];
+    float s1[kAtOnce], s2[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) s1[k] = s2[k] = 0.0f;
+    channels_of_wave(a.C, [&](int k, int c, bool in) {
+      const float xh = (load1(x + c * a.inner) - mean) * rstd, dy = load1(g + c * a.inner);
       const float wa = dy * load_weight(a.w, a.wdtype, c, 1.0f);
-      s1 += wa;
-      s2 += wa * xh;
-      if (a.partial) {
-        const float dw = group_sum<64>(dy * xh), db = group_sum<64>(dy);
+      s1[k] += in ? wa : 0.0f;
+      s2[k] += in ? wa * xh : 0.0f;
+      if (a.partial && in) {                    // a position past the last counts for nothing
+        const float dw = group_sum<64>(valid ? dy * xh : 0.0f), db = group_sum<64>(valid ? dy : 0.0f);
         if (lane == 0) {
           sums[c] += dw;
           sums[a.C + c] += db;
         }
       }
-    }
+    });
     if (!a.y) continue;
-    const float m1 = positions_sum(s1, part) * a.inv_c;
-    const float m2 = positions_sum(s2, part) * a.inv_c;
-    for (int c = wave; c < a.C; c += kThreads / 64)
-      if (in) {
+    const float m1 = positions_sum(tree_sum(s1), part) * a.inv_c;
+    const float m2 = positions_sum(tree_sum(s2), part) * a.inv_c;
+    if (valid)
+#pragma unroll 4
+      for (int c = wave; c < a.C; c += kWaves) {
         const float xh = (load1(x + c * a.inner) - mean) * rstd;
         const float wa = load1(g + c * a.inner) * load_weight(a.w, a.wdtype, c, 1.0f);
         store1(dx + c * a.inner, rstd * (wa - m1 - xh * m2));
@@ -564,11 +604,11 @@ __device__ __forceinline__ void slots_sum(float (&s)[M], float (*part)[64][M / 4
   }
   ganet_vec::lds_barrier();
 #pragma unroll
-  for (int i = 0; i < Q; ++i) s[i] = part[0][lane][i];
+  for (int i = 0; i < Q; ++i) s[i] = WAVES > 1 ? part[0][lane][i] + part[WAVES > 1][lane][i] : part[0][lane][i];
 #pragma unroll
-  for (int w = 1; w < WAVES; ++w)
+  for (int w = 2; w < WAVES; w += 2)                   // two wavefronts at once: half as many sums in order
 #pragma unroll
-    for (int i = 0; i < Q; ++i) s[i] += part[w][lane][i];
+    for (int i = 0; i < Q; ++i) s[i] += part[w][lane][i] + part[w + 1][lane][i];
 #pragma unroll
   for (int i = 0; i < Q; ++i) {
     s[i + Q] = s[i];
@@ -634,21 +674,21 @@ __global__ __launch_bounds__(64 * WAVES) void ln_planes_fwd(Args a, int tiles, i
 #pragma unroll
   for (int j = 0; j < N; ++j) mean[j] = rstd[j] = 0.0f;
 #pragma unroll
-  for (int k = 0; k < NC; ++k)
+  for (int k = 0; k < NC; k += 2)                    // two channels at once: half as many sums in order
 #pragma unroll
-    for (int j = 0; j < N; ++j) mean[j] += v[k].get(j);
+    for (int j = 0; j < N; ++j) mean[j] += v[k].get(j) + v[k + 1].get(j);
   slots_sum<N, WAVES>(mean, part[0]);                // its barrier also covers the weights
 #pragma unroll
   for (int k = 0; k < NC; ++k) v[k].forget();
 #pragma unroll
   for (int j = 0; j < N; ++j) mean[j] /= a.c;
 #pragma unroll
-  for (int k = 0; k < NC; ++k) {
-    const bool in = k < nc && c0 + k < a.C;
+  for (int k = 0; k < NC; k += 2) {
+    const bool in0 = k < nc && c0 + k < a.C, in1 = k + 1 < nc && c0 + k + 1 < a.C;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const float d = in ? v[k].get(j) - mean[j] : 0.0f;
-      rstd[j] += d * d;
+      const float d0 = in0 ? v[k].get(j) - mean[j] : 0.0f, d1 = in1 ? v[k + 1].get(j) - mean[j] : 0.0f;
+      rstd[j] += d0 * d0 + d1 * d1;
     }
   }
   slots_sum<N, WAVES>(rstd, part[1]);

@@ -45,3 +45,29 @@ def test_evaluation_gives_the_same_values():
     assert torch.equal(y, z) and torch.equal(y, i)
     m.requires_grad_(False)
     assert not m(x).requires_grad and torch.equal(m(x), y)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", [(1, 8193, 3, 5), (2, 16384, 2, 3), (1, 16384, 1, 2)])
+def test_widest_maps(shape, dtype):
+    """All channels that are accepted: two float32 sums a channel take 128 KiB of LDS."""
+    both(*make(shape, 1, dtype, torch.float32, offset=40.0), 1)
+    both(*make(shape, 1, dtype, dtype, offset=0.5), 1)
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(1, 1100, 3, 9), (1, 16384, 3, 5), (2, 64, 1, 3)])
+def test_sums_over_many_channels(shape):
+    """Terms whose sum is rounded the same way again and again: from 2048 on a term of
+    1 + 2^-13 - 2^-23 loses 2^-13 each time it is added by itself.  A lane that adds C / 4 terms in order is off by
+    some 1000 u of the mean, past the bound of chain(C)."""
+    term = 1 + 2.0 ** -13 - 2.0 ** -23
+    g = torch.full(shape, term, device="cuda")
+    x = torch.randn(shape, device="cuda")
+    w = torch.ones(shape[1], device="cuda")
+    for v in (x, g):
+        y, mean, rstd = norm.layer_norm_forward(v, w, w, channel_dim=1)
+        check_forward(v, w, w, 1e-5, 1, y, mean, rstd)
+    y, mean, rstd = norm.layer_norm_forward(x, w, w, channel_dim=1)
+    check_backward(x, w, g, mean, rstd, 1, *norm.layer_norm_backward(x, w, g, mean, rstd, 1))
