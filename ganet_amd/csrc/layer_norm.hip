@@ -5,11 +5,16 @@
 //   dx = rstd (a - mean_C(a) - xh mean_C(a xh)),  dw = sum dy xh,  db = sum dy.
 //
 // The variance is formed from (x - mean), a second pass over the values: sums of squares would lose
-// it where the mean is large.  Everything between the loads and the one rounding of each output is
+// it where the mean is large.  Where the first sum is rounded even over equal values (kRounded), that pass also
+// adds up d = x - mean, which is small: mean += sum d / C, var = sum d^2 / C - (sum d / C)^2.  The mean is then
+// right to a rounding of its own, and equal values have no variance (without it a row of 96 times 15538.596
+// came out as 0.3 instead of 0).  Everything between the loads and the one rounding of each output is
 // float32.  dw and db: every workgroup keeps sums of its own and leaves them in the workspace, a
 // second launch adds them in a fixed order; few positions are added in the first (no atomics: the same
 // inputs give the same bits).
 #include <math.h>
+
+#include <type_traits>
 
 #include "vec_device.h"
 
@@ -40,6 +45,26 @@ __device__ __forceinline__ float load_weight(const void *w, int dtype, int c, fl
   if (dtype == GANET_BF16)
     return ganet_vec::Elem<bf16_t>::widen(((const GANET_GLOBAL unsigned short *)w)[c]);
   return (float)((const GANET_GLOBAL _Float16 *)w)[c];
+}
+
+// Whether a float32 sum of equal values may be rounded: those of up to 16384 bfloat16 values (8 bits each) and
+// of up to 8192 float16 ones (11 bits) are exact.
+template <typename T>
+constexpr bool kRounded = sizeof(T) == 4;
+
+// The mean of c values from the sums of two halves.  Where each half is exact (float16), so is the mean of
+// equal values: what the sum of the halves and the division round off goes back in.
+__device__ __forceinline__ float mean_of_halves(float a, float b, float c) {
+  const float s = a + b, back = s - a, lost = (a - (s - back)) + (b - back);
+  const float m = s / c;
+  return m + (fmaf(-m, c, s) + lost) / c;
+}
+
+// The corrected mean and 1 / deviation from the sums of d and d^2.
+__device__ __forceinline__ void correct(float sum, float squares, const Args &a, float &mean, float &rstd) {
+  const float more = sum / a.c, var = squares * a.inv_c - more * more;
+  mean += more;
+  rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + a.eps);
 }
 
 template <typename T>
@@ -124,15 +149,22 @@ constexpr int kThreads = 256;
 // Planes: lane l of every wavefront owns position 64 * tile + l, the wavefronts share the channels.
 constexpr int kTile = 64;
 
-__device__ __forceinline__ float positions_sum(float v, float (*part)[kTile]) {
+// The sums of the first and the second two wavefronts.
+struct Halves {
+  float a, b;
+};
+__device__ __forceinline__ Halves positions_halves(float v, float (*part)[kTile]) {
+  static_assert(kThreads / 64 == 4, "two halves of two");
   const int lane = threadIdx.x & 63;
   part[threadIdx.x >> 6][lane] = v;
   __syncthreads();
-  v = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kThreads / 64; ++i) v += part[i][lane];
+  const Halves h = {part[0][lane] + part[1][lane], part[2][lane] + part[3][lane]};
   __syncthreads();
-  return v;
+  return h;
+}
+__device__ __forceinline__ float positions_sum(float v, float (*part)[kTile]) {
+  const Halves h = positions_halves(v, part);
+  return h.a + h.b;
 }
 
 // A wavefront's channels, kAtOnce of them at once: f(i, c, in) for the i-th of each turn; past the last
@@ -169,14 +201,22 @@ __global__ __launch_bounds__(kThreads) void ln_planes_any_fwd(Args a) {
       const float v = load1(x + c * a.inner);
       s[k] += in ? v : 0.0f;
     });
-    const float mean = positions_sum(tree_sum(s), part) / a.c;
+    const Halves sum = positions_halves(tree_sum(s), part);
+    float mean = mean_of_halves(sum.a, sum.b, a.c), rstd;
+    constexpr bool AGAIN = kRounded<T>;
+    float more[kAtOnce];
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) s[k] = 0.0f;
+    for (int k = 0; k < kAtOnce; ++k) s[k] = more[k] = 0.0f;
     channels_of_wave(a.C, [&](int k, int c, bool in) {
       const float d = load1(x + c * a.inner) - mean;
       s[k] += in ? d * d : 0.0f;
+      if constexpr (AGAIN) more[k] += in ? d : 0.0f;
     });
-    const float rstd = 1.0f / sqrtf(positions_sum(tree_sum(s), part) * a.inv_c + a.eps);
+    const float squares = positions_sum(tree_sum(s), part);
+    if constexpr (AGAIN)
+      correct(positions_sum(tree_sum(more), part), squares, a, mean, rstd);
+    else
+      rstd = 1.0f / sqrtf(squares * a.inv_c + a.eps);
     if (valid)
 #pragma unroll 4
       for (int c = wave; c < a.C; c += kWaves)
@@ -255,15 +295,46 @@ __device__ __forceinline__ float row_sum(float v, float *part, int slot) {
   if constexpr (LANES <= 64) {
     return group_sum<LANES>(v);
   } else {
-    // `part` holds two sets of one float a wavefront; calls alternate, so one barrier a call does
+    // `part` holds a set of one float a wavefront for each slot; neighbouring calls use unlike ones, so one
+    // barrier a call does
     constexpr int W = LANES / 64;
     v = group_sum<64>(v);
     if ((threadIdx.x & 63) == 0) part[slot * W + (threadIdx.x >> 6)] = v;
     ganet_vec::lds_barrier();
-    v = 0.0f;
-#pragma unroll
-    for (int i = 0; i < W; ++i) v += part[slot * W + i];
-    return v;
+    return group_sum<W>(part[slot * W + (threadIdx.x & (W - 1))]);
+  }
+}
+// Two sums over one barrier, in slots 1 and 2.
+template <int LANES>
+__device__ __forceinline__ void row_sums(float &v, float &w, float *part) {
+  if constexpr (LANES <= 64) {
+    v = group_sum<LANES>(v);
+    w = group_sum<LANES>(w);
+  } else {
+    constexpr int W = LANES / 64;
+    v = group_sum<64>(v);
+    w = group_sum<64>(w);
+    if ((threadIdx.x & 63) == 0) {
+      part[W + (threadIdx.x >> 6)] = v;
+      part[2 * W + (threadIdx.x >> 6)] = w;
+    }
+    ganet_vec::lds_barrier();
+    v = group_sum<W>(part[W + (threadIdx.x & (W - 1))]);
+    w = group_sum<W>(part[2 * W + (threadIdx.x & (W - 1))]);
+  }
+}
+// The mean of a row from its lanes' sums.
+template <typename T, int LANES>
+__device__ __forceinline__ float row_mean(float v, float *part, float c) {
+  if constexpr (std::is_same<T, f16_t>::value && LANES == 512) {          // more than 8192 columns
+    constexpr int W = LANES / 64;
+    v = group_sum<64>(v);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    ganet_vec::lds_barrier();
+    const float half = group_sum<W / 2>(part[threadIdx.x & (W - 1)]);
+    return mean_of_halves(half, ganet_vec::dpp<0x141>(half), c);          // mirrored in eight lanes: the other one
+  } else {
+    return row_sum<LANES>(v, part, 0) / c;
   }
 }
 
@@ -274,7 +345,8 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_rows_fwd(Args a)
   constexpr int N = kN<T>;
   constexpr int THREADS = LANES > 256 ? LANES : 256;
   constexpr int ROWS = THREADS / LANES;              // of a workgroup at once
-  __shared__ float part[2 * (LANES > 64 ? LANES / 64 : 1)];
+  constexpr bool AGAIN = kRounded<T>;
+  __shared__ float part[(AGAIN ? 3 : 2) * (LANES > 64 ? LANES / 64 : 1)];
   const int l = (int)threadIdx.x % LANES;
   const long long row0 = (long long)blockIdx.x * (ROWS * R) + (int)threadIdx.x / LANES;
   Vec<T, N> x[R][NV];
@@ -305,7 +377,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_rows_fwd(Args a)
     for (int v = 0; v < NV; ++v)
 #pragma unroll
       for (int k = 0; k < N; ++k) s += x[r][v].get(k);
-    const float mean = row_sum<LANES>(s, part, 0) / a.c;      // exact for equal values
+    float mean = row_mean<T, LANES>(s, part, a.c), rstd, more = 0.0f;
     s = 0.0f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -313,11 +385,17 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_rows_fwd(Args a)
       const int left = a.C - (v * LANES + l) * N;
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        const float d = x[r][v].get(k) - mean;
-        s += k < left ? d * d : 0.0f;
+        const float d = k < left ? x[r][v].get(k) - mean : 0.0f;
+        s += d * d;
+        if constexpr (AGAIN) more += d;
       }
     }
-    const float rstd = 1.0f / sqrtf(row_sum<LANES>(s, part, 1) * a.inv_c + a.eps);
+    if constexpr (AGAIN) {
+      row_sums<LANES>(s, more, part);
+      correct(more, s, a, mean, rstd);
+    } else {
+      rstd = 1.0f / sqrtf(row_sum<LANES>(s, part, 1) * a.inv_c + a.eps);
+    }
     if (row >= a.outer) continue;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -649,7 +727,9 @@ template <typename T, int VB, int NC, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void ln_planes_fwd(Args a, int tiles, int nc) {
   typedef Plane<T, VB, NC, WAVES> P;
   constexpr int N = P::N;
-  __shared__ __align__(16) float part[2][WAVES][64][N / 4];
+  constexpr bool AGAIN = kRounded<T>;
+  constexpr int M = AGAIN ? 2 * N : N;               // sums of the second pass: of d^2, and of d
+  __shared__ __align__(16) float part0[WAVES][64][N / 4], part1[WAVES][64][M / 4];
   __shared__ float weights[2][P::SLOTS * NC];
   int own;
   const Share share((unsigned)a.outer * (unsigned)tiles, gridDim.x);
@@ -670,14 +750,16 @@ __global__ __launch_bounds__(64 * WAVES) void ln_planes_fwd(Args a, int tiles, i
     weights[0][c] = load_weight(a.w, a.wdtype, c, 1.0f);
     weights[1][c] = load_weight(a.b, a.wdtype, c, 0.0f);
   }
-  float mean[N], rstd[N];
+  float mean[N], rstd[M];
 #pragma unroll
-  for (int j = 0; j < N; ++j) mean[j] = rstd[j] = 0.0f;
+  for (int j = 0; j < N; ++j) mean[j] = 0.0f;
+#pragma unroll
+  for (int j = 0; j < M; ++j) rstd[j] = 0.0f;
 #pragma unroll
   for (int k = 0; k < NC; k += 2)                    // two channels at once: half as many sums in order
 #pragma unroll
     for (int j = 0; j < N; ++j) mean[j] += v[k].get(j) + v[k + 1].get(j);
-  slots_sum<N, WAVES>(mean, part[0]);                // its barrier also covers the weights
+  slots_sum<N, WAVES>(mean, part0);                  // its barrier also covers the weights
 #pragma unroll
   for (int k = 0; k < NC; ++k) v[k].forget();
 #pragma unroll
@@ -689,13 +771,19 @@ __global__ __launch_bounds__(64 * WAVES) void ln_planes_fwd(Args a, int tiles, i
     for (int j = 0; j < N; ++j) {
       const float d0 = in0 ? v[k].get(j) - mean[j] : 0.0f, d1 = in1 ? v[k + 1].get(j) - mean[j] : 0.0f;
       rstd[j] += d0 * d0 + d1 * d1;
+      if constexpr (AGAIN) rstd[N + j] += d0 + d1;
     }
   }
-  slots_sum<N, WAVES>(rstd, part[1]);
+  slots_sum<M, WAVES>(rstd, part1);
 #pragma unroll
   for (int k = 0; k < NC; ++k) v[k].forget();
 #pragma unroll
-  for (int j = 0; j < N; ++j) rstd[j] = 1.0f / sqrtf(rstd[j] * a.inv_c + a.eps);
+  for (int j = 0; j < N; ++j) {
+    if constexpr (AGAIN)
+      correct(rstd[N + j], rstd[j], a, mean[j], rstd[j]);
+    else
+      rstd[j] = 1.0f / sqrtf(rstd[j] * a.inv_c + a.eps);
+  }
   T *y = (T *)a.y + img * a.ys + (long long)c0 * a.inner + pos;
 #pragma unroll
   for (int k = 0; k < NC; ++k) {
@@ -950,7 +1038,8 @@ int with_type(int dtype, F &&f) {
 // Rows: the narrowest of these that holds C, i.e. LANES * NV vectors of 16 bytes.  Forward: a
 // wavefront a row while two vectors a lane do; then four vectors a lane rather than more wavefronts at
 // the barriers for 16-bit values (2048 rows of 16384: 512 lanes of four 33 us, 1024 of two 39 us),
-// the other way round for float32 (8192 rows of 4096: 256 lanes of four 54 us, 1024 of one 48 us).
+// two vectors a lane for float32 (8192 rows of 4096: 512 lanes of two 49 us, 256 of four 58, 1024 of one 54;
+// 12000 of 2500: 52, 54 and 63 us).
 // Backward: one vector a lane as long as possible, the registers hold the columns' sums and the next
 // row (16384 rows of 4096 bf16: 512 lanes of one 70 us, 256 of two, without the next row, 76 us).
 template <bool BACKWARD, typename T, typename F>
@@ -978,7 +1067,11 @@ int with_row_shape(int C, F &&f) {
     GANET_ROW(256, 4);
     GANET_ROW(512, 4);
   } else {
-    GANET_ROW(1024, 1);
+    if constexpr (BACKWARD) {
+      GANET_ROW(1024, 1);
+    } else {
+      GANET_ROW(512, 2);
+    }
     GANET_ROW(1024, 2);
     if constexpr (sizeof(T) == 4) GANET_ROW(1024, 4);
   }

@@ -71,3 +71,47 @@ def test_sums_over_many_channels(shape):
         check_forward(v, w, w, 1e-5, 1, y, mean, rstd)
     y, mean, rstd = norm.layer_norm_forward(x, w, w, channel_dim=1)
     check_backward(x, w, g, mean, rstd, 1, *norm.layer_norm_backward(x, w, g, mean, rstd, 1))
+
+
+EQUAL = [0.1, 15538.596, -1.0 / 3, 1e6 / 7, -3e-20]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape,dim", [((5, 96), -1), ((3, 777), -1), ((600, 64), -1), ((2, 3001), -1),
+                                       ((2, 9001), -1), ((2, 16383), -1), ((2, 12, 3, 3), 1),
+                                       ((1, 256, 10, 25), 1), ((1, 1000, 4, 33), 1), ((1, 1100, 3, 9), 1),
+                                       ((2, 9001, 1, 3), 1)])
+def test_equal_values_have_no_variance(shape, dim, dtype):
+    """y is the bias and the mean the value itself, whatever the value: the sum of equal float32
+    values is rounded, their mean is not.  The variance is the difference of two numbers below
+    e^2, e = (chain + 4) u |x| the error of a first mean, each off by relative (chain + 4) u or twice
+    that, so it is (3 chain + 12) u e^2 at most."""
+    C = shape[dim]
+    wide = [1] * len(shape)
+    wide[dim] = C
+    w, b = torch.rand(C, device="cuda") + 0.5, torch.randn(C, device="cuda")
+    for value in EQUAL:
+        x = torch.full(shape, value, device="cuda").to(dtype)
+        if not torch.isfinite(x).all():                             # past float16
+            continue
+        y, mean, rstd = norm.layer_norm_forward(x, w, b, channel_dim=dim)
+        exact = x.flatten()[0].float()
+        assert (mean == exact).all(), value
+        assert torch.equal(y, b.to(dtype).reshape(wide).expand(shape)), value
+        k = chain(C)
+        var = (3 * k + 12) * U * ((k + 4) * U * float(exact)) ** 2
+        assert ((rstd.double() / 1e-5 ** -0.5 - 1).abs() <= 4 * U + var / 1e-5).all(), value
+
+
+@gpu
+@pytest.mark.parametrize("shape,dim", [((40, 320), -1), ((9, 5000), -1), ((3, 40, 9, 7), 1),
+                                       ((1, 1100, 3, 9), 1)])
+def test_mean_of_values_far_from_zero(shape, dim):
+    """Values around 3e5 that differ by about one: the mean is off by a rounding, not by one a term."""
+    x, w, b, _ = make(shape, dim, torch.float32, torch.float32, offset=3e5)
+    y, mean, rstd = norm.layer_norm_forward(x, w, b, channel_dim=dim)
+    check_forward(x, w, b, 1e-5, dim, y, mean, rstd)
+    X = as_rows(x, dim)
+    off = (mean.double() - X.mean(1)).abs()
+    assert (off <= 2 * U * X.abs().amax(1)).all()
