@@ -115,3 +115,14 @@ def test_mean_of_values_far_from_zero(shape, dim):
     X = as_rows(x, dim)
     off = (mean.double() - X.mean(1)).abs()
     assert (off <= 2 * U * X.abs().amax(1)).all()
+
+
+@gpu
+def test_mean_of_values_around_zero():
+    """A sum of C independent values of deviation 1 goes through some 16 levels of partial sums; the C / n sums
+    of n values of a level are each off by a rounding of sqrt(n), u sqrt(n) at most and independent, so a level
+    adds u sqrt(C) to the deviation of the sum: the mean's is u sqrt(16 / C) at most."""
+    C = 4096
+    x = make((2000, C), -1, torch.float32, torch.float32, offset=0.0)[0] / 1.3
+    mean = norm.layer_norm_forward(x)[1]
+    assert float((mean.double() - x.double().mean(1)).abs().mean()) <= U * (16 / C) ** 0.5
