@@ -292,14 +292,14 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(Args8<MASTER> a) {
     um = ur = 0;
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
-      const unsigned cm = vm >> (8 * j) & 0x7F, cr = vr >> (8 * j) & 0x7F;
-      if (sq[j] == INFINITY || (cr == 0x7F && cm != 0x7F)) nr[j] = INFINITY;
+      // (a NaN of its root by a finite m can only come from r's code)
       const unsigned mb = __float_as_uint(nm[j]) & 0x7FFFFFFFu, rb = __float_as_uint(nr[j]);
-      if (mb >= kInf || rb > kInf)
+      if (mb >= kInf) {
         bad |= 1u << j;
-      else if (rb == kInf)
+      } else if (rb >= kInf) {
         held |= 1u << j;
-      else {
+        nr[j] = INFINITY;
+      } else {
         if (mb > um) um = mb;
         if (rb > ur) ur = rb;
       }
