@@ -403,6 +403,30 @@ class AdamW(torch.optim.Optimizer):
         if capturing:
             self._captured.update((id(sts[0]["step"]), sts[0]["step"]) for sts in now.values())
 
+    def _call(self, calls, grad_stats, counters):
+        """The raw calls of a step.  What has been stepped is counted; its numbers on the device leave
+        `counters`."""
+        place = 0                                 # 8-bit tensors of the calls before
+        for key, (group, ps, gs, st) in calls.items():
+            common = dict(lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                          weight_decay=group["weight_decay"], grad_stats=grad_stats,
+                          masters=[s["master"] for s in st] if key[5] else None,
+                          skip_nonfinite=self.skip_nonfinite)
+            number = st[0]["step"] if self.capturable else key[6] + 1
+            if key[4]:
+                adamw_step_8bit(ps, gs, [s["exp_avg"] for s in st], [s["exp_rms"] for s in st],
+                                [s["avg_scale"] for s in st], [s["rms_scale"] for s in st],
+                                number, seed=self.seed + place * _PLACE, **common)
+                place += len(ps)
+            else:
+                adamw_step(ps, gs, [s["exp_avg"] for s in st], [s["exp_avg_sq"] for s in st],
+                           number, **common)
+            if self.capturable:
+                counters.pop(key[6], None)
+            else:
+                for s in st:
+                    s["step"] = number
+
     @torch.no_grad()
     def step(self, closure=None, grad_stats=None):
         loss = None
@@ -457,24 +481,12 @@ class AdamW(torch.optim.Optimizer):
             call[3].append(st)
         for t in counters.values():
             t.add_(1)
-        place = 0                             # 8-bit tensors of the calls before
-        for key, (group, ps, gs, st) in calls.items():
-            common = dict(lr=group["lr"], betas=group["betas"], eps=group["eps"],
-                          weight_decay=group["weight_decay"], grad_stats=grad_stats,
-                          masters=[s["master"] for s in st] if key[5] else None,
-                          skip_nonfinite=self.skip_nonfinite)
-            number = st[0]["step"] if self.capturable else key[6] + 1
-            if key[4]:
-                adamw_step_8bit(ps, gs, [s["exp_avg"] for s in st], [s["exp_rms"] for s in st],
-                                [s["avg_scale"] for s in st], [s["rms_scale"] for s in st],
-                                number, seed=self.seed + place * _PLACE, **common)
-                place += len(ps)
-            else:
-                adamw_step(ps, gs, [s["exp_avg"] for s in st], [s["exp_avg_sq"] for s in st],
-                           number, **common)
-            if not self.capturable:               # a call that is refused has stepped nothing
-                for s in st:
-                    s["step"] = number
+        try:
+            self._call(calls, grad_stats, counters)
+        except Exception:
+            for t in counters.values():           # of what has not been stepped
+                t.sub_(1)
+            raise
         return loss
 
     def load_state_dict(self, state_dict):

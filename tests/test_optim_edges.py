@@ -313,6 +313,14 @@ def test_a_refused_step_counts_nothing():
         # whatever was stepped has been counted, and what was not has not
         assert numbers(opt, [good, late]) == [int(not torch.equal(good, torch.ones_like(good))), 0]
 
+        before = numbers(opt, [good, late])
+        opt.param_groups[1]["lr"] = torch.tensor(1e-4)              # on the host: not taken
+        for _ in range(2):
+            opt.param_groups[0]["lr"] = torch.tensor(1e-3)
+            with pytest.raises(ValueError):
+                opt.step()
+        assert numbers(opt, [good, late]) == before
+
 
 def test_overlaps():
     inside = optim._overlap
