@@ -526,6 +526,9 @@ _SCALES = dict(exp_avg="avg_scale", exp_rms="rms_scale")      # of the states in
 
 def _values_like(p, value):
     """A copy of a state's values in the parameter's memory order."""
+    if value.shape != p.shape:
+        raise ValueError("AdamW: a saved state of shape %s for a parameter of shape %s"
+                         % (tuple(value.shape), tuple(p.shape)))
     return torch.empty_like(p, dtype=value.dtype).copy_(value.detach())
 
 
@@ -537,7 +540,7 @@ def _codes_like(p, codes, scale, root):
     scale = scale.to(p.device, copy=True)
     if _same_order(p, codes):
         return codes, scale
-    if not _dense(codes) or not _dense(p):
+    if codes.shape != p.shape or not _dense(codes) or not _dense(p):
         raise ValueError("AdamW: a saved state of shape %s and strides %s for a parameter of shape %s and "
                          "strides %s" % (tuple(codes.shape), codes.stride(), tuple(p.shape), p.stride()))
     n = p.numel()

@@ -376,3 +376,15 @@ def test_out_of_memory_keeps_its_type():
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0)
     assert float(optim.grad_norm([g])[0]) == 0.0 and torch.equal(norm.layer_norm(x)[0], x[0])
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_states_of_another_shape_are_refused(bits):
+    """A state of one value would have been spread over all."""
+    one, many = (torch.nn.Parameter(torch.ones(n, 5, device="cuda")) for n in (1, 9))
+    a, b = (optim.AdamW([p], state_bits=bits, min_8bit_size=1) for p in (one, many))
+    one.grad = torch.ones_like(one)
+    a.step()
+    with pytest.raises(ValueError):
+        b.load_state_dict(a.state_dict())
