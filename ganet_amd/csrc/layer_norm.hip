@@ -64,7 +64,9 @@ __device__ __forceinline__ float mean_of_halves(float a, float b, float c) {
 // is rounded to x's spacing, which is more than the first sum lost (rows of 4096 normal values: 4 times as far
 // off with `more`).
 __device__ __forceinline__ void correct(float sum, float squares, const Args &a, float &mean, float &rstd) {
-  const float more = sum / a.c, left = squares * a.inv_c - more * more, var = left < 0.0f ? 0.0f : left;
+  const float more = sum / a.c, all = squares * a.inv_c, left = all - more * more;
+  // (no number where both are past the largest float32)
+  const float var = left > 0.0f ? left : (left <= 0.0f ? 0.0f : all);
   if (mean * mean > var) mean += more;
   rstd = 1.0f / sqrtf(var + a.eps);
 }

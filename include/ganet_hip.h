@@ -536,10 +536,10 @@ typedef struct {
  * (largest magnitude / 448), rounded up or down at random: the random word of a value is a
  * hash of (seed, t, the tensor's place in the list, the value's place in it), so the same
  * inputs give the same bits.  A list that goes on in another call, k tensors later, goes on with
- * the words of one list if its seed is seed + k * 0x85EBCA6B (modulo 2^32).  The parameter's step uses m and v before that rounding.  A
- * v under 2^-126 counts as zero there, and the divisor is 2^-64 at least.  A v past the largest
- * float32 is infinite in 8 bits as it is in 32 (the value stands still from then on): its code in
- * `second` is e4m3's NaN, over an exp_avg that is none. */
+ * the words of one list if its seed is seed + k * 0x85EBCA6B (modulo 2^32).  The parameter's step
+ * uses m and v before that rounding.  A v under 2^-126 counts as zero there, and the divisor is
+ * 2^-64 at least.  A v past the largest float32 is infinite in 8 bits as it is in 32 (the value
+ * stands still from then on): its code in `second` is e4m3's NaN, over an exp_avg that is none. */
 typedef struct {
   int32_t param_dtype, grad_dtype; /* ganet_dtype */
   int32_t state_bits;              /* 32 or 8 */

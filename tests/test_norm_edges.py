@@ -126,3 +126,19 @@ def test_mean_of_values_around_zero():
     x = make((2000, C), -1, torch.float32, torch.float32, offset=0.0)[0] / 1.3
     mean = norm.layer_norm_forward(x)[1]
     assert float((mean.double() - x.double().mean(1)).abs().mean()) <= U * (16 / C) ** 0.5
+
+
+@gpu
+@pytest.mark.parametrize("shape,dim", [((5, 96), -1), ((2, 3001), -1), ((2, 12, 3, 3), 1),
+                                       ((1, 1100, 3, 9), 1)])
+def test_values_whose_squares_overflow(shape, dim):
+    """A deviation past the largest root counts as infinite, and y is the bias: also where the rounding of
+    a mean is such a deviation."""
+    C = shape[dim]
+    wide = [1] * len(shape)
+    wide[dim] = C
+    w, b = torch.rand(C, device="cuda") + 0.5, torch.randn(C, device="cuda")
+    for x in (torch.full(shape, 1.1e30, device="cuda"), torch.full(shape, 1.3e34, device="cuda"),
+              torch.randn(shape, device="cuda") * 1e25, torch.randn(shape, device="cuda") * 1e25 + 1e32):
+        y = norm.layer_norm_forward(x, w, b, channel_dim=dim)[0]
+        assert torch.equal(y, b.reshape(wide).expand(shape))
